@@ -12,10 +12,10 @@ _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libhachiue_cuda.so")
 
 HCU_OK, HCU_EINVAL, HCU_ECUDA, HCU_ENCCL, HCU_ETIMEDOUT, HCU_ENOMEM, HCU_EUNSUPPORTED = range(7)
-KV_F32, KV_F16, KV_BF16, KV_Q8_0, KV_Q8_0_WGSL = 0, 1, 2, 3, 4
+KV_F32, KV_F16, KV_BF16, KV_Q8_0, KV_Q8_0_WGSL, KV_Q4_0 = 0, 1, 2, 3, 4, 5
 OPT_ATTN_CUDA_CORES, OPT_ATTN_CHUNK, OPT_GDN_SCRATCH_MB, OPT_SWA_CTAS, OPT_GDN_CHAIN_COLS = 1, 2, 3, 4, 5
 COMM_ID_BYTES = 128
-DT_F32, DT_BF16 = 0, 2
+DT_F32, DT_F16, DT_BF16 = 0, 1, 2
 
 STATUS_NAMES = {
     HCU_OK: "HCU_OK", HCU_EINVAL: "HCU_EINVAL", HCU_ECUDA: "HCU_ECUDA", HCU_ENCCL: "HCU_ENCCL",
@@ -33,6 +33,7 @@ EXPORTS = (
     "hcu_rmsnorm", "hcu_rope", "hcu_split_q_gate", "hcu_sigmoid_gate", "hcu_attn_prologue",
     "hcu_selftest_dirty_tickets", "hcu_attention_noalloc_status", "hcu_set_q8_convention", "hcu_set_option",
     "hcu_comm_unique_id", "hcu_comm_init_rank", "hcu_kv_append_rows_kv",
+    "hcu_rope_append_paged", "hcu_read_paged", "hcu_attention_paged", "hcu_prefill_varlen",
 )
 
 
@@ -96,6 +97,32 @@ class hcu_gdn_prefill_params(ctypes.Structure):
                 ("v_row_stride", ctypes.c_uint64), ("q_seq_stride", ctypes.c_uint64),
                 ("k_seq_stride", ctypes.c_uint64), ("v_seq_stride", ctypes.c_uint64),
                 ("gb_row_stride", ctypes.c_uint64), ("gb_seq_stride", ctypes.c_uint64)]
+
+
+class hcu_paged_kv(ctypes.Structure):
+    _fields_ = [("format", ctypes.c_uint32), ("page_size", ctypes.c_uint32), ("n_pages", ctypes.c_uint32),
+                ("KV", ctypes.c_uint32), ("Dh", ctypes.c_uint32), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p)]
+
+
+class hcu_rope_append_params(ctypes.Structure):
+    _fields_ = [("n", ctypes.c_uint32), ("H", ctypes.c_uint32), ("dtype", ctypes.c_uint32),
+                ("rotaryDim", ctypes.c_uint32), ("table_rows", ctypes.c_uint32), ("q_row_stride", ctypes.c_uint64),
+                ("k_row_stride", ctypes.c_uint64), ("v_row_stride", ctypes.c_uint64)]
+
+
+class hcu_attention_paged_params(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_uint32), ("S", ctypes.c_uint32), ("H", ctypes.c_uint32),
+                ("windowSize", ctypes.c_uint32), ("dtype", ctypes.c_uint32), ("max_context", ctypes.c_uint32),
+                ("table_stride", ctypes.c_uint32), ("block_table", ctypes.c_void_p), ("context", ctypes.c_void_p)]
+
+
+class hcu_prefill_varlen_params(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_uint32), ("H", ctypes.c_uint32), ("KV", ctypes.c_uint32), ("D", ctypes.c_uint32),
+                ("window", ctypes.c_uint32), ("dtype", ctypes.c_uint32), ("total_q", ctypes.c_uint32),
+                ("total_k", ctypes.c_uint32), ("cu_q", ctypes.c_void_p), ("cu_k", ctypes.c_void_p),
+                ("q_row_stride", ctypes.c_uint64), ("k_row_stride", ctypes.c_uint64),
+                ("v_row_stride", ctypes.c_uint64)]
 
 
 _lock = threading.Lock()
@@ -164,6 +191,12 @@ def load(path: str | None = None):
             "hcu_comm_unique_id": ([ctypes.POINTER(ctypes.c_uint8)], i32),
             "hcu_comm_init_rank": ([i32, i32, ctypes.POINTER(ctypes.c_uint8), i32, i32, ctypes.POINTER(vp)], i32),
             "hcu_kv_append_rows_kv": ([vp, u32, u32, u32, vp, vp, vp, ctypes.POINTER(hcu_kv_cache)], i32),
+            "hcu_rope_append_paged": ([vp, ctypes.POINTER(hcu_rope_append_params)] + [vp] * 9
+                                      + [ctypes.POINTER(hcu_paged_kv)], i32),
+            "hcu_read_paged": ([vp, u32, u32, vp, ctypes.POINTER(hcu_paged_kv), vp, vp], i32),
+            "hcu_attention_paged": ([vp, ctypes.POINTER(hcu_attention_paged_params), vp, ctypes.POINTER(hcu_paged_kv),
+                                     vp], i32),
+            "hcu_prefill_varlen": ([vp, ctypes.POINTER(hcu_prefill_varlen_params), vp, vp, vp, vp], i32),
         }
         for name, (args, res) in sig.items():
             fn = getattr(L, name)

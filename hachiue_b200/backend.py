@@ -21,10 +21,10 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from ._lib import (DT_BF16, DT_F32, KV_BF16, KV_F16, KV_F32, KV_Q8_0, KV_Q8_0_WGSL, HachiueError, check,
-                   hcu_attention_params,
+from ._lib import (DT_BF16, DT_F16, DT_F32, KV_BF16, KV_F16, KV_F32, KV_Q4_0, KV_Q8_0, KV_Q8_0_WGSL, HachiueError, check,
+                   hcu_attention_paged_params, hcu_attention_params,
                    hcu_attn_prologue_params, hcu_conv1d_params, hcu_deltanet_params, hcu_gdn_prefill_params, hcu_gdn_step_params, hcu_kv_cache,
-                   hcu_swa_params)
+                   hcu_paged_kv, hcu_prefill_varlen_params, hcu_rope_append_params, hcu_swa_params)
 
 # The reference's op names on this path (src/kernels.ts SHADERS keys).
 SHADERS = ("kv_append_q8", "attention_q8", "deltanet_gbeta", "deltanet_recur", "conv1d_causal", "deltanet_norm_gate",
@@ -32,6 +32,7 @@ SHADERS = ("kv_append_q8", "attention_q8", "deltanet_gbeta", "deltanet_recur", "
 
 _DTYPE_OF_FORMAT = {KV_F32: torch.float32, KV_F16: torch.float16, KV_BF16: torch.bfloat16, KV_Q8_0: torch.int8,
                     KV_Q8_0_WGSL: torch.int8}
+_DT = {torch.float32: DT_F32, torch.float16: DT_F16, torch.bfloat16: DT_BF16}
 _OPTIONS = {"attn_cuda_cores": _lib.OPT_ATTN_CUDA_CORES, "attn_chunk": _lib.OPT_ATTN_CHUNK,
             "gdn_scratch_mb": _lib.OPT_GDN_SCRATCH_MB, "swa_ctas": _lib.OPT_SWA_CTAS,
             "gdn_chain_cols": _lib.OPT_GDN_CHAIN_COLS}
@@ -91,6 +92,59 @@ class KVCache:
         if cached is None or cached[0] != key:
             cached = (key, hcu_kv_cache(self.fmt, self.rows, _ptr(self.k), _ptr(self.v), _ptr(self.k_scale),
                                         _ptr(self.v_scale)))
+            self.__dict__["_c_struct"] = cached
+        return cached[1]
+
+
+@dataclass
+class PagedKVCache:
+    """One layer's paged 4-bit KV cache (hcu_paged_kv, format ``KV_Q4_0``):
+    k and v uint8 [n_pages, KV, page_size, Dh / 2] and their f16 scales
+    [n_pages, KV, page_size, Dh / 32].  Slot ``page * page_size + offset`` names
+    a token row."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+    @staticmethod
+    def allocate(n_pages: int, page_size: int, kv_heads: int, head_dim: int, device="cuda") -> "PagedKVCache":
+        k = torch.zeros((n_pages, kv_heads, page_size, head_dim // 2), dtype=torch.uint8, device=device)
+        ks = torch.zeros((n_pages, kv_heads, page_size, head_dim // 32), dtype=torch.float16, device=device)
+        return PagedKVCache(k, torch.zeros_like(k), ks, torch.zeros_like(ks))
+
+    @property
+    def n_pages(self) -> int:
+        return self.k.shape[0]
+
+    @property
+    def kv_heads(self) -> int:
+        return self.k.shape[1]
+
+    @property
+    def page_size(self) -> int:
+        return self.k.shape[2]
+
+    @property
+    def head_dim(self) -> int:
+        return self.k.shape[3] * 2
+
+    def c_struct(self) -> hcu_paged_kv:
+        """The C view of the cache, checked and rebuilt only when a tensor
+        changed (a decode step calls this once per layer)."""
+        key = (self.k, self.v, self.k_scale, self.v_scale)
+        cached = self.__dict__.get("_c_struct")
+        # the tensors themselves are compared, not their addresses, which a freed cache's successor can have
+        if cached is None or any(a is not b for a, b in zip(cached[0], key)) or cached[2] != self.k.data_ptr():
+            shape, scales = tuple(self.k.shape), (*self.k.shape[:3], self.k.shape[3] // 16)
+            if (len(shape) != 4 or self.v.shape != self.k.shape or any(tuple(t.shape) != scales for t in key[2:])
+                    or any(t.dtype != torch.uint8 for t in key[:2]) or any(t.dtype != torch.float16 for t in key[2:])
+                    or any(not t.is_contiguous() or t.device != self.k.device for t in key)):
+                raise HachiueError(_lib.HCU_EINVAL,
+                                   "hachiue: a paged cache is contiguous uint8 k / v [n_pages, KV, page_size, Dh / 2] and "
+                                   "f16 scales [n_pages, KV, page_size, Dh / 32] on one device")
+            st = hcu_paged_kv(KV_Q4_0, shape[2], shape[0], shape[1], 2 * shape[3], *(_ptr(t) for t in key))
+            cached = (key, st, self.k.data_ptr())
             self.__dict__["_c_struct"] = cached
         return cached[1]
 
@@ -410,3 +464,146 @@ class CudaBackend:
             return
         check(self.lib.hcu_deltanet_chunked_prefill(self._h, ctypes.byref(p), _ptr(q), _ptr(k), _ptr(v), _ptr(g),
                                                     _ptr(beta), _ptr(state_in), _ptr(core), _ptr(state_out)))
+
+    # -- paged serving ---------------------------------------------------------
+    def _on_device(self, op: str, *tensors: torch.Tensor) -> None:
+        """Refuses tensors of another device than the handle's."""
+        for t in tensors:
+            if t.device != self.device:
+                raise HachiueError(_lib.HCU_EINVAL, f"hachiue: {op}: a tensor is on {t.device}, the handle on {self.device}")
+
+    def rope_append_paged(self, k: torch.Tensor, v: torch.Tensor, cache: PagedKVCache, slots: torch.Tensor,
+                          cos: torch.Tensor | None = None, sin: torch.Tensor | None = None,
+                          positions: torch.Tensor | None = None, q: torch.Tensor | None = None,
+                          q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None) -> None:
+        """Rotate keys (and queries) and append keys and values to the 4-bit
+        pages: k, v [n, KV, Dh] and q [n, H, Dh] of one dtype (f32, f16 or bf16;
+        token-major views with contiguous heads are accepted), cos / sin f32
+        [positions, rotary_dim / 2], positions int32 [n], slots int64 [n]
+        (negative: padding, skipped).  q_out and k_out (optional) receive the
+        rotated rows; without cos / sin nothing is rotated."""
+        kv = cache.c_struct()
+        n, KV, Dh = k.shape
+        H = 0 if q is None else q.shape[1]
+        self._on_device("rope_append_paged", cache.k, k, v, slots)
+        if (v.shape != k.shape or KV != kv.KV or Dh != kv.Dh or k.dtype not in _DT or v.dtype != k.dtype
+                or slots.dtype != torch.int64 or slots.shape != (n,) or not slots.is_contiguous()):
+            raise HachiueError(_lib.HCU_EINVAL, f"hachiue: rope_append_paged takes k / v [n, {kv.KV}, {kv.Dh}] of one float dtype "
+                                                "and contiguous int64 slots [n]")
+        rotary = 0
+        if cos is not None:
+            rotary = 2 * cos.shape[-1]
+            if sin is None or positions is None:
+                raise HachiueError(_lib.HCU_EINVAL, "hachiue: rope_append_paged: a rotation needs cos, sin and positions")
+            self._on_device("rope_append_paged", cos, sin, positions)
+            if (cos.dim() != 2 or sin.shape != cos.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32
+                    or not cos.is_contiguous() or not sin.is_contiguous() or positions.dtype != torch.int32
+                    or positions.shape != (n,) or not positions.is_contiguous()):
+                raise HachiueError(_lib.HCU_EINVAL, "hachiue: rope_append_paged takes contiguous f32 cos / sin "
+                                                    "[positions, rotary_dim / 2] and int32 positions [n]")
+        elif sin is not None:
+            raise HachiueError(_lib.HCU_EINVAL, "hachiue: rope_append_paged: sin without cos")
+        if (q is None) != (q_out is None):
+            raise HachiueError(_lib.HCU_EINVAL, "hachiue: rope_append_paged: q and q_out go together")
+        rows = [k, v]
+        if q is not None:
+            self._on_device("rope_append_paged", q, q_out)
+            if (q.shape != (n, H, Dh) or q.dtype != k.dtype or q_out.shape != q.shape or q_out.dtype != k.dtype
+                    or not q_out.is_contiguous()):
+                raise HachiueError(_lib.HCU_EINVAL, "hachiue: rope_append_paged takes q and a contiguous q_out [n, H, Dh] "
+                                                    "of k's dtype")
+            rows.append(q)
+        if k_out is not None:
+            self._on_device("rope_append_paged", k_out)
+            if k_out.shape != k.shape or k_out.dtype != k.dtype or not k_out.is_contiguous():
+                raise HachiueError(_lib.HCU_EINVAL, "hachiue: rope_append_paged takes a contiguous k_out like k")
+        for t in rows:
+            if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != Dh):
+                raise HachiueError(_lib.HCU_EINVAL, "hachiue: rope_append_paged: heads must be contiguous")
+        if n == 0:
+            return
+        self._bind_stream()
+        p = hcu_rope_append_params(n, H, _DT[k.dtype], rotary, 0 if cos is None else cos.shape[0],
+                                   0 if q is None else self._row_stride(q), self._row_stride(k), self._row_stride(v))
+        check(self.lib.hcu_rope_append_paged(self._h, ctypes.byref(p), _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(cos),
+                                             _ptr(sin), _ptr(positions), slots.data_ptr(), _ptr(q_out), _ptr(k_out),
+                                             ctypes.byref(kv)))
+
+    @staticmethod
+    def _row_stride(t: torch.Tensor) -> int:
+        """Elements between the token rows of t [n, heads, D] (0, dense, for a single row)."""
+        return t.stride(0) if t.shape[0] > 1 else 0
+
+    def read_paged(self, cache: PagedKVCache, slots: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor) -> None:
+        """The values of cached rows: k_out, v_out [n, KV, Dh] (f32, f16 or
+        bf16, contiguous) receive rows slots[i] (int64 [n]; negative: left as it was)."""
+        kv = cache.c_struct()
+        n = slots.shape[0]
+        self._on_device("read_paged", cache.k, slots, k_out, v_out)
+        if (slots.dtype != torch.int64 or slots.dim() != 1 or not slots.is_contiguous() or k_out.shape != (n, kv.KV, kv.Dh)
+                or v_out.shape != k_out.shape or k_out.dtype not in _DT or v_out.dtype != k_out.dtype
+                or not k_out.is_contiguous() or not v_out.is_contiguous()):
+            raise HachiueError(_lib.HCU_EINVAL, f"hachiue: read_paged takes contiguous int64 slots [n] and contiguous outputs "
+                                                f"[n, {kv.KV}, {kv.Dh}] of one float dtype")
+        if n == 0:
+            return
+        self._bind_stream()
+        check(self.lib.hcu_read_paged(self._h, n, _DT[k_out.dtype], slots.data_ptr(), ctypes.byref(kv), k_out.data_ptr(),
+                                      v_out.data_ptr()))
+
+    def attention_paged(self, q: torch.Tensor, cache: PagedKVCache, out: torch.Tensor, block_table: torch.Tensor,
+                        context: torch.Tensor, max_context: int = 0, window_size: int = 0) -> None:
+        """Decode attention of q [B, S, H, Dh] over the 4-bit pages into out
+        (like q; f32, f16 or bf16): block_table int32 [B, pages], context int32
+        [B] tokens per sequence, this call's S included.  ``max_context`` is an
+        upper bound of context (0: what the table can hold; a near one lets
+        the split of the key axis fit the call)."""
+        kv = cache.c_struct()
+        self._on_device("attention_paged", cache.k, q, out, block_table, context)
+        if (q.dim() != 4 or q.shape[3] != kv.Dh or q.dtype not in _DT or out.shape != q.shape or out.dtype != q.dtype
+                or not q.is_contiguous() or not out.is_contiguous()):
+            raise HachiueError(_lib.HCU_EINVAL, f"hachiue: attention_paged takes contiguous q and out [B, S, H, {kv.Dh}] of one "
+                                                "float dtype")
+        B, S, H = q.shape[:3]
+        if (block_table.dtype != torch.int32 or context.dtype != torch.int32 or block_table.dim() != 2
+                or block_table.shape[0] != B or context.shape != (B,) or not block_table.is_contiguous()
+                or not context.is_contiguous()):
+            raise HachiueError(_lib.HCU_EINVAL, "hachiue: attention_paged takes contiguous int32 block_table [B, pages] and "
+                                                "context [B]")
+        if B == 0 or S == 0:
+            return
+        pages = block_table.shape[1]
+        self._bind_stream()
+        p = hcu_attention_paged_params(B, S, H, window_size, _DT[q.dtype], max_context or pages * kv.page_size, pages,
+                                       block_table.data_ptr(), context.data_ptr())
+        check(self.lib.hcu_attention_paged(self._h, ctypes.byref(p), q.data_ptr(), ctypes.byref(kv), out.data_ptr()))
+
+    def prefill_varlen(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor,
+                       cu_k: torch.Tensor | None = None, window: int = 0) -> None:
+        """Causal attention over packed prompts: q [total_q, H, 128], k / v
+        [total_k, KV, 128] (bf16 or f16; token-major views with contiguous heads
+        are accepted), out [total_q, H, 128] contiguous; cu_q, cu_k int32
+        [B + 1] offsets of the sequences (cu_k None: the same).  With more
+        keys than queries the queries are the last tokens; window 0 = causal."""
+        self._on_device("prefill_varlen", q, k, v, out, cu_q)
+        if cu_k is not None:
+            self._on_device("prefill_varlen", cu_k)
+        nq, H, D = q.shape
+        nk, KV = k.shape[:2]
+        if (q.dtype not in (torch.bfloat16, torch.float16) or any(t.dtype != q.dtype for t in (k, v, out))
+                or k.shape != (nk, KV, D) or v.shape != k.shape or out.shape != q.shape or not out.is_contiguous()):
+            raise HachiueError(_lib.HCU_EINVAL, "hachiue: prefill_varlen takes q and a contiguous out [total_q, H, D] and "
+                                                "k / v [total_k, KV, D], all bf16 or all f16")
+        for t in (q, k, v):
+            if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != D):
+                raise HachiueError(_lib.HCU_EINVAL, "hachiue: prefill_varlen: heads must be contiguous")
+        for t in (cu_q, cu_k if cu_k is not None else cu_q):
+            if t.dtype != torch.int32 or t.dim() != 1 or t.shape != cu_q.shape or t.shape[0] < 1 or not t.is_contiguous():
+                raise HachiueError(_lib.HCU_EINVAL, "hachiue: prefill_varlen takes contiguous int32 offsets [B + 1]")
+        if nq == 0 or cu_q.shape[0] == 1:
+            return
+        self._bind_stream()
+        p = hcu_prefill_varlen_params(cu_q.shape[0] - 1, H, KV, D, window, _DT[q.dtype], nq, nk, cu_q.data_ptr(),
+                                      _ptr(cu_k), self._row_stride(q), self._row_stride(k), self._row_stride(v))
+        check(self.lib.hcu_prefill_varlen(self._h, ctypes.byref(p), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                          out.data_ptr()))

@@ -64,6 +64,16 @@ int once_per_device(std::atomic<uint64_t>& done, int device, F&& set) {
 // stream (queued work may still read the old buffer) and reallocates.
 int ensure_scratch(hcu_context* h, size_t bytes, const char* what);
 
+// Restores the calling thread's current CUDA device when it goes out of scope:
+// an op on a handle of another device leaves the caller's device as it was.
+struct DeviceScope {
+  int device = -1;
+  DeviceScope() { if (cudaGetDevice(&device) != cudaSuccess) device = -1; }
+  ~DeviceScope() { if (device >= 0) cudaSetDevice(device); }
+  DeviceScope(const DeviceScope&) = delete;
+  DeviceScope& operator=(const DeviceScope&) = delete;
+};
+
 // Encodes a tiled TMA descriptor (row-major tensor, dims innermost first).
 int make_tensor_map(CUtensorMap* map, CUtensorMapDataType dtype, int rank, void* base,
                     const uint64_t* dims, const uint64_t* strides_bytes /* rank-1 */,

@@ -1,0 +1,76 @@
+// paged.cuh - the paged 4-bit KV cache (hcu_paged_kv, HCU_KV_Q4_0) as its
+// append, read and attention kernels see it, and the activation types.
+#pragma once
+
+#include "common.cuh"
+#include "context.h"
+
+namespace hcu {
+
+// Four consecutive elements of an activation row, as f32 (16 or 8 bytes of memory).
+__device__ __forceinline__ void load4(const float* p, float (&x)[4]) {
+  const float4 v = *reinterpret_cast<const float4*>(p);
+  x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+}
+__device__ __forceinline__ void load4(const __half* p, float (&x)[4]) {
+  const uint2 v = *reinterpret_cast<const uint2*>(p);
+  const float2 a = f16x2_to_f2(v.x), b = f16x2_to_f2(v.y);
+  x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+}
+__device__ __forceinline__ void load4(const __nv_bfloat16* p, float (&x)[4]) {
+  const uint2 v = *reinterpret_cast<const uint2*>(p);
+  x[0] = bf16_lo(v.x), x[1] = bf16_hi(v.x), x[2] = bf16_lo(v.y), x[3] = bf16_hi(v.y);
+}
+__device__ __forceinline__ void store4(float* p, const float (&x)[4]) {
+  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+}
+__device__ __forceinline__ void store4(__half* p, const float (&x)[4]) {
+  const __half2 a = __floats2half2_rn(x[0], x[1]), b = __floats2half2_rn(x[2], x[3]);
+  *reinterpret_cast<uint2*>(p) =
+      make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+__device__ __forceinline__ void store4(__nv_bfloat16* p, const float (&x)[4]) {
+  const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
+  *reinterpret_cast<uint2*>(p) =
+      make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+
+// The device view of an hcu_paged_kv.
+struct PagedKV {
+  uint8_t* k;
+  uint8_t* v;
+  __half* ks;
+  __half* vs;
+  int page_log2, n_pages, KV;
+};
+
+// Row index of `offset` in page `page` for KV head g (rows of Dh / 2 code bytes, Dh / 32 scales).
+__device__ __forceinline__ long long paged_row(const PagedKV& c, long long page, int g, int offset) {
+  return ((page * c.KV + g) << c.page_log2) + offset;
+}
+
+// Checks the cache's geometry and fills the device view (host).
+inline int check_paged(const char* op, const hcu_paged_kv* kv, PagedKV* out) {
+  if (!kv) return fail(HCU_EINVAL, "%s: null cache", op);
+  if (kv->format != HCU_KV_Q4_0) return fail(HCU_EUNSUPPORTED, "%s: paged cache format %u (built: HCU_KV_Q4_0)", op, kv->format);
+  if (kv->page_size < 16 || kv->page_size > 256 || (kv->page_size & (kv->page_size - 1)))
+    return fail(HCU_EINVAL, "%s: page_size (%u) must be 16, 32, 64, 128 or 256", op, kv->page_size);
+  if (kv->n_pages == 0 || kv->KV == 0) return fail(HCU_EINVAL, "%s: n_pages and KV must be positive", op);
+  if (kv->n_pages > 0x7fffffffu || kv->KV > 65535u) return fail(HCU_EINVAL, "%s: n_pages or KV too large", op);
+  if (kv->Dh != 128 && kv->Dh != 256) return fail(HCU_EUNSUPPORTED, "%s: Dh=%u (built: 128, 256)", op, kv->Dh);
+  if (!kv->k || !kv->v || !kv->k_scale || !kv->v_scale) return fail(HCU_EINVAL, "%s: null cache buffer", op);
+  if ((reinterpret_cast<uintptr_t>(kv->k) | reinterpret_cast<uintptr_t>(kv->v) |
+       reinterpret_cast<uintptr_t>(kv->k_scale) | reinterpret_cast<uintptr_t>(kv->v_scale)) % 16)
+    return fail(HCU_EINVAL, "%s: cache buffers must be 16-byte aligned", op);
+  int lg = 4;
+  while ((1u << lg) < kv->page_size) lg++;
+  *out = PagedKV{static_cast<uint8_t*>(kv->k),       static_cast<uint8_t*>(kv->v),
+                 static_cast<__half*>(kv->k_scale),  static_cast<__half*>(kv->v_scale),
+                 lg,                                 (int)kv->n_pages,
+                 (int)kv->KV};
+  return HCU_OK;
+}
+
+inline int dtype_bytes(uint32_t dt) { return dt == HCU_DT_F32 ? 4 : (dt == HCU_DT_F16 || dt == HCU_DT_BF16) ? 2 : 0; }
+
+}  // namespace hcu

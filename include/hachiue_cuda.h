@@ -63,9 +63,18 @@ extern "C" {
  * hold the same int8 values up to the rounding rule (WGSL round() is
  * half-to-even in f32, the JS Math.round half-up in f64). */
 #define HCU_KV_Q8_0_WGSL 4
+/* 4-bit blocks of 32 elements, the format of a paged cache (hcu_paged_kv,
+ * which says how rows and pages are laid out).  Of a block x, m is the element
+ * of the largest magnitude (the first of equals); its scale is
+ * d = f16(m / -8), held within +-65504, the code of an element is
+ * floor(x / d + 8.5) held within 0..15 (8 where d is 0), found exactly, and the
+ * element then stands for (code - 8) * d. */
+#define HCU_KV_Q4_0 5
 
-/* Element types of the tensor-core prefill inputs and outputs. */
+/* Element types of activations: the tensor-core prefill inputs and outputs,
+ * and the paged ops' queries, keys, values and outputs. */
 #define HCU_DT_F32 0
+#define HCU_DT_F16 1
 #define HCU_DT_BF16 2
 
 typedef struct hcu_context *hcu_handle;
@@ -521,6 +530,120 @@ int hcu_deltanet_chunked_prefill_snap(hcu_handle h, const hcu_gdn_prefill_params
                                       const void *k, const void *v, const float *g, const float *beta,
                                       const float *state_in, float *core, float *state_out,
                                       uint32_t snap_every, float *snapshots);
+
+/* ------------------------------------------------------------------------ */
+/* Paged serving: a 4-bit cache in pages, packed prompts                      */
+/* ------------------------------------------------------------------------ */
+
+/* The paged ops have no counterpart in the reference, which keeps one
+ * contiguous cache for one sequence (src/engine.ts:483-492).
+ *
+ * A paged KV cache of one attention layer.  Token rows live in pages of
+ * page_size rows (a power of two, 16..256) that any sequence may hold; slot
+ * page * page_size + offset names a row.  Page p holds, for each KV head g,
+ * page_size rows of Dh / 2 bytes of k and v at row index
+ * (p * KV + g) * page_size + offset, and Dh / 32 f16 scales in k_scale and
+ * v_scale at the same row index (so the rows of a head lie together in a
+ * page).  With nb = Dh / 32 blocks, the 4-bit codes of a row are held in the
+ * order in which the attention's registers take them:
+ *   k: 32-bit word t * nb + b (t = 0..3) holds dimensions 32b + 8t .. + 7,
+ *   v: 16-bit halfword g * nb + b (g = 0..7) holds dimensions 32b + 4g .. + 3,
+ * the lowest dimension in the lowest four bits.  k and v are 16-byte aligned,
+ * the scales too.  Dh 128 or 256.  Rows that no slot names are never looked
+ * at, whatever they hold. */
+typedef struct {
+  uint32_t format;     /* HCU_KV_Q4_0 */
+  uint32_t page_size;  /* token rows of a page: 16, 32, 64, 128 or 256 */
+  uint32_t n_pages, KV, Dh;
+  void *k, *v;             /* device, [n_pages, KV, page_size, Dh / 2] bytes */
+  void *k_scale, *v_scale; /* device, [n_pages, KV, page_size, Dh / 32] f16 */
+} hcu_paged_kv;
+
+/* Rotates and appends n tokens: row i of k is rotated at positions[i] (pairs
+ * (j, j + rotaryDim / 2), tables cos / sin f32 [table_rows, rotaryDim / 2]:
+ * y1 = x1 * c - x2 * s, y2 = x2 * c + x1 * s, in f64 and rounded to f32, as
+ * hcu_rope does), and it and row i of v go to slot slots[i] of the cache.
+ * Row i of k_out (optional) receives the rotated key and row i of q_out the
+ * rotated query (in f32 arithmetic), so that a prefill can follow without
+ * another pass.  rotaryDim 0 rotates nothing (cos, sin and positions may be
+ * NULL).  q [n, H, Dh] (H = 0 and NULL: no queries), k and v [n, KV, Dh] of
+ * `dtype`, rows at the given strides in elements (0 = dense: views of one fused
+ * projection have its width), k_out and q_out dense, of the same type; q_out
+ * may be a dense q itself and k_out a dense k (in place).  rotaryDim is a
+ * multiple of 8, at most Dh.  Row pointers and strides are multiples of four
+ * elements.
+ *
+ * A negative slot marks padding: nothing of that row is read but its slot, and
+ * nothing is written.  A slot past the cache or a position outside the tables
+ * sets bit 2 of the device status and is skipped the same way.  The slots of
+ * one call must differ: a row named twice holds parts of both tokens. */
+typedef struct {
+  uint32_t n, H, dtype, rotaryDim, table_rows;
+  uint64_t q_row_stride, k_row_stride, v_row_stride;
+} hcu_rope_append_params;
+
+int hcu_rope_append_paged(hcu_handle h, const hcu_rope_append_params *p, const void *q, const void *k, const void *v,
+                          const float *cos_tab, const float *sin_tab, const int32_t *positions,
+                          const int64_t *slots, void *q_out, void *k_out, const hcu_paged_kv *kv);
+
+/* Gathers cached rows: k_out and v_out [n, KV, Dh] of `dtype` receive the
+ * values that slot slots[i]'s row stands for, rounded once (a shared prefix
+ * as dense keys and values for hcu_prefill_varlen).  A slot may be named more
+ * than once.  A negative slot leaves its output rows as they were, a slot past
+ * the cache does too and sets bit 2 of the device status. */
+int hcu_read_paged(hcu_handle h, uint32_t n, uint32_t dtype, const int64_t *slots, const hcu_paged_kv *kv,
+                   void *k_out, void *v_out);
+
+/* Decode attention over the paged cache: sequence b holds context[b] tokens
+ * (those of this call included), token j at row j % page_size of page
+ * block_table[b * table_stride + j / page_size].  Its S queries are its last S
+ * tokens: query i sits at position pos = context[b] - S + i and sees tokens
+ * max(0, pos + 1 - windowSize) .. pos (windowSize 0: from 0), scale
+ * 1 / sqrt(Dh), grouped heads as in hcu_attention.  A query that sees no token
+ * (context[b] < S - i, an empty sequence) gives zeros.  q and out
+ * [batch, S, H, Dh] of `dtype`.
+ *
+ * max_context >= every context[b] (the host plans the split of the key axis
+ * with it); a longer sequence sets bit 2 of the device status and its outputs
+ * are zeros.  A page index outside the cache sets bit 2 too and that page's
+ * tokens are left out; only the pages that hold visible tokens are looked up.
+ * f32 outputs keep f32 accuracy; bf16 and f16 ones are rounded once. */
+typedef struct {
+  uint32_t batch, S, H, windowSize, dtype, max_context;
+  uint32_t table_stride;      /* block_table entries per sequence */
+  const int32_t *block_table; /* device [batch, table_stride] */
+  const int32_t *context;     /* device [batch] */
+} hcu_attention_paged_params;
+
+int hcu_attention_paged(hcu_handle h, const hcu_attention_paged_params *p, const void *q, const hcu_paged_kv *kv,
+                        void *out);
+
+/* Causal attention over packed prompts of different lengths: the queries of
+ * sequence b are rows cu_q[b] .. cu_q[b + 1] - 1 of q, its keys and values rows
+ * cu_k[b] .. cu_k[b + 1] - 1 of k and v (cu_k NULL: cu_q).  With Lq queries and
+ * Lk keys, query i sits at position pos = Lk - Lq + i (a prefix of Lk - Lq
+ * cached tokens comes first) and sees keys max(0, pos + 1 - window) .. pos
+ * (window 0: from 0), scale 1 / sqrt(D), kvh = h / (H / KV).  A query that sees
+ * no key (Lk < Lq) gives zeros.  q [total_q, H, D], k and v [total_k, KV, D] of
+ * `dtype` (HCU_DT_BF16 or HCU_DT_F16), rows at the given strides in elements
+ * (0 = dense), a multiple of 8; out [total_q, H, D] dense, of the same type.
+ * D = 128.  Tensor cores, f32 accumulation; the probabilities are rounded to
+ * `dtype` for their product with the values.
+ *
+ * Rows of out that no sequence covers are left as they were, and rows of k and
+ * v outside a sequence have no influence on it, whatever they hold.  The
+ * offsets must not decrease and must lie within the totals: a sequence whose
+ * offsets do not is skipped and sets bit 2 of the device status. */
+typedef struct {
+  uint32_t batch, H, KV, D, window, dtype;
+  uint32_t total_q, total_k;
+  const int32_t *cu_q;  /* device [batch + 1] */
+  const int32_t *cu_k;  /* device [batch + 1] or NULL */
+  uint64_t q_row_stride, k_row_stride, v_row_stride;
+} hcu_prefill_varlen_params;
+
+int hcu_prefill_varlen(hcu_handle h, const hcu_prefill_varlen_params *p, const void *q, const void *k, const void *v,
+                       void *out);
 
 #ifdef __cplusplus
 }
