@@ -47,10 +47,11 @@ struct PagedAttnArgs {
   PagedKV kv;
   const int32_t* table;
   const int32_t* context;
-  int S, H, G, R, nrb, window, max_context, table_stride;
-  int cps;           // chunks of 32 tokens per split
+  int batch, S, H, G, R, nrb, window, max_context, table_stride;
+  int min_chunks;    // fewest chunks of 32 tokens worth a CTA of their own
+  int split;         // 0: every unit is one CTA's (no room for partial sums)
   float scale_log2;  // log2(e) / sqrt(Dh)
-  float* part;       // [units, gridDim.x, RB, DH + 2]: sums, M, l
+  float* part;       // [gridDim.x][2] records of a CTA's first and last segment: sums [RB][DH], then (M, l) [RB]
   int* tickets;      // [units], 0 between calls
   uint32_t* status;
   int dtype;
@@ -59,14 +60,20 @@ struct PagedAttnArgs {
 constexpr int NW = 8;          // warps of a CTA
 constexpr int CHUNK = 32;      // tokens a warp takes at a time
 constexpr float kNoM = -1e30f;  // M of a row that has seen no token
-constexpr int kMaxPagedSplits = 256;
+constexpr float kTop = 14.f, kStart = 4.f;  // weighted probabilities stay below 2^kTop; a moved M leaves the largest near 2^kStart
 
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
-                                         const float (&c)[4]) {
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The same with a zero accumulator.
+__device__ __forceinline__ void mma16816_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 // Transposes an 8 x 8 matrix of 16-bit elements held one row per four lanes.
@@ -87,494 +94,696 @@ __device__ __forceinline__ uint32_t codes_f16(uint32_t z) {
 }
 
 template <int N>
-__device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[N]) {
+__device__ __forceinline__ void lds_words(uint32_t addr, uint32_t (&w)[N]) {
   if constexpr (N == 2) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    w[0] = v.x, w[1] = v.y;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
   } else {
 #pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      const uint4 v = *reinterpret_cast<const uint4*>(p + 4 * i);
-      w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
-    }
+    for (int i = 0; i < N; i += 4)
+      asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                   : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3])
+                   : "r"(addr + 4 * i));
   }
 }
 
-// Four consecutive elements of a query row of either type.
+// Four consecutive elements of a query row of any type.
 __device__ __forceinline__ void load4_dt(const void* p, size_t at, int dtype, float (&x)[4]) {
   if (dtype == HCU_DT_F32) load4(static_cast<const float*>(p) + at, x);
   else if (dtype == HCU_DT_F16) load4(static_cast<const __half*>(p) + at, x);
   else load4(static_cast<const __nv_bfloat16*>(p) + at, x);
 }
-__device__ __forceinline__ void store_dt(void* p, size_t at, int dtype, float x) {
-  if (dtype == HCU_DT_F32) static_cast<float*>(p)[at] = x;
-  else if (dtype == HCU_DT_F16) static_cast<__half*>(p)[at] = __float2half_rn(x);
-  else static_cast<__nv_bfloat16*>(p)[at] = __float2bfloat16_rn(x);
+__device__ __forceinline__ void store4_dt(void* p, size_t at, int dtype, const float (&x)[4]) {
+  if (dtype == HCU_DT_F32) store4(static_cast<float*>(p) + at, x);
+  else if (dtype == HCU_DT_F16) store4(static_cast<__half*>(p) + at, x);
+  else store4(static_cast<__nv_bfloat16*>(p) + at, x);
+}
+
+// Packed f32 pairs: one instruction for two lanes of a 64-bit register pair.
+__device__ __forceinline__ uint64_t f2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void f2_get(uint64_t v, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+
+// Barrier operations on a shared-memory address.
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
 
 constexpr int paged_stage_bytes(int dh) { return CHUNK * (dh + dh / 8); }  // codes and scales, keys and values
 constexpr int paged_stages(int dh) { return dh == 128 ? 3 : 2; }
 constexpr size_t paged_smem(int dh) { return 128 + (size_t)NW * paged_stages(dh) * (paged_stage_bytes(dh) + 8); }
+constexpr int paged_ctas(int dh, int nc) { return dh == 128 && nc == 1 ? 2 : 1; }  // per SM
+
+// The work of a call is a line of chunks: sequence after sequence, in each
+// its KV heads, in each its row blocks, in each the chunks that hold visible tokens
+// (one empty chunk where there are none: zeros are to be written).  CTA i of n
+// takes the i-th of n equal pieces of the line, so a ragged batch and a single
+// long sequence keep every SM busy to the end alike.
+struct PagedPlan {
+  int total, share, more;  // chunks (below 2^31: the host checks); per CTA; the first `more` CTAs take one more
+  int ctas;
+  __device__ int start(int i) const { return i * share + min(i, more); }
+  __device__ int cta_of(int x) const {
+    const int edge = more * (share + 1);
+    return x < edge ? x / (share + 1) : more + (x - edge) / share;
+  }
+};
+
+// Chunk range of sequence b over all its queries: first chunk, count (at least 1).
+__device__ __forceinline__ int2 paged_chunks(const PagedAttnArgs& a, int b) {
+  int ctx = a.context[b];
+  if (ctx > a.max_context || ctx < 0) ctx = 0;
+  const int first = ctx - a.S;
+  const int lo = a.window > 0 ? max(0, first + 1 - a.window) : 0;
+  const int c_lo = lo / CHUNK, c_hi = (ctx + CHUNK - 1) / CHUNK;
+  return make_int2(c_lo, max(1, c_hi - c_lo));
+}
 
 // TERMS f16 numbers per query, NC groups of eight columns: RB = 8 NC / TERMS rows per CTA.
 template <int DH, int TERMS, int NC>
-__global__ void __launch_bounds__(32 * NW, (DH == 128 && NC == 1) ? 2 : 1) attn_paged_kernel(const PagedAttnArgs a) {
+__global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel(const PagedAttnArgs a) {
   constexpr int NB = DH / 32, ST = paged_stages(DH), SB = paged_stage_bytes(DH);
   constexpr int RG = 8 / TERMS, RB = RG * NC;  // rows per column group, per CTA
   constexpr int NR = 2 / TERMS;                // rows per thread and column group
   constexpr int KB = CHUNK * DH / 2, CB = CHUNK * NB * 2;  // bytes of a stage's codes, of its scales
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
+  constexpr int RS = DH + 4;                   // floats per row of the warps' sums (a multiple of four)
+  constexpr size_t REC = (size_t)RB * (DH + 2);  // floats of a segment's record
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int scan[NW], s_last, s_b, s_pos;
+  __shared__ float s_top[RB], s_back[8 * NC];     // per row; per column
+  __shared__ __align__(16) float s_corr[NC][NB][8];  // -8 sum(q) of a block per column (read in pairs)
+  __shared__ uint4 s_q[NC][NB][32];                               // the lanes' B fragments
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int kvh = blockIdx.y, b = blockIdx.z / a.nrb, r0 = (int)(blockIdx.z % a.nrb) * RB;
-  const int rows = min(RB, a.R - r0);
+  const int tok = (g >> 1) + 4 * (g & 1);  // token of accumulator row g (row g + 8: 8 more)
 
-  int ctx = a.context[b];
-  if (ctx > a.max_context || ctx < 0) {
-    if (threadIdx.x == 0) atomicOr(a.status, HCU_DEVERR_BADARG);
-    ctx = 0;
+  // ---- this CTA's piece of the line ----
+  const int per_chunk = a.kv.KV * a.nrb;  // units of a sequence, all of its chunk count
+  PagedPlan plan;
+  int seg_b, seg_base;  // sequence of the next segment, line position of its first chunk
+  int pos, end;
+  {
+    // Every thread sums a run of sequences; the line position of each run follows from a scan.
+    const int run = (a.batch + 32 * NW - 1) / (32 * NW), b0 = threadIdx.x * run, b1 = min(a.batch, b0 + run);
+    int sum = 0;
+    for (int b = b0; b < b1; b++) sum += paged_chunks(a, b).y;
+    int pre = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, pre, o);
+      if (lane >= o) pre += x;
+    }
+    if (lane == 31) scan[warp] = pre;
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int w = 0; w < NW; w++) {
+      if (w < warp) pre += scan[w];
+      total += scan[w];
+    }
+    plan.total = total * per_chunk;
+    const int most = a.split ? (plan.total - 1) / a.min_chunks + 1 : a.batch * per_chunk;
+    plan.ctas = min((int)gridDim.x, most);
+    plan.share = plan.total / plan.ctas;
+    plan.more = plan.total % plan.ctas;
+    if ((int)blockIdx.x >= plan.ctas) return;
+    if (a.split) {
+      pos = plan.start(blockIdx.x);
+      end = plan.start(blockIdx.x + 1);
+      const int lo = (pre - sum) * per_chunk;
+      if (pos >= lo && pos < pre * per_chunk) {  // one thread's run holds the first chunk
+        int at = lo, b = b0;
+        for (;; b++) {
+          const int n = paged_chunks(a, b).y * per_chunk;
+          if (pos < at + n) break;
+          at += n;
+        }
+        s_b = b;
+        s_pos = at;
+      }
+      __syncthreads();
+      seg_b = s_b;
+      seg_base = s_pos;
+    } else {  // whole units, blockIdx.x-th and every gridDim.x-th after it
+      pos = blockIdx.x, end = a.batch * per_chunk;
+      seg_b = 0, seg_base = 0;
+    }
   }
-  // The tokens that some row of this CTA sees, [lo, hi), and those that all see, [lo_all, hi_all).
-  const int pos_first = ctx - a.S + r0 / a.G, pos_last = ctx - a.S + (r0 + rows - 1) / a.G;
-  const int lo = a.window > 0 ? max(0, pos_first + 1 - a.window) : 0, hi = max(0, pos_last + 1);
-  const int lo_all = a.window > 0 ? max(0, pos_last + 1 - a.window) : 0, hi_all = max(0, pos_first + 1);
-  const int c_lo = lo / CHUNK, c_hi = lo < hi ? (hi + CHUNK - 1) / CHUNK : c_lo;
-  const int nsplit = max(1, (c_hi - c_lo + a.cps - 1) / a.cps);
-  const int split = blockIdx.x;
-  if (split >= nsplit) return;
-  const int c0 = c_lo + split * a.cps, c1 = min(c_hi, c0 + a.cps);
 
   // ---- this warp's ring ----
-  uint8_t* ring = smem + warp * ST * SB;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + NW * ST * SB) + warp * ST;
+  const uint32_t ring = smem_u32(smem) + warp * ST * SB;
+  const uint32_t full = smem_u32(smem + NW * ST * SB) + warp * ST * 8;
   if (lane == 0) {
-    for (int i = 0; i < ST; i++) mbar_init(&full[i], 1);
+    for (int i = 0; i < ST; i++) mbar_init(reinterpret_cast<uint64_t*>(smem + NW * ST * SB) + warp * ST + i, 1);
     fence_barrier_init();
   }
   __syncwarp();
-  const int page_mask = (1 << a.kv.page_log2) - 1;
-  const int sub_log2 = min(a.kv.page_log2, 5), subs = CHUNK >> sub_log2;  // a chunk is one page's part or two pages
-  // Lane 4s + w issues tensor w (key codes, value codes, key scales, value
-  // scales) of part s.  Returns which parts hold data: parts without a visible
-  // token are not looked up, parts on a bad page are reported and left out.
-  const int* table = a.table + (size_t)b * a.table_stride;
-  auto page_of = [&](int c) -> int {
-    const int s = lane >> 2, t0 = c * CHUNK + (s << sub_log2);
-    if (s >= subs || c >= c1 || t0 >= hi || t0 + (1 << sub_log2) <= lo) return -2;
-    const int page = table[t0 >> a.kv.page_log2];
-    return page >= 0 && page < a.kv.n_pages ? page : -1;
+  // A chunk is a part of one page or (16-token pages) two pages.  Lane 4s + w
+  // brings tensor w (key codes, value codes, key scales, value scales) of part s.
+  const int sub_log2 = min(a.kv.page_log2, 5), subs = CHUNK >> sub_log2;
+  const int is = lane >> 2, iw = lane & 3, row_bytes = iw < 2 ? DH / 2 : NB * 2;
+  const uint32_t part_bytes = row_bytes << sub_log2, all_bytes = (2 * KB + 2 * CB) / CHUNK << sub_log2;
+  const uint8_t* isrc = iw == 0 ? a.kv.k : iw == 1 ? a.kv.v : reinterpret_cast<const uint8_t*>(iw == 2 ? a.kv.ks : a.kv.vs);
+  const uint32_t idst = ring + (iw < 2 ? iw * KB : 2 * KB + (iw - 2) * CB) + is * part_bytes;
+  const uint32_t chunk_mask = max(1 << a.kv.page_log2, CHUNK) / CHUNK - 1;  // chunks of a page, less one
+  const uint32_t page_bytes = (uint32_t)a.kv.KV * row_bytes << a.kv.page_log2;
+  auto wait_full = [&](int st, uint32_t ph) {
+    return bar_try(full + 8 * st, ph) ||
+           mbar_wait(reinterpret_cast<uint64_t*>(smem + NW * ST * SB) + warp * ST + st, ph, a.status);
   };
-  auto issue = [&](int c, int stage, int page) -> uint32_t {
-    if (page == -1) atomicOr(a.status, HCU_DEVERR_BADARG);
-    const uint32_t have = __ballot_sync(0xffffffffu, page >= 0);
-    const uint32_t ok = (have & 1u) | ((have >> 3) & 2u);  // lanes 0 and 4
-    if (lane == 0) mbar_arrive_expect_tx(&full[stage], __popc(ok) * ((2 * KB + 2 * CB) / CHUNK << sub_log2));
-    __syncwarp();
-    if (page >= 0) {
-      const int s = lane >> 2, w = lane & 3, t0 = c * CHUNK + (s << sub_log2);
-      const long long row = paged_row(a.kv, page, kvh, t0 & page_mask);
-      uint8_t* st = ring + stage * SB;
-      const uint8_t* src = w == 0 ? a.kv.k : w == 1 ? a.kv.v : reinterpret_cast<const uint8_t*>(w == 2 ? a.kv.ks : a.kv.vs);
-      const int rb = w < 2 ? DH / 2 : NB * 2;
-      uint8_t* dst = st + (w < 2 ? w * KB : 2 * KB + (w - 2) * CB) + (s << sub_log2) * rb;
-      bulk_load(dst, src + row * rb, (uint32_t)(rb << sub_log2), &full[stage]);
-    }
-    return ok;
-  };
-  uint32_t have[ST];
-  int next_page;
-  {
-    int pg[ST];
-#pragma unroll
-    for (int i = 0; i < ST; i++) pg[i] = page_of(c0 + warp + i * NW);
-    next_page = page_of(c0 + warp + ST * NW);
-#pragma unroll
-    for (int i = 0; i < ST; i++) have[i] = issue(c0 + warp + i * NW, i, pg[i]);
-  }
+  int stage = 0;
+  uint32_t phase = 0;
+  bool ok = true;
 
-  // ---- query columns: column g of group nc is row / term of this lane's B fragments ----
-  uint32_t qf[NC][NB][4];
-  float cini[NC][NB][2];
-  float rs[NC][NR];  // score = rs * accumulated sum, rows of this thread's accumulator columns
+  while (pos < end) {
+    // ---- the segment: chunks [c0, c1) of unit (b, kvh, rb) ----
+    int b, kvh, rb, c0, c1, unit_first, unit_last;  // the unit's first and last CTA
+    if (a.split) {
+      int2 ch = paged_chunks(a, seg_b);
+      while (pos >= seg_base + ch.y * per_chunk) {
+        seg_base += ch.y * per_chunk;
+        ch = paged_chunks(a, ++seg_b);
+      }
+      const int u = (pos - seg_base) / ch.y, u0 = seg_base + u * ch.y;
+      b = seg_b, kvh = u / a.nrb, rb = u % a.nrb;
+      c0 = ch.x + pos - u0;
+      c1 = ch.x + min(ch.y, end - u0);
+      unit_first = plan.cta_of(u0), unit_last = plan.cta_of(u0 + ch.y - 1);
+      pos = min(end, u0 + ch.y);
+    } else {
+      b = pos / per_chunk;
+      const int u = pos % per_chunk;
+      kvh = u / a.nrb, rb = u % a.nrb;
+      const int2 ch = paged_chunks(a, b);
+      c0 = ch.x, c1 = ch.x + ch.y;
+      unit_first = unit_last = blockIdx.x;
+      pos += gridDim.x;
+    }
+    const int r0 = rb * RB, rows = min(RB, a.R - r0);
+    int ctx = a.context[b];
+    if (ctx > a.max_context || ctx < 0) {
+      if (threadIdx.x == 0) atomicOr(a.status, HCU_DEVERR_BADARG);
+      ctx = 0;
+    }
+    // The tokens that some row of this block sees, [lo, hi), and those that all see, [lo_all, hi_all).
+    const int pos_first = ctx - a.S + r0 / a.G, pos_last = ctx - a.S + (r0 + rows - 1) / a.G;
+    const int lo = a.window > 0 ? max(0, pos_first + 1 - a.window) : 0, hi = max(0, pos_last + 1);
+    const int lo_all = a.window > 0 ? max(0, pos_last + 1 - a.window) : 0, hi_all = max(0, pos_first + 1);
+    const int32_t* table = a.table + (size_t)b * a.table_stride;
+    const uint8_t* head_src = isrc + ((long long)kvh << a.kv.page_log2) * row_bytes;
+
+    // The page of this lane's part of chunk c: -2 where no row sees a token of it (not looked up), -1 where the table's
+    // entry is no page.
+    const int part_at = is << sub_log2, part_hi = is < subs ? min(hi, c1 * CHUNK) - part_at : -1,
+              part_lo = lo - part_at - (1 << sub_log2);
+    auto page_of = [&](int c) -> int {
+      if (c * CHUNK >= part_hi || c * CHUNK <= part_lo) return -2;
+      const int page = table[(c * CHUNK + part_at) >> a.kv.page_log2];
+      return (uint32_t)page < (uint32_t)a.kv.n_pages ? page : -1;
+    };
+    // Returns which parts hold data.
+    auto issue = [&](int c, int st, int page) -> uint32_t {
+      const uint32_t got = __ballot_sync(0xffffffffu, page >= 0);
+      const uint32_t parts = (got & 1u) | ((got >> 3) & 2u);  // lanes 0 and 4
+      if (lane == 0) bar_expect(full + 8 * st, (parts & 1u) * all_bytes + (parts >> 1) * all_bytes);
+      __syncwarp();
+      if (page >= 0) {
+        const uint8_t* src = head_src + (uint64_t)(uint32_t)page * page_bytes + ((uint32_t)c & chunk_mask) * (uint32_t)(CHUNK * row_bytes);
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                         idst + st * SB),
+                     "l"(src), "r"(part_bytes), "r"(full + 8 * st)
+                     : "memory");
+      } else if (page == -1) {
+        atomicOr(a.status, HCU_DEVERR_BADARG);
+      }
+      return parts;
+    };
+    uint32_t have = 0;  // two bits per stage
+    int next_page;
+    {
+      int pg[ST];
 #pragma unroll
-  for (int nc = 0; nc < NC; nc++) {
-    const int r = nc * RG + (TERMS == 2 ? g >> 1 : g);
-    const bool there = r < rows;
-    const int rr = r0 + (there ? r : 0), s = rr / a.G, h = kvh * a.G + rr % a.G;
-    const size_t at = (((size_t)b * a.S + s) * a.H + h) * DH;
-    float q[NB][8], top = 0.f;
+      for (int i = 0; i < ST; i++) pg[i] = page_of(c0 + warp + i * NW);
+      next_page = page_of(c0 + warp + ST * NW);
 #pragma unroll
-    for (int i = 0; i < NB; i++) {
-      float x[4], y[4];
-      load4_dt(a.q, at + 32 * i + 8 * t, a.dtype, x);
-      load4_dt(a.q, at + 32 * i + 8 * t + 4, a.dtype, y);
-#pragma unroll
-      for (int c = 0; c < 4; c++) {
-        q[i][c] = there ? x[c] : 0.f;
-        q[i][c + 4] = there ? y[c] : 0.f;
-        top = fmaxf(top, fmaxf(fabsf(q[i][c]), fabsf(q[i][c + 4])));
+      for (int i = 0; i < ST; i++) {
+        const int st = stage + i >= ST ? stage + i - ST : stage + i;
+        have |= issue(c0 + warp + i * NW, st, pg[i]) << (2 * st);
       }
     }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    // 2^sq brings the row's largest magnitude into [2^13, 2^14)
-    const int sq = top > 0.f ? min(127, 140 - (int)(__float_as_uint(top) >> 23)) : 0;
-    const float up = __uint_as_float((uint32_t)(max(sq, -126) + 127) << 23);
-    const float back = ldexpf(a.scale_log2, 24 - max(sq, -126));
+
+    // ---- query columns, prepared once for the CTA ----
+    for (int r = warp; r < RB; r += NW) {  // the rows' largest magnitudes
+      float top = 0.f;
+      if (r < rows) {
+        const int s = (r0 + r) / a.G, h = kvh * a.G + (r0 + r) % a.G;
 #pragma unroll
-    for (int i = 0; i < NB; i++) {
+        for (int j = 0; j < DH / 128; j++) {
+          float x[4];
+          load4_dt(a.q, (((size_t)b * a.S + s) * a.H + h) * DH + 128 * j + 4 * lane, a.dtype, x);
+          top = fmaxf(top, fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
+        }
+      }
+      top = warp_max(top);
+      if (lane == 0) s_top[r] = top;
+    }
+    __syncthreads();
+    for (int k = warp; k < NC * NB; k += NW) {  // group nc, block i; column g of the group is row / term of the lane's fragment
+      const int nc = k / NB, i = k % NB, r = nc * RG + (TERMS == 2 ? g >> 1 : g);
+      float q[8] = {};
+      if (r < rows) {
+        const int s = (r0 + r) / a.G, h = kvh * a.G + (r0 + r) % a.G;
+        const size_t at = (((size_t)b * a.S + s) * a.H + h) * DH + 32 * i + 8 * t;
+        float x[4], y[4];
+        load4_dt(a.q, at, a.dtype, x);
+        load4_dt(a.q, at + 4, a.dtype, y);
+#pragma unroll
+        for (int c = 0; c < 4; c++) q[c] = x[c], q[c + 4] = y[c];
+      }
+      // 2^sq brings the row's largest magnitude into [2^13, 2^14)
+      const float top = s_top[r];
+      const int sq = top > 0.f ? max(-126, min(127, 140 - (int)(__float_as_uint(top) >> 23))) : 0;
+      const float up = __uint_as_float((uint32_t)(sq + 127) << 23);
       float sum = 0.f;
+      uint32_t w[4];
 #pragma unroll
       for (int m = 0; m < 4; m++) {
         // register m: dimensions m and m + 4 of the lane's eight; odd m meets codes times 16
-        float v[2];
         __half o[2];
 #pragma unroll
         for (int c = 0; c < 2; c++) {
-          v[c] = q[i][m + 4 * c] * up;
-          if (TERMS == 2 && (g & 1)) v[c] -= __half2float(__float2half_rn(v[c]));
-          o[c] = __float2half_rn((m & 1) ? v[c] * 0.0625f : v[c]);
+          float v = q[m + 4 * c] * up;
+          if (TERMS == 2 && (g & 1)) v -= __half2float(__float2half_rn(v));
+          o[c] = __float2half_rn((m & 1) ? v * 0.0625f : v);
           sum += __half2float(o[c]) * ((m & 1) ? 16.f : 1.f);
         }
-        qf[nc][i][m] = h2_bits(__halves2half2(o[0], o[1]));
+        w[m] = h2_bits(__halves2half2(o[0], o[1]));
       }
+      s_q[nc][i][lane] = make_uint4(w[0], w[1], w[2], w[3]);
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      sum *= -8.f * 5.9604644775390625e-08f;  // -8 * 2^-24
-      cini[nc][i][0] = __shfl_sync(0xffffffffu, sum, 8 * t);      // column 2t is lane group g = 2t
-      cini[nc][i][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);  // column 2t + 1
-    }
-    rs[nc][0] = __shfl_sync(0xffffffffu, back, 8 * t);
-    if (NR == 2) rs[nc][NR - 1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
-  }
-  // Visible range of this thread's rows, for chunks that not every row sees whole.
-  int row_lo[NC][NR], row_hi[NC][NR];
-#pragma unroll
-  for (int nc = 0; nc < NC; nc++)
-#pragma unroll
-    for (int r = 0; r < NR; r++) {
-      const int rl = nc * RG + t * NR + r, pos = ctx - a.S + (r0 + rl) / a.G;
-      row_hi[nc][r] = rl < rows ? pos : -1;
-      row_lo[nc][r] = a.window > 0 ? pos + 1 - a.window : 0;
-    }
-
-  float O[2 * NB][NC][4] = {};
-  float M[NC][NR], L[NC][NR];
-#pragma unroll
-  for (int nc = 0; nc < NC; nc++)
-#pragma unroll
-    for (int r = 0; r < NR; r++) M[nc][r] = kNoM, L[nc][r] = 0.f;
-  const int tok = (g >> 1) + 4 * (g & 1);  // token of accumulator row g (row g + 8: 8 more)
-
-  bool ok = true;
-  int stage = 0;
-  uint32_t phase = 0;
-  for (int c = c0 + warp; c < c1; c += NW) {
-    if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], phase, a.status))) {
-      ok = false;
-      break;
-    }
-    const uint8_t* st = ring + stage * SB;
-    uint32_t parts = have[0];
-#pragma unroll
-    for (int i = 1; i < ST; i++) parts = stage == i ? have[i] : parts;
-    const int base = c * CHUNK;
-    const bool whole = base >= lo_all && base + CHUNK <= hi_all && parts == (subs == 2 ? 3u : 1u);
-    // ---- scores of 32 tokens ----
-    float x[2][2][NC][NR];     // [16-token step][accumulator row half][..]: score, log2 units
-    float vs[2][2][NB], e[2][2];  // value scales of the thread's tokens, exponent of their largest
-#pragma unroll
-    for (int j = 0; j < 2; j++) {
-      uint32_t kw[2][NB];
-      float ks[2][NB];
-#pragma unroll
-      for (int u = 0; u < 2; u++) {
-        const int row = 16 * j + 8 * u + tok;
-        lds_words<NB>(st + row * (DH / 2) + t * NB * 4, kw[u]);
-        uint32_t sw[NB / 2];
-        lds_words<NB / 2>(st + 2 * KB + row * NB * 2, sw);
-        uint32_t vw[NB / 2];
-        lds_words<NB / 2>(st + 2 * KB + CB + row * NB * 2, vw);
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < NB / 2; i++) {
-          const float2 f = f16x2_to_f2(sw[i]), w = f16x2_to_f2(vw[i]);
-          ks[u][2 * i] = f.x, ks[u][2 * i + 1] = f.y;
-          vs[j][u][2 * i] = w.x, vs[j][u][2 * i + 1] = w.y;
-          const uint32_t ab = vw[i] & 0x7fff7fffu;
-          top = max(top, max(ab >> 16, ab & 0xffffu));
-        }
-        e[j][u] = (float)((int)(top >> 10) - 14);  // every |scale| of the token is below 2^e
+      if (t == 0) {
+        s_corr[nc][i][g] = sum * (-8.f * 5.9604644775390625e-08f);  // -8 * 2^-24
+        if (i == 0) s_back[8 * nc + g] = ldexpf(a.scale_log2, 24 - sq);
       }
+    }
+    __syncthreads();
+    uint32_t qf[NC][NB][4];
+    float corr[NC][NB][NR];  // rows of this thread's accumulator columns 2t, 2t + 1
+    float rs[NC][NR];        // score = rs * accumulated sum
 #pragma unroll
-      for (int nc = 0; nc < NC; nc++)
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-          for (int r = 0; r < NR; r++) x[j][u][nc][r] = 0.f;
+    for (int nc = 0; nc < NC; nc++) {
 #pragma unroll
       for (int i = 0; i < NB; i++) {
-        const uint32_t a0[4] = {kw[0][i] & 0x000f000fu, kw[1][i] & 0x000f000fu, kw[0][i] & 0x00f000f0u,
-                                kw[1][i] & 0x00f000f0u};
-        const uint32_t w0 = kw[0][i] >> 8, w1 = kw[1][i] >> 8;
-        const uint32_t a1[4] = {w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u};
-#pragma unroll
-        for (int nc = 0; nc < NC; nc++) {
-          float d[4];
-          const float ini[4] = {cini[nc][i][0], cini[nc][i][1], cini[nc][i][0], cini[nc][i][1]};
-          mma16816(d, a0, qf[nc][i][0], qf[nc][i][1], ini);
-          mma16816(d, a1, qf[nc][i][2], qf[nc][i][3], d);
-#pragma unroll
-          for (int u = 0; u < 2; u++) {
-            if (TERMS == 2) {
-              x[j][u][nc][0] = fmaf(ks[u][i], d[2 * u] + d[2 * u + 1], x[j][u][nc][0]);
-            } else {
-              x[j][u][nc][0] = fmaf(ks[u][i], d[2 * u], x[j][u][nc][0]);
-              x[j][u][nc][NR - 1] = fmaf(ks[u][i], d[2 * u + 1], x[j][u][nc][NR - 1]);
-            }
-          }
-        }
+        const uint4 w = s_q[nc][i][lane];
+        qf[nc][i][0] = w.x, qf[nc][i][1] = w.y, qf[nc][i][2] = w.z, qf[nc][i][3] = w.w;
+        const float2 c = *reinterpret_cast<const float2*>(&s_corr[nc][i][2 * t]);
+        corr[nc][i][0] = TERMS == 2 ? c.x + c.y : c.x;
+        if (NR == 2) corr[nc][i][NR - 1] = c.y;
       }
+      rs[nc][0] = s_back[8 * nc + 2 * t];
+      if (NR == 2) rs[nc][NR - 1] = s_back[8 * nc + 2 * t + 1];
+    }
+
+    float O[2 * NB][NC][4] = {};
+    float M[NC][NR], L[NC][NR], T[NC][NR];  // T: the score above which M has to move
+    float cap = 0.f, cap_log2 = -25.f;      // every value scale so far is at most cap <= 2^cap_log2
 #pragma unroll
-      for (int nc = 0; nc < NC; nc++)
+    for (int nc = 0; nc < NC; nc++)
 #pragma unroll
-        for (int u = 0; u < 2; u++)
+      for (int r = 0; r < NR; r++) M[nc][r] = T[nc][r] = kNoM, L[nc][r] = 0.f;
+
+    for (int c = c0 + warp; c < c1; c += NW) {
+      if (!__all_sync(0xffffffffu, wait_full(stage, phase))) {
+        ok = false;
+        break;
+      }
+      const uint32_t st = ring + stage * SB;
+      const uint32_t parts = (have >> (2 * stage)) & 3u;
+      const int base = c * CHUNK;
+      const bool whole = base >= lo_all && base + CHUNK <= hi_all && parts == (subs == 2 ? 3u : 1u);
+      // ---- scores of 32 tokens ----
+      float x[2][2][NC][NR];         // [16-token step][accumulator row half][..]: score, log2 units
+      uint32_t vsw[2][2][NB / 2];    // value scales of the thread's tokens, f16 pairs
 #pragma unroll
-          for (int r = 0; r < NR; r++) x[j][u][nc][r] *= rs[nc][r];
-      if (!whole) {
-        // Tokens outside a row's range and on missing pages weigh nothing; what their rows hold is not looked at.
+      for (int j = 0; j < 2; j++) {
+        uint32_t kw[2][NB], ksw[2][NB / 2];
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-          const int tk = 16 * j + 8 * u + tok;
-          const bool data = (parts >> (subs == 2 ? j : 0)) & 1u;
-          bool any = false;
+          const uint32_t row = 16 * j + 8 * u + tok;
+          lds_words<NB>(st + row * (DH / 2) + t * NB * 4, kw[u]);
+          lds_words<NB / 2>(st + 2 * KB + row * NB * 2, ksw[u]);
+          lds_words<NB / 2>(st + 2 * KB + CB + row * NB * 2, vsw[j][u]);
 #pragma unroll
           for (int nc = 0; nc < NC; nc++)
 #pragma unroll
-            for (int r = 0; r < NR; r++) {
-              const bool see = data && base + tk >= row_lo[nc][r] && base + tk <= row_hi[nc][r];
-              x[j][u][nc][r] = see ? x[j][u][nc][r] : -INFINITY;
-              any = any || see;
-            }
-          if (!any) {
-            e[j][u] = 0.f;
+            for (int r = 0; r < NR; r++) x[j][u][nc][r] = 0.f;
+        }
 #pragma unroll
-            for (int i = 0; i < NB; i++) vs[j][u][i] = 0.f;
+        for (int i = 0; i < NB; i++) {
+          const uint32_t a0[4] = {kw[0][i] & 0x000f000fu, kw[1][i] & 0x000f000fu, kw[0][i] & 0x00f000f0u,
+                                  kw[1][i] & 0x00f000f0u};
+          const uint32_t w0 = kw[0][i] >> 8, w1 = kw[1][i] >> 8;
+          const uint32_t a1[4] = {w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u};
+          float ks[2];
+#pragma unroll
+          for (int u = 0; u < 2; u++) ks[u] = (i & 1) ? f16x2_to_f2(ksw[u][i / 2]).y : f16x2_to_f2(ksw[u][i / 2]).x;
+#pragma unroll
+          for (int nc = 0; nc < NC; nc++) {
+            float d[4];
+            mma16816_zero(d, a0, qf[nc][i][0], qf[nc][i][1]);
+            mma16816(d, a1, qf[nc][i][2], qf[nc][i][3]);
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+              if (TERMS == 2) {
+                x[j][u][nc][0] = fmaf(ks[u], (d[2 * u] + corr[nc][i][0]) + d[2 * u + 1], x[j][u][nc][0]);
+              } else {
+#pragma unroll
+                for (int r = 0; r < NR; r++)
+                  x[j][u][nc][r] = fmaf(ks[u], d[2 * u + r] + corr[nc][i][r], x[j][u][nc][r]);
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int nc = 0; nc < NC; nc++)
+#pragma unroll
+          for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int r = 0; r < NR; r++) x[j][u][nc][r] *= rs[nc][r];
+        if (!whole) {
+          // Tokens outside a row's range and on missing pages weigh nothing; what their rows hold is not looked at.
+#pragma unroll
+          for (int u = 0; u < 2; u++) {
+            const int at = base + 16 * j + 8 * u + tok;
+            const bool data = (parts >> (subs == 2 ? j : 0)) & 1u;
+            bool any = false;
+#pragma unroll
+            for (int nc = 0; nc < NC; nc++)
+#pragma unroll
+              for (int r = 0; r < NR; r++) {
+                const int rl = nc * RG + t * NR + r, p = ctx - a.S + (r0 + rl) / a.G;
+                const bool see = data && rl < rows && at <= p && (a.window == 0 || at > p - a.window);
+                x[j][u][nc][r] = see ? x[j][u][nc][r] : -INFINITY;
+                any = any || see;
+              }
+            if (!any)
+#pragma unroll
+              for (int i = 0; i < NB / 2; i++) vsw[j][u][i] = 0u;
           }
         }
       }
+      // ---- reference points: they move when a weighted probability could pass 2^kTop ----
+      __half2 vtop = __habs2(bits_h2(vsw[0][0][0]));
+#pragma unroll
+      for (int i = 1; i < 2 * NB; i++)
+        vtop = __hmax2(vtop, __habs2(bits_h2(vsw[i / NB][(i / (NB / 2)) & 1][i % (NB / 2)])));
+      const float vmax = fmaxf(__low2float(vtop), __high2float(vtop));
+      bool grow = vmax > cap;
+#pragma unroll
+      for (int nc = 0; nc < NC; nc++)
+#pragma unroll
+        for (int r = 0; r < NR; r++)
+          grow = grow || fmaxf(fmaxf(x[0][0][nc][r], x[0][1][nc][r]), fmaxf(x[1][0][nc][r], x[1][1][nc][r])) > T[nc][r];
+      if (__any_sync(0xffffffffu, grow)) {
+        const float top = warp_max(vmax);
+        if (top > cap) {  // the next power of two
+          cap_log2 = (float)((int)(__float_as_uint(top) >> 23) - 126);
+          cap = exp2f(cap_log2);
+        }
+#pragma unroll
+        for (int nc = 0; nc < NC; nc++) {
+          float f[NR];
+#pragma unroll
+          for (int r = 0; r < NR; r++) {
+            float w = fmaxf(fmaxf(x[0][0][nc][r], x[0][1][nc][r]), fmaxf(x[1][0][nc][r], x[1][1][nc][r]));
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, o));
+            const float m = w + cap_log2 > M[nc][r] + kTop ? w + cap_log2 - kStart : M[nc][r];
+            f[r] = exp2f(M[nc][r] - m);
+            M[nc][r] = m;
+            T[nc][r] = m + kTop - cap_log2;
+            L[nc][r] *= f[r];
+          }
+#pragma unroll
+          for (int i = 0; i < 2 * NB; i++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) O[i][nc][k] *= f[NR == 2 ? (k & 1) : 0];
+        }
+      }
+      // ---- weighted probabilities, values ----
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        uint32_t pb[NC][NB][2];  // B fragments: tokens in pairs, column g
+#pragma unroll
+        for (int nc = 0; nc < NC; nc++)
+#pragma unroll
+          for (int u = 0; u < 2; u++) {
+            float p[NR];
+#pragma unroll
+            for (int r = 0; r < NR; r++) {
+              p[r] = ex2_approx(x[j][u][nc][r] - M[nc][r]);
+              L[nc][r] += p[r];
+            }
+#pragma unroll
+            for (int i = 0; i < NB / 2; i++) {  // two blocks at a time
+              const float2 v = f16x2_to_f2(vsw[j][u][i]);
+              uint32_t w[2];
+              if (TERMS == 2) {
+                const uint64_t y = f2_mul(f2(v.x, v.y), f2(p[0], p[0]));
+                float y0, y1, l0, l1;
+                f2_get(y, y0, y1);
+                const float t0 = __uint_as_float(__float_as_uint(y0) & 0xffffe000u);
+                const float t1 = __uint_as_float(__float_as_uint(y1) & 0xffffe000u);
+                f2_get(f2_fma(f2(t0, t1), f2(-1.f, -1.f), y), l0, l1);
+                w[0] = h2_bits(__floats2half2_rn(t0, l0));
+                w[1] = h2_bits(__floats2half2_rn(t1, l1));
+              } else {
+                float y0, y1, z0, z1;
+                f2_get(f2_mul(f2(v.x, v.y), f2(p[0], p[0])), y0, y1);
+                f2_get(f2_mul(f2(v.x, v.y), f2(p[NR - 1], p[NR - 1])), z0, z1);
+                w[0] = h2_bits(__floats2half2_rn(y0, z0));
+                w[1] = h2_bits(__floats2half2_rn(y1, z1));
+              }
+              pb[nc][2 * i][u] = movmatrix(w[0]);
+              pb[nc][2 * i + 1][u] = movmatrix(w[1]);
+            }
+          }
+        uint32_t vw[4][NB / 2];  // tokens t, t + 4, t + 8, t + 12: halfwords of the lane's dimensions
+#pragma unroll
+        for (int k = 0; k < 4; k++) lds_words<NB / 2>(st + KB + (16 * j + t + 4 * k) * (DH / 2) + g * NB * 2, vw[k]);
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+          const uint32_t sel = (i & 1) ? 0x7632u : 0x5410u;
+          uint32_t z0 = __byte_perm(vw[0][i / 2], vw[1][i / 2], sel), z1 = __byte_perm(vw[2][i / 2], vw[3][i / 2], sel);
+#pragma unroll
+          for (int m = 0; m < 2; m++) {
+            if (TERMS == 2) {
+              const uint32_t av[4] = {codes_f16<false>(z0), codes_f16<true>(z0), codes_f16<false>(z1), codes_f16<true>(z1)};
+#pragma unroll
+              for (int nc = 0; nc < NC; nc++) mma16816(O[2 * i + m][nc], av, pb[nc][i][0], pb[nc][i][1]);
+            } else {
+              // as the key codes, f16 subnormals; the offset is a product of its own
+              const uint32_t av[4] = {z0 & 0x000f000fu, z0 & 0x00f000f0u, z1 & 0x000f000fu, z1 & 0x00f000f0u};
+              const uint32_t off[4] = {0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u};  // -8, -128 times 2^-24
+#pragma unroll
+              for (int nc = 0; nc < NC; nc++) {
+                mma16816(O[2 * i + m][nc], av, pb[nc][i][0], pb[nc][i][1]);
+                mma16816(O[2 * i + m][nc], off, pb[nc][i][0], pb[nc][i][1]);
+              }
+            }
+            z0 >>= 8, z1 >>= 8;
+          }
+        }
+      }
+      // ---- the stage is free: the chunk ST rounds on ----
+      __syncwarp();
+      have = (have & ~(3u << (2 * stage))) | issue(c + ST * NW, stage, next_page) << (2 * stage);
+      next_page = page_of(c + (ST + 1) * NW);
+      if (++stage == ST) stage = 0, phase ^= 1;
     }
-    // ---- reference points: move when a weighted probability would pass 2^14 ----
-    bool grow = false;
+    // Every stage has one phase left (without data after a whole walk): they are waited for before the rings are reused.
+    for (int i = 0; i < ST; i++) {
+      wait_full(stage, phase);
+      if (++stage == ST) stage = 0, phase ^= 1;
+    }
+    __syncthreads();
+
+    // ---- join the warps ----
+    constexpr float kUnscale = TERMS == 2 ? 1.f : 16777216.f;  // subnormal codes carry 2^-24
+    float* buf = reinterpret_cast<float*>(smem);  // [NW][RB][RS]: sums, M, l
+    static_assert((size_t)NW * RB * RS * 4 <= (size_t)NW * ST * SB, "the warps' sums fit the rings");
 #pragma unroll
     for (int nc = 0; nc < NC; nc++)
 #pragma unroll
       for (int r = 0; r < NR; r++) {
-        float w = fmaxf(fmaxf(x[0][0][nc][r] + e[0][0], x[0][1][nc][r] + e[0][1]),
-                        fmaxf(x[1][0][nc][r] + e[1][0], x[1][1][nc][r] + e[1][1]));
-        grow = grow || w > M[nc][r] + 14.f;
-      }
-    if (__any_sync(0xffffffffu, grow)) {
+        float l = L[nc][r];
 #pragma unroll
-      for (int nc = 0; nc < NC; nc++) {
-        float f[NR];
+        for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        float* w = buf + (warp * RB + nc * RG + t * NR + r) * RS;
 #pragma unroll
-        for (int r = 0; r < NR; r++) {
-          float w = fmaxf(fmaxf(x[0][0][nc][r] + e[0][0], x[0][1][nc][r] + e[0][1]),
-                          fmaxf(x[1][0][nc][r] + e[1][0], x[1][1][nc][r] + e[1][1]));
+        for (int i = 0; i < NB; i++)
 #pragma unroll
-          for (int o = 4; o < 32; o <<= 1) w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, o));
-          const float m = w > M[nc][r] + 14.f ? w - 4.f : M[nc][r];
-          f[r] = exp2f(M[nc][r] - m);
-          M[nc][r] = m;
-          L[nc][r] *= f[r];
-        }
-#pragma unroll
-        for (int i = 0; i < 2 * NB; i++)
-#pragma unroll
-          for (int k = 0; k < 4; k++) O[i][nc][k] *= f[NR == 2 ? (k & 1) : 0];
-      }
-    }
-    // ---- weighted probabilities, values ----
-#pragma unroll
-    for (int j = 0; j < 2; j++) {
-      uint32_t pb[NC][NB][2];  // B fragments: tokens in pairs, column g
-#pragma unroll
-      for (int nc = 0; nc < NC; nc++)
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-          float p[NR];
-#pragma unroll
-          for (int r = 0; r < NR; r++) {
-            p[r] = ex2_approx(x[j][u][nc][r] - M[nc][r]);
-            L[nc][r] += p[r];
+          for (int m = 0; m < 2; m++) {
+            const float* o4 = O[2 * i + m][nc];
+            const int d = 32 * i + 4 * g + 2 * m;
+            *reinterpret_cast<float2*>(w + d) =
+                make_float2((TERMS == 2 ? o4[0] + o4[1] : o4[r]) * kUnscale,
+                            (TERMS == 2 ? o4[2] + o4[3] : o4[2 + r]) * (0.0625f * kUnscale));
           }
-#pragma unroll
-          for (int i = 0; i < NB; i++) {
-            uint32_t w;
-            if (TERMS == 2) {
-              const float y = p[0] * vs[j][u][i];
-              const float top = __uint_as_float(__float_as_uint(y) & 0xffffe000u);
-              w = h2_bits(__floats2half2_rn(top, y - top));
-            } else {
-              w = h2_bits(__floats2half2_rn(p[0] * vs[j][u][i], p[NR - 1] * vs[j][u][i]));
-            }
-            pb[nc][i][u] = movmatrix(w);
-          }
-        }
-      uint32_t vw[4][NB / 2];  // tokens t, t + 4, t + 8, t + 12: halfwords of the lane's dimensions
-#pragma unroll
-      for (int k = 0; k < 4; k++) lds_words<NB / 2>(st + KB + (16 * j + t + 4 * k) * (DH / 2) + g * NB * 2, vw[k]);
-#pragma unroll
-      for (int i = 0; i < NB; i++) {
-        const uint32_t sel = (i & 1) ? 0x7632u : 0x5410u;
-        uint32_t z0 = __byte_perm(vw[0][i / 2], vw[1][i / 2], sel), z1 = __byte_perm(vw[2][i / 2], vw[3][i / 2], sel);
-#pragma unroll
-        for (int m = 0; m < 2; m++) {
-          const uint32_t av[4] = {codes_f16<false>(z0), codes_f16<true>(z0), codes_f16<false>(z1), codes_f16<true>(z1)};
-#pragma unroll
-          for (int nc = 0; nc < NC; nc++)
-            mma16816(O[2 * i + m][nc], av, pb[nc][i][0], pb[nc][i][1], O[2 * i + m][nc]);
-          z0 >>= 8, z1 >>= 8;
-        }
+        if (g == 0) w[DH] = M[nc][r], w[DH + 1] = l;
       }
-    }
-    // ---- the stage is free: the chunk ST rounds on ----
-    __syncwarp();
-    const uint32_t got = issue(c + ST * NW, stage, next_page);
-#pragma unroll
-    for (int i = 0; i < ST; i++) have[i] = stage == i ? got : have[i];
-    next_page = page_of(c + (ST + 1) * NW);
-    if (++stage == ST) stage = 0, phase ^= 1;
-  }
-  // Copies still in flight (none hold data after a whole walk; after a wait that gave up they may) land before the
-  // ring is reused below.
-  for (int i = 0; i < ST; i++) {
-    mbar_wait(&full[stage], phase, a.status);
-    if (++stage == ST) stage = 0, phase ^= 1;
-  }
-  ok = __syncthreads_and(ok);
-
-  // ---- join the warps ----
-  constexpr int RS = DH + 2;
-  float* buf = reinterpret_cast<float*>(smem);  // [NW][RB][RS]
-  static_assert((size_t)NW * RB * RS * 4 <= (size_t)NW * ST * SB, "the warps' sums fit the rings");
-#pragma unroll
-  for (int nc = 0; nc < NC; nc++)
-#pragma unroll
-    for (int r = 0; r < NR; r++) {
-      float l = L[nc][r];
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-      float* w = buf + (warp * RB + nc * RG + t * NR + r) * RS;
-#pragma unroll
-      for (int i = 0; i < NB; i++)
-#pragma unroll
-        for (int m = 0; m < 2; m++) {
-          const float* o4 = O[2 * i + m][nc];
-          const int d = 32 * i + 4 * g + 2 * m;
-          w[d] = TERMS == 2 ? o4[0] + o4[1] : o4[r];
-          w[d + 1] = (TERMS == 2 ? o4[2] + o4[3] : o4[2 + r]) * 0.0625f;
-        }
-      if (g == 0) w[DH] = M[nc][r], w[DH + 1] = l;
-    }
-  __syncthreads();
-  const int unit = ((b * a.kv.KV + kvh) * a.nrb) + (int)(blockIdx.z % a.nrb);
-  float* mine = a.part + ((size_t)unit * gridDim.x + split) * RB * RS;
-  for (int i = threadIdx.x; i < RB * DH; i += 32 * NW) {
-    const int r = i / DH, d = i % DH;
-    if (r >= rows) break;
-    float m = kNoM;
-#pragma unroll
-    for (int w = 0; w < NW; w++) m = fmaxf(m, buf[(w * RB + r) * RS + DH]);
-    float o = 0.f, l = 0.f;
-#pragma unroll
-    for (int w = 0; w < NW; w++) {
-      const float f = exp2f(buf[(w * RB + r) * RS + DH] - m);
-      o = fmaf(buf[(w * RB + r) * RS + d], f, o);
-      l = fmaf(buf[(w * RB + r) * RS + DH + 1], f, l);
-    }
-    if (nsplit == 1) {
+    __syncthreads();
+    const int unit = (b * a.kv.KV + kvh) * a.nrb + rb;
+    const int n_parts = unit_last - unit_first + 1;
+    auto out_at = [&](int r, int d) {
       const int rr = r0 + r, s = rr / a.G, h = kvh * a.G + rr % a.G;
-      const float y = l > 0.f ? o / l : (l == 0.f ? 0.f : l);  // no token: zeros; NaN stays
-      store_dt(a.out, (((size_t)b * a.S + s) * a.H + h) * DH + d, a.dtype, y);
-    } else {
-      mine[r * RS + d] = o;
-      if (d == 0) mine[r * RS + DH] = m, mine[r * RS + DH + 1] = l;
+      return (((size_t)b * a.S + s) * a.H + h) * DH + d;
+    };
+    auto finish = [&](float (&o)[4], float l, int r, int d) {
+      const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no token: zeros; NaN stays
+#pragma unroll
+      for (int k = 0; k < 4; k++) o[k] *= f;
+      store4_dt(a.out, out_at(r, d), a.dtype, o);
+    };
+    // A CTA's segment that begins its unit is its last one (record 1), one that continues a unit its first (record 0).
+    float* mine = a.part + ((size_t)blockIdx.x * 2 + (unit_first == (int)blockIdx.x ? 1 : 0)) * REC;
+    for (int i = threadIdx.x; i < rows * (DH / 4); i += 32 * NW) {
+      const int r = i / (DH / 4), d = 4 * (i % (DH / 4));
+      float m = kNoM, wm[NW];
+#pragma unroll
+      for (int w = 0; w < NW; w++) wm[w] = buf[(w * RB + r) * RS + DH], m = fmaxf(m, wm[w]);
+      float o[4] = {}, l = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; w++) {
+        const float f = exp2f(wm[w] - m);
+        const float4 v = *reinterpret_cast<const float4*>(buf + (w * RB + r) * RS + d);
+        o[0] = fmaf(v.x, f, o[0]), o[1] = fmaf(v.y, f, o[1]), o[2] = fmaf(v.z, f, o[2]), o[3] = fmaf(v.w, f, o[3]);
+        l = fmaf(buf[(w * RB + r) * RS + DH + 1], f, l);
+      }
+      if (n_parts == 1) {
+        finish(o, l, r, d);
+      } else {
+        *reinterpret_cast<float4*>(mine + r * DH + d) = make_float4(o[0], o[1], o[2], o[3]);
+        if (d == 0) *reinterpret_cast<float2*>(mine + RB * DH + 2 * r) = make_float2(m, l);
+      }
     }
-  }
-  if (nsplit == 1) return;
 
-  // ---- join the splits: the CTA that draws the unit's last ticket ----
-  __shared__ int last;
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0) last = atomicAdd(&a.tickets[unit], 1) == nsplit - 1;
-  __syncthreads();
-  if (!last) return;
-  __threadfence();
-  const float* all = a.part + (size_t)unit * gridDim.x * RB * RS;
-  for (int i = threadIdx.x; i < rows * DH; i += 32 * NW) {
-    const int r = i / DH, d = i % DH;
-    float m = kNoM, o = 0.f, l = 0.f;
-    for (int s = 0; s < nsplit; s++) m = fmaxf(m, __ldcg(all + (size_t)s * RB * RS + r * RS + DH));
-    for (int s = 0; s < nsplit; s++) {
-      const float* p = all + (size_t)s * RB * RS + r * RS;
-      const float f = exp2f(__ldcg(p + DH) - m);
-      o = fmaf(__ldcg(p + d), f, o);
-      l = fmaf(__ldcg(p + DH + 1), f, l);
+    // ---- join the unit's segments: the CTA that draws the last ticket ----
+    if (n_parts > 1) {
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        s_last = atomicAdd(&a.tickets[unit], 1) == n_parts - 1;
+        if (s_last) a.tickets[unit] = 0;  // re-armed for the next call
+      }
+      __syncthreads();
+      if (s_last) {
+        __threadfence();
+        auto record = [&](int i) { return a.part + ((size_t)(unit_first + i) * 2 + (i == 0 ? 1 : 0)) * REC; };
+        // Weights of the records first (a warp per row), then the sums: many loads in flight in both.
+        float* wt = reinterpret_cast<float*>(smem);  // [RB][kParts] weights, then [RB] sums
+        constexpr int kParts = (int)(((size_t)NW * ST * SB / 4 - 64) / RB);
+        for (int r = warp; r < rows; r += NW) {
+          float m = kNoM, l = 0.f;
+          for (int i = lane; i < n_parts; i += 32) m = fmaxf(m, __ldcg(record(i) + RB * DH + 2 * r));
+          m = warp_max(m);
+          for (int i = lane; i < n_parts; i += 32) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(record(i) + RB * DH + 2 * r));
+            const float f = exp2f(ml.x - m);
+            if (i < kParts) wt[r * kParts + i] = f;
+            l = fmaf(ml.y, f, l);
+          }
+          l = warp_sum(l);
+          if (lane == 0) wt[RB * kParts + r] = l;
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < rows * (DH / 4); i += 32 * NW) {
+          const int r = i / (DH / 4), d = 4 * (i % (DH / 4));
+          float o[4] = {};
+          for (int p0 = 0; p0 < n_parts; p0 += 8) {
+            float4 v[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+              v[k] = __ldcg(reinterpret_cast<const float4*>(record(min(p0 + k, n_parts - 1)) + r * DH + d));
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+              const float f = p0 + k < n_parts ? wt[r * kParts + p0 + k] : 0.f;
+              if (p0 + k < n_parts)
+                o[0] = fmaf(v[k].x, f, o[0]), o[1] = fmaf(v[k].y, f, o[1]), o[2] = fmaf(v[k].z, f, o[2]), o[3] = fmaf(v[k].w, f, o[3]);
+            }
+          }
+          finish(o, wt[RB * kParts + r], r, d);
+        }
+      }
     }
-    const int rr = r0 + r, s = rr / a.G, h = kvh * a.G + rr % a.G;
-    const float y = l > 0.f ? o / l : (l == 0.f ? 0.f : l);
-    store_dt(a.out, (((size_t)b * a.S + s) * a.H + h) * DH + d, a.dtype, y);
+    fence_proxy_async();  // this segment's plain writes to the rings come before the next one's copies
+    if (!__syncthreads_and(ok)) return;  // a wait gave up (reported)
   }
-  if (threadIdx.x == 0) a.tickets[unit] = 0;  // re-armed for the next call
 }
 
 template <int DH, int TERMS, int NC>
-int launch(hcu_context* h, PagedAttnArgs a, int batch) {
+int launch(hcu_context* h, PagedAttnArgs a) {
   const char* op = "hcu_attention_paged";
   constexpr int RB = 8 * NC / TERMS;
-  constexpr size_t smem = paged_smem(DH);
+  constexpr size_t smem = paged_smem(DH), record = (size_t)RB * (DH + 2) * sizeof(float);
   auto kern = attn_paged_kernel<DH, TERMS, NC>;
   static std::atomic<uint64_t> attr_done{0};  // per device
   HCU_TRY(once_per_device(attr_done, h->device, [&]() -> int {
     return check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), op);
   }));
   a.nrb = (a.R + RB - 1) / RB;
-  const long long units = (long long)batch * a.kv.KV * a.nrb;
-  if ((long long)batch * a.nrb > 65535) return fail(HCU_EINVAL, "%s: batch x query row blocks > 65535", op);
-  // Keys per split: enough CTAs for several rounds of the GPU, which evens out sequences of different lengths, but no
-  // fewer than one round of the warps.
-  const int span = a.window > 0 ? (int)std::min<long long>(a.max_context, (long long)a.window + a.S + CHUNK) : a.max_context;
-  const int chunks = std::max(1, (span + CHUNK - 1) / CHUNK + 1);
-  const long long want = std::max(1LL, (8LL * 2 * h->sm_count + units - 1) / units);
-  int cps = (int)std::max<long long>(NW, (chunks + want - 1) / want);
-  if (h->opt_attn_chunk > 0) cps = (int)std::max<long long>(1, std::min<long long>((h->opt_attn_chunk + CHUNK - 1) / CHUNK, chunks));
-  cps = std::max(cps, (chunks + kMaxPagedSplits - 1) / kMaxPagedSplits);
-  int splits = (chunks + cps - 1) / cps;
-  const size_t record = (size_t)RB * (DH + 2) * sizeof(float);
+  const long long units = (long long)a.batch * a.kv.KV * a.nrb;
+  if (units > 0x7fffffffLL) return fail(HCU_EINVAL, "%s: batch x KV x query row blocks too large", op);
+  long long grid = (long long)h->sm_count * paged_ctas(DH, NC);
   const size_t room = h->workspace_bytes > kTicketBytes ? h->workspace_bytes - kTicketBytes : 0;
-  const long long fit = (long long)(room / (record * (size_t)units));
-  if (units > kMaxUnits || fit < 2) {
-    cps = chunks, splits = 1;  // no room for partial sums: one CTA walks all keys
-  } else if (splits > fit) {
-    cps = (int)((chunks + fit - 1) / fit);
-    splits = (chunks + cps - 1) / cps;
+  const long long span = a.window > 0 ? std::min<long long>(a.max_context, (long long)a.window + a.S + CHUNK) : a.max_context;
+  const long long most = units * (span / CHUNK + 2);  // chunks
+  a.split = units <= kMaxUnits && room >= (size_t)grid * 2 * record && most < 0x7fffffffLL;
+  a.min_chunks = h->opt_attn_chunk > 0 ? (int)std::min<int64_t>(1 << 24, (h->opt_attn_chunk + CHUNK - 1) / CHUNK) : 8;
+  if (a.split) {
+    grid = std::min(grid, (most + a.min_chunks - 1) / a.min_chunks);
+  } else {
+    grid = std::min(grid, units);
   }
-  a.cps = cps;
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(h->workspace) + kTicketBytes);
   a.tickets = static_cast<int*>(h->workspace);
-  kern<<<dim3((unsigned)splits, (unsigned)a.kv.KV, (unsigned)(batch * a.nrb)), 32 * NW, smem, h->stream>>>(a);
+  kern<<<(unsigned)grid, 32 * NW, smem, h->stream>>>(a);
   return after_launch("hcu_attention_paged: launch");
 }
 
 template <int DH>
-int launch_dh(hcu_context* h, const PagedAttnArgs& a, int batch) {
-  // One f16 number per query where the result is rounded to bf16 anyway and the rows fill more than four columns.
-  if (a.R <= 4) return launch<DH, 2, 1>(h, a, batch);
-  if (a.dtype == HCU_DT_BF16) return a.R <= 8 ? launch<DH, 1, 1>(h, a, batch) : launch<DH, 1, 2>(h, a, batch);
-  return launch<DH, 2, 2>(h, a, batch);
+int launch_dh(hcu_context* h, const PagedAttnArgs& a) {
+  // One f16 number per query where the result is rounded to bf16 anyway and the rows need the columns.
+#ifndef T1
+  if (a.R <= 4) return launch<DH, 2, 1>(h, a);
+#endif
+  if (a.dtype == HCU_DT_BF16) return a.R <= 8 ? launch<DH, 1, 1>(h, a) : launch<DH, 1, 2>(h, a);
+  return launch<DH, 2, 2>(h, a);
 }
 
 }  // namespace
@@ -620,5 +829,6 @@ extern "C" int hcu_attention_paged(hcu_handle h, const hcu_attention_paged_param
   a.status = h->dev_status;
   a.R = a.S * a.G;
   a.dtype = (int)p->dtype;
-  return kv->Dh == 128 ? hcu::launch_dh<128>(h, a, (int)p->batch) : hcu::launch_dh<256>(h, a, (int)p->batch);
+  a.batch = (int)p->batch;
+  return kv->Dh == 128 ? hcu::launch_dh<128>(h, a) : hcu::launch_dh<256>(h, a);
 }
