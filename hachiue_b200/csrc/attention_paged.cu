@@ -49,9 +49,9 @@ struct PagedAttnArgs {
   const int32_t* context;
   int batch, S, H, G, R, nrb, window, max_context, table_stride;
   int min_chunks;    // fewest chunks of 32 tokens worth a CTA of their own
-  int split;         // 0: every unit is one CTA's (no room for partial sums)
+  int split;         // 0: every unit is one warp's (no room for partial sums)
   float scale_log2;  // log2(e) / sqrt(Dh)
-  float* part;       // [gridDim.x][2] records of a CTA's first and last segment: sums [RB][DH], then (M, l) [RB]
+  float* part;       // [gridDim.x][2] records of the units at a CTA's two ends: sums [RB][DH], then (M, l) [RB]
   int* tickets;      // [units], 0 between calls
   uint32_t* status;
   int dtype;
@@ -138,32 +138,33 @@ __device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
   return d;
 }
 
-// Barrier operations on a shared-memory address.
-__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+// 16 bytes from global into shared memory by the asynchronous copy unit; nothing is read and zeros are written unless `there`.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+constexpr int kMaxParts = 320;  // CTAs of a call, and so of a unit
+constexpr int STAGES = 2;
 constexpr int paged_stage_bytes(int dh) { return CHUNK * (dh + dh / 8); }  // codes and scales, keys and values
-constexpr int paged_stages(int dh) { return dh == 128 ? 3 : 2; }
-constexpr size_t paged_smem(int dh) { return 128 + (size_t)NW * paged_stages(dh) * (paged_stage_bytes(dh) + 8); }
+constexpr int paged_row_floats(int dh) { return dh + 4; }  // of the warps' sums (a multiple of four)
+constexpr size_t paged_smem(int dh, int rb) {
+  return (size_t)NW * STAGES * paged_stage_bytes(dh) + (size_t)NW * rb * paged_row_floats(dh) * 4 + (rb > 8 ? (size_t)rb * (kMaxParts + 1) * 4 : 0);
+}
 constexpr int paged_ctas(int dh, int nc) { return dh == 128 && nc == 1 ? 2 : 1; }  // per SM
 
 // The work of a call is a line of chunks: sequence after sequence, in each
 // its KV heads, in each its row blocks, in each the chunks that hold visible tokens
 // (one empty chunk where there are none: zeros are to be written).  CTA i of n
-// takes the i-th of n equal pieces of the line, so a ragged batch and a single
-// long sequence keep every SM busy to the end alike.
+// takes the i-th of n equal pieces of the line and each of its warps an
+// eighth of that, so a ragged batch and a single long sequence keep every warp
+// busy to the end alike, and no warp waits for another before that.  A unit (a
+// sequence's KV head and row block) that lies within a warp's piece is
+// finished by that warp; the others leave records that are joined at the end.
 struct PagedPlan {
   int total, share, more;  // chunks (below 2^31: the host checks); per CTA; the first `more` CTAs take one more
   int ctas;
@@ -184,20 +185,26 @@ __device__ __forceinline__ int2 paged_chunks(const PagedAttnArgs& a, int b) {
   return make_int2(c_lo, max(1, c_hi - c_lo));
 }
 
-// TERMS f16 numbers per query, NC groups of eight columns: RB = 8 NC / TERMS rows per CTA.
-template <int DH, int TERMS, int NC>
+// TERMS f16 numbers per query, NC groups of eight columns: RB = 8 NC / TERMS
+// rows per warp.  EXACT: code - 8 for both operands (f32 results); otherwise
+// the codes as they are, the offset taken off the sums, whose larger terms
+// the tensor cores' f32 sums truncate (about 3e-6 of the result, measured).
+template <int DH, int TERMS, int NC, bool EXACT>
 __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel(const PagedAttnArgs a) {
-  constexpr int NB = DH / 32, ST = paged_stages(DH), SB = paged_stage_bytes(DH);
-  constexpr int RG = 8 / TERMS, RB = RG * NC;  // rows per column group, per CTA
+  constexpr int NB = DH / 32, ST = STAGES, SB = paged_stage_bytes(DH);
+  constexpr int RG = 8 / TERMS, RB = RG * NC;  // rows per column group, per warp
   constexpr int NR = 2 / TERMS;                // rows per thread and column group
   constexpr int KB = CHUNK * DH / 2, CB = CHUNK * NB * 2;  // bytes of a stage's codes, of its scales
-  constexpr int RS = DH + 4;                   // floats per row of the warps' sums (a multiple of four)
-  constexpr size_t REC = (size_t)RB * (DH + 2);  // floats of a segment's record
+  constexpr int RS = paged_row_floats(DH);
+  constexpr size_t REC = (size_t)RB * (DH + 2);  // floats of a global record
+  static_assert(RB * RS * 4 <= ST * SB, "a record fits a ring");
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int scan[NW], s_last, s_b, s_pos;
-  __shared__ float s_top[RB], s_back[8 * NC];     // per row; per column
-  __shared__ __align__(16) float s_corr[NC][NB][8];  // -8 sum(q) of a block per column (read in pairs)
-  __shared__ uint4 s_q[NC][NB][32];                               // the lanes' B fragments
+  // Records of a warp's units that lie only partly in its piece: [2w] the one that ends there, [2w + 1] the one that
+  // goes on.  u0 < 0: none.
+  __shared__ struct {
+    int u0, n, b, kvh, rb, begins;
+  } s_rec[2 * NW];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int tok = (g >> 1) + 4 * (g & 1);  // token of accumulator row g (row g + 8: 8 more)
 
@@ -205,7 +212,7 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
   const int per_chunk = a.kv.KV * a.nrb;  // units of a sequence, all of its chunk count
   PagedPlan plan;
   int seg_b, seg_base;  // sequence of the next segment, line position of its first chunk
-  int pos, end;
+  int pos, end, cta_first;
   {
     // Every thread sums a run of sequences; the line position of each run follows from a scan.
     const int run = (a.batch + 32 * NW - 1) / (32 * NW), b0 = threadIdx.x * run, b1 = min(a.batch, b0 + run);
@@ -226,20 +233,20 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
       total += scan[w];
     }
     plan.total = total * per_chunk;
-    const int most = a.split ? (plan.total - 1) / a.min_chunks + 1 : a.batch * per_chunk;
+    const int most = a.split ? (plan.total - 1) / a.min_chunks + 1 : (int)gridDim.x;
     plan.ctas = min((int)gridDim.x, most);
     plan.share = plan.total / plan.ctas;
     plan.more = plan.total % plan.ctas;
     if ((int)blockIdx.x >= plan.ctas) return;
+    if (threadIdx.x < 2 * NW) s_rec[threadIdx.x].u0 = -1;
     if (a.split) {
-      pos = plan.start(blockIdx.x);
-      end = plan.start(blockIdx.x + 1);
-      const int lo = (pre - sum) * per_chunk;
-      if (pos >= lo && pos < pre * per_chunk) {  // one thread's run holds the first chunk
+      cta_first = plan.start(blockIdx.x);
+      const int len = plan.start(blockIdx.x + 1) - cta_first, lo = (pre - sum) * per_chunk;
+      if (cta_first >= lo && cta_first < pre * per_chunk) {  // one thread's run holds the first chunk
         int at = lo, b = b0;
         for (;; b++) {
           const int n = paged_chunks(a, b).y * per_chunk;
-          if (pos < at + n) break;
+          if (cta_first < at + n) break;
           at += n;
         }
         s_b = b;
@@ -248,185 +255,201 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
       __syncthreads();
       seg_b = s_b;
       seg_base = s_pos;
-    } else {  // whole units, blockIdx.x-th and every gridDim.x-th after it
-      pos = blockIdx.x, end = a.batch * per_chunk;
+      pos = cta_first + (int)((long long)len * warp / NW);
+      end = cta_first + (int)((long long)len * (warp + 1) / NW);
+    } else {  // whole units: every (gridDim.x * NW)-th
+      __syncthreads();
+      cta_first = 0;
+      pos = blockIdx.x * NW + warp, end = a.batch * per_chunk;
       seg_b = 0, seg_base = 0;
     }
   }
 
-  // ---- this warp's ring ----
-  const uint32_t ring = smem_u32(smem) + warp * ST * SB;
-  const uint32_t full = smem_u32(smem + NW * ST * SB) + warp * ST * 8;
-  if (lane == 0) {
-    for (int i = 0; i < ST; i++) mbar_init(reinterpret_cast<uint64_t*>(smem + NW * ST * SB) + warp * ST + i, 1);
-    fence_barrier_init();
-  }
-  __syncwarp();
-  // A chunk is a part of one page or (16-token pages) two pages.  Lane 4s + w
-  // brings tensor w (key codes, value codes, key scales, value scales) of part s.
-  const int sub_log2 = min(a.kv.page_log2, 5), subs = CHUNK >> sub_log2;
-  const int is = lane >> 2, iw = lane & 3, row_bytes = iw < 2 ? DH / 2 : NB * 2;
-  const uint32_t part_bytes = row_bytes << sub_log2, all_bytes = (2 * KB + 2 * CB) / CHUNK << sub_log2;
-  const uint8_t* isrc = iw == 0 ? a.kv.k : iw == 1 ? a.kv.v : reinterpret_cast<const uint8_t*>(iw == 2 ? a.kv.ks : a.kv.vs);
-  const uint32_t idst = ring + (iw < 2 ? iw * KB : 2 * KB + (iw - 2) * CB) + is * part_bytes;
-  const uint32_t chunk_mask = max(1 << a.kv.page_log2, CHUNK) / CHUNK - 1;  // chunks of a page, less one
-  const uint32_t page_bytes = (uint32_t)a.kv.KV * row_bytes << a.kv.page_log2;
-  auto wait_full = [&](int st, uint32_t ph) {
-    return bar_try(full + 8 * st, ph) ||
-           mbar_wait(reinterpret_cast<uint64_t*>(smem + NW * ST * SB) + warp * ST + st, ph, a.status);
+  // The segment at line position `at` (or, unsplit, unit number `at`): chunks [c0, c1) of unit (b, kvh, rb), which
+  // begins at position u0 and has n chunks.  seq_b and seq_base walk along.
+  struct Segment {
+    int b, kvh, rb, c0, c1, u0, n;
   };
+  auto segment = [&](int at, int& seq_b, int& seq_base) -> Segment {
+    Segment s;
+    int u;
+    int2 ch;
+    if (a.split) {
+      ch = paged_chunks(a, seq_b);
+      while (at >= seq_base + ch.y * per_chunk) {
+        seq_base += ch.y * per_chunk;
+        ch = paged_chunks(a, ++seq_b);
+      }
+      s.b = seq_b;
+      u = (at - seq_base) / ch.y;
+      s.u0 = seq_base + u * ch.y;
+      s.c0 = ch.x + at - s.u0;
+      s.c1 = ch.x + min(ch.y, end - s.u0);
+    } else {
+      s.b = at / per_chunk;
+      u = at % per_chunk;
+      ch = paged_chunks(a, s.b);
+      s.u0 = at;
+      s.c0 = ch.x, s.c1 = ch.x + ch.y;
+    }
+    s.n = ch.y;
+    s.kvh = u / a.nrb, s.rb = u % a.nrb;
+    return s;
+  };
+  auto after = [&](int at, const Segment& s) { return a.split ? at + s.c1 - s.c0 : at + (int)gridDim.x * NW; };
+
+  // ---- this warp's ring: the chunks it will take, fetched ahead across segments ----
+  const uint32_t ring = smem_u32(smem) + warp * ST * SB;
+  float* buf = reinterpret_cast<float*>(smem + NW * ST * SB);  // [NW][RB][RS]: sums, M, l
+  const int page_mask = (1 << a.kv.page_log2) - 1;
+  int f_pos = pos, f_seq = seg_b, f_base = seg_base;  // the segment being fetched begins at f_pos
+  Segment f{};
+  int f_c = 0, f_lo, f_hi;
+  const int32_t* f_table;
+  // The tokens of a fetched sequence that any query sees, [f_lo, f_hi).
+  auto fetch_seq = [&]() {
+    int ctx = a.context[f.b];
+    if (ctx > a.max_context || ctx < 0) ctx = 0;
+    f_hi = ctx;
+    f_lo = a.window > 0 ? max(0, ctx - a.S + 1 - a.window) : 0;
+    f_table = a.table + (size_t)f.b * a.table_stride;
+  };
+  // The pages of chunk c's two halves of 16 tokens: -2 where no query sees a token of the half (not looked up).
+  auto look_up = [&](int c, int (&pg)[2]) {
+#pragma unroll
+    for (int p = 0; p < 2; p++) {
+      const int t0 = c * CHUNK + 16 * p;
+      pg[p] = c < f.c1 && t0 < f_hi && t0 + 16 > f_lo ? f_table[t0 >> a.kv.page_log2] : -2;
+    }
+  };
+  int f_page[2] = {-2, -2};
+  auto enter = [&]() {  // the segment at f_pos
+    f = segment(f_pos, f_seq, f_base);
+    f_c = f.c0;
+    fetch_seq();
+    // its queries will be read soon
+    const char* q = static_cast<const char*>(a.q) + (((size_t)f.b * a.S * a.H + f.kvh * a.G) * DH + lane * 32) * (a.dtype == HCU_DT_F32 ? 4 : 2);
+    if (lane * 32 < min(a.G, RB) * DH) asm volatile("prefetch.global.L2 [%0];" ::"l"(q));
+  };
+  if (pos < end) {
+    enter();
+    look_up(f_c, f_page);
+  }
+  // Fetches the next chunk into a stage and looks the one after it up.  Returns which halves hold data.
+  auto fetch = [&](int st) -> uint32_t {
+    uint32_t halves = 0;
+    if (f_c < f.c1) {
+      const uint32_t dst = ring + st * SB;
+      long long row[2];
+#pragma unroll
+      for (int p = 0; p < 2; p++) {
+        const bool there = (uint32_t)f_page[p] < (uint32_t)a.kv.n_pages;
+        if (!there && f_page[p] != -2 && lane == 0) atomicOr(a.status, HCU_DEVERR_BADARG);  // the table's entry is no page
+        halves |= (there ? 1u : 0u) << p;
+        row[p] = paged_row(a.kv, there ? f_page[p] : 0, f.kvh, (f_c * CHUNK + 16 * p) & page_mask);
+      }
+      const bool there[2] = {(halves & 1u) != 0, (halves & 2u) != 0};
+#pragma unroll
+      for (int p = 0; p < 2; p++) {
+        const uint8_t* k = a.kv.k + row[p] * (DH / 2) + lane * 16;
+        const uint8_t* v = a.kv.v + row[p] * (DH / 2) + lane * 16;
+        const uint32_t d = dst + p * (KB / 2) + lane * 16;
+#pragma unroll
+        for (int i = 0; i < KB / 1024; i++) {
+          copy16(d + 512 * i, k + 512 * i, there[p]);
+          copy16(d + KB + 512 * i, v + 512 * i, there[p]);
+        }
+      }
+      // scales: CB / 32 lanes per half, key scales then value scales
+      constexpr int LH = CB / 32;
+#pragma unroll
+      for (int i = 0; i < 4 * LH; i += 32) {
+        const int l = i + lane, p = (l / LH) & 1;
+        const __half* src = (l / (2 * LH) ? a.kv.vs : a.kv.ks) + (p ? row[1] : row[0]) * NB + (l % LH) * 8;
+        copy16(dst + 2 * KB + l * 16, src, p ? there[1] : there[0]);
+      }
+      if (++f_c == f.c1 && (f_pos = after(f_pos, f)) < end) enter();
+      look_up(f_c, f_page);
+    }
+    copy_commit();
+    return halves;
+  };
+  uint32_t have = 0;  // two bits per stage
+#pragma unroll
+  for (int i = 0; i < ST; i++) have |= fetch(i) << (2 * i);
   int stage = 0;
-  uint32_t phase = 0;
-  bool ok = true;
 
   while (pos < end) {
-    // ---- the segment: chunks [c0, c1) of unit (b, kvh, rb) ----
-    int b, kvh, rb, c0, c1, unit_first, unit_last;  // the unit's first and last CTA
-    if (a.split) {
-      int2 ch = paged_chunks(a, seg_b);
-      while (pos >= seg_base + ch.y * per_chunk) {
-        seg_base += ch.y * per_chunk;
-        ch = paged_chunks(a, ++seg_b);
-      }
-      const int u = (pos - seg_base) / ch.y, u0 = seg_base + u * ch.y;
-      b = seg_b, kvh = u / a.nrb, rb = u % a.nrb;
-      c0 = ch.x + pos - u0;
-      c1 = ch.x + min(ch.y, end - u0);
-      unit_first = plan.cta_of(u0), unit_last = plan.cta_of(u0 + ch.y - 1);
-      pos = min(end, u0 + ch.y);
-    } else {
-      b = pos / per_chunk;
-      const int u = pos % per_chunk;
-      kvh = u / a.nrb, rb = u % a.nrb;
-      const int2 ch = paged_chunks(a, b);
-      c0 = ch.x, c1 = ch.x + ch.y;
-      unit_first = unit_last = blockIdx.x;
-      pos += gridDim.x;
-    }
+    const Segment sg = segment(pos, seg_b, seg_base);
+    const int b = sg.b, kvh = sg.kvh, rb = sg.rb, c1 = sg.c1;
+    const bool begins = pos == sg.u0, ends = !a.split || sg.u0 + sg.n == pos + c1 - sg.c0;
+    pos = after(pos, sg);
     const int r0 = rb * RB, rows = min(RB, a.R - r0);
     int ctx = a.context[b];
     if (ctx > a.max_context || ctx < 0) {
-      if (threadIdx.x == 0) atomicOr(a.status, HCU_DEVERR_BADARG);
+      if (lane == 0) atomicOr(a.status, HCU_DEVERR_BADARG);
       ctx = 0;
     }
-    // The tokens that some row of this block sees, [lo, hi), and those that all see, [lo_all, hi_all).
+    // The tokens that every row of this block sees: [lo_all, hi_all).
     const int pos_first = ctx - a.S + r0 / a.G, pos_last = ctx - a.S + (r0 + rows - 1) / a.G;
-    const int lo = a.window > 0 ? max(0, pos_first + 1 - a.window) : 0, hi = max(0, pos_last + 1);
     const int lo_all = a.window > 0 ? max(0, pos_last + 1 - a.window) : 0, hi_all = max(0, pos_first + 1);
-    const int32_t* table = a.table + (size_t)b * a.table_stride;
-    const uint8_t* head_src = isrc + ((long long)kvh << a.kv.page_log2) * row_bytes;
-
-    // The page of this lane's part of chunk c: -2 where no row sees a token of it (not looked up), -1 where the table's
-    // entry is no page.
-    const int part_at = is << sub_log2, part_hi = is < subs ? min(hi, c1 * CHUNK) - part_at : -1,
-              part_lo = lo - part_at - (1 << sub_log2);
-    auto page_of = [&](int c) -> int {
-      if (c * CHUNK >= part_hi || c * CHUNK <= part_lo) return -2;
-      const int page = table[(c * CHUNK + part_at) >> a.kv.page_log2];
-      return (uint32_t)page < (uint32_t)a.kv.n_pages ? page : -1;
-    };
-    // Returns which parts hold data.
-    auto issue = [&](int c, int st, int page) -> uint32_t {
-      const uint32_t got = __ballot_sync(0xffffffffu, page >= 0);
-      const uint32_t parts = (got & 1u) | ((got >> 3) & 2u);  // lanes 0 and 4
-      if (lane == 0) bar_expect(full + 8 * st, (parts & 1u) * all_bytes + (parts >> 1) * all_bytes);
-      __syncwarp();
-      if (page >= 0) {
-        const uint8_t* src = head_src + (uint64_t)(uint32_t)page * page_bytes + ((uint32_t)c & chunk_mask) * (uint32_t)(CHUNK * row_bytes);
-        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                         idst + st * SB),
-                     "l"(src), "r"(part_bytes), "r"(full + 8 * st)
-                     : "memory");
-      } else if (page == -1) {
-        atomicOr(a.status, HCU_DEVERR_BADARG);
-      }
-      return parts;
-    };
-    uint32_t have = 0;  // two bits per stage
-    int next_page;
-    {
-      int pg[ST];
-#pragma unroll
-      for (int i = 0; i < ST; i++) pg[i] = page_of(c0 + warp + i * NW);
-      next_page = page_of(c0 + warp + ST * NW);
-#pragma unroll
-      for (int i = 0; i < ST; i++) {
-        const int st = stage + i >= ST ? stage + i - ST : stage + i;
-        have |= issue(c0 + warp + i * NW, st, pg[i]) << (2 * st);
-      }
-    }
-
-    // ---- query columns, prepared once for the CTA ----
-    for (int r = warp; r < RB; r += NW) {  // the rows' largest magnitudes
-      float top = 0.f;
-      if (r < rows) {
-        const int s = (r0 + r) / a.G, h = kvh * a.G + (r0 + r) % a.G;
-#pragma unroll
-        for (int j = 0; j < DH / 128; j++) {
-          float x[4];
-          load4_dt(a.q, (((size_t)b * a.S + s) * a.H + h) * DH + 128 * j + 4 * lane, a.dtype, x);
-          top = fmaxf(top, fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
-        }
-      }
-      top = warp_max(top);
-      if (lane == 0) s_top[r] = top;
-    }
-    __syncthreads();
-    for (int k = warp; k < NC * NB; k += NW) {  // group nc, block i; column g of the group is row / term of the lane's fragment
-      const int nc = k / NB, i = k % NB, r = nc * RG + (TERMS == 2 ? g >> 1 : g);
-      float q[8] = {};
-      if (r < rows) {
-        const int s = (r0 + r) / a.G, h = kvh * a.G + (r0 + r) % a.G;
-        const size_t at = (((size_t)b * a.S + s) * a.H + h) * DH + 32 * i + 8 * t;
-        float x[4], y[4];
-        load4_dt(a.q, at, a.dtype, x);
-        load4_dt(a.q, at + 4, a.dtype, y);
-#pragma unroll
-        for (int c = 0; c < 4; c++) q[c] = x[c], q[c + 4] = y[c];
-      }
-      // 2^sq brings the row's largest magnitude into [2^13, 2^14)
-      const float top = s_top[r];
-      const int sq = top > 0.f ? max(-126, min(127, 140 - (int)(__float_as_uint(top) >> 23))) : 0;
-      const float up = __uint_as_float((uint32_t)(sq + 127) << 23);
-      float sum = 0.f;
-      uint32_t w[4];
-#pragma unroll
-      for (int m = 0; m < 4; m++) {
-        // register m: dimensions m and m + 4 of the lane's eight; odd m meets codes times 16
-        __half o[2];
-#pragma unroll
-        for (int c = 0; c < 2; c++) {
-          float v = q[m + 4 * c] * up;
-          if (TERMS == 2 && (g & 1)) v -= __half2float(__float2half_rn(v));
-          o[c] = __float2half_rn((m & 1) ? v * 0.0625f : v);
-          sum += __half2float(o[c]) * ((m & 1) ? 16.f : 1.f);
-        }
-        w[m] = h2_bits(__halves2half2(o[0], o[1]));
-      }
-      s_q[nc][i][lane] = make_uint4(w[0], w[1], w[2], w[3]);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      if (t == 0) {
-        s_corr[nc][i][g] = sum * (-8.f * 5.9604644775390625e-08f);  // -8 * 2^-24
-        if (i == 0) s_back[8 * nc + g] = ldexpf(a.scale_log2, 24 - sq);
-      }
-    }
-    __syncthreads();
+    // ---- query columns: column g of group nc is row / term of this lane's B fragments ----
     uint32_t qf[NC][NB][4];
-    float corr[NC][NB][NR];  // rows of this thread's accumulator columns 2t, 2t + 1
+    float corr[NC][NB][NR];  // -8 sum(q) of the block (not EXACT), rows of this thread's accumulator columns 2t, 2t + 1
     float rs[NC][NR];        // score = rs * accumulated sum
 #pragma unroll
     for (int nc = 0; nc < NC; nc++) {
+      const int r = nc * RG + (TERMS == 2 ? g >> 1 : g);
+      const bool there = r < rows;
+      const int rr = r0 + (there ? r : 0), s = rr / a.G, h = kvh * a.G + rr % a.G;
+      const size_t at = (((size_t)b * a.S + s) * a.H + h) * DH;
+      float q[NB][8], top = 0.f;
 #pragma unroll
       for (int i = 0; i < NB; i++) {
-        const uint4 w = s_q[nc][i][lane];
-        qf[nc][i][0] = w.x, qf[nc][i][1] = w.y, qf[nc][i][2] = w.z, qf[nc][i][3] = w.w;
-        const float2 c = *reinterpret_cast<const float2*>(&s_corr[nc][i][2 * t]);
-        corr[nc][i][0] = TERMS == 2 ? c.x + c.y : c.x;
-        if (NR == 2) corr[nc][i][NR - 1] = c.y;
+        float x[4], y[4];
+        load4_dt(a.q, at + 32 * i + 8 * t, a.dtype, x);
+        load4_dt(a.q, at + 32 * i + 8 * t + 4, a.dtype, y);
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          q[i][c] = there ? x[c] : 0.f;
+          q[i][c + 4] = there ? y[c] : 0.f;
+          top = fmaxf(top, fmaxf(fabsf(q[i][c]), fabsf(q[i][c + 4])));
+        }
       }
-      rs[nc][0] = s_back[8 * nc + 2 * t];
-      if (NR == 2) rs[nc][NR - 1] = s_back[8 * nc + 2 * t + 1];
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^sq brings the row's largest magnitude into [2^13, 2^14)
+      const int sq = top > 0.f ? max(-126, min(127, 140 - (int)(__float_as_uint(top) >> 23))) : 0;
+      const float up = __uint_as_float((uint32_t)(sq + 127) << 23);
+      const float back = ldexpf(a.scale_log2, (EXACT ? 0 : 24) - sq);
+#pragma unroll
+      for (int i = 0; i < NB; i++) {
+        float sum = 0.f;
+#pragma unroll
+        for (int m = 0; m < 4; m++) {
+          // register m: dimensions m and m + 4 of the lane's eight; odd m meets codes times 16
+          __half o[2];
+#pragma unroll
+          for (int c = 0; c < 2; c++) {
+            float v = q[i][m + 4 * c] * up;
+            if (TERMS == 2 && (g & 1)) v -= __half2float(__float2half_rn(v));
+            o[c] = __float2half_rn((m & 1) ? v * 0.0625f : v);
+            if (!EXACT) sum += __half2float(o[c]) * ((m & 1) ? 16.f : 1.f);
+          }
+          qf[nc][i][m] = h2_bits(__halves2half2(o[0], o[1]));
+        }
+        if (!EXACT) {
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+          sum *= -8.f * 5.9604644775390625e-08f;  // -8 * 2^-24
+          // column 2t is lane group g = 2t, column 2t + 1 the next
+          const float u0 = __shfl_sync(0xffffffffu, sum, 8 * t), u1 = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+          corr[nc][i][0] = TERMS == 2 ? u0 + u1 : u0;
+          if (NR == 2) corr[nc][i][NR - 1] = u1;
+        }
+      }
+      rs[nc][0] = __shfl_sync(0xffffffffu, back, 8 * t);
+      if (NR == 2) rs[nc][NR - 1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
     }
 
     float O[2 * NB][NC][4] = {};
@@ -437,15 +460,13 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
 #pragma unroll
       for (int r = 0; r < NR; r++) M[nc][r] = T[nc][r] = kNoM, L[nc][r] = 0.f;
 
-    for (int c = c0 + warp; c < c1; c += NW) {
-      if (!__all_sync(0xffffffffu, wait_full(stage, phase))) {
-        ok = false;
-        break;
-      }
+    for (int c = sg.c0; c < c1; c++) {
+      copy_wait<ST - 1>();
+      __syncwarp();
       const uint32_t st = ring + stage * SB;
-      const uint32_t parts = (have >> (2 * stage)) & 3u;
+      const uint32_t halves = (have >> (2 * stage)) & 3u;
       const int base = c * CHUNK;
-      const bool whole = base >= lo_all && base + CHUNK <= hi_all && parts == (subs == 2 ? 3u : 1u);
+      const bool whole = base >= lo_all && base + CHUNK <= hi_all && halves == 3u;
       // ---- scores of 32 tokens ----
       float x[2][2][NC][NR];         // [16-token step][accumulator row half][..]: score, log2 units
       uint32_t vsw[2][2][NB / 2];    // value scales of the thread's tokens, f16 pairs
@@ -465,10 +486,17 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
         }
 #pragma unroll
         for (int i = 0; i < NB; i++) {
-          const uint32_t a0[4] = {kw[0][i] & 0x000f000fu, kw[1][i] & 0x000f000fu, kw[0][i] & 0x00f000f0u,
-                                  kw[1][i] & 0x00f000f0u};
+          uint32_t a0[4], a1[4];
           const uint32_t w0 = kw[0][i] >> 8, w1 = kw[1][i] >> 8;
-          const uint32_t a1[4] = {w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u};
+          if (EXACT) {
+            a0[0] = codes_f16<false>(kw[0][i]), a0[1] = codes_f16<false>(kw[1][i]);
+            a0[2] = codes_f16<true>(kw[0][i]), a0[3] = codes_f16<true>(kw[1][i]);
+            a1[0] = codes_f16<false>(w0), a1[1] = codes_f16<false>(w1), a1[2] = codes_f16<true>(w0), a1[3] = codes_f16<true>(w1);
+          } else {
+            a0[0] = kw[0][i] & 0x000f000fu, a0[1] = kw[1][i] & 0x000f000fu;
+            a0[2] = kw[0][i] & 0x00f000f0u, a0[3] = kw[1][i] & 0x00f000f0u;
+            a1[0] = w0 & 0x000f000fu, a1[1] = w1 & 0x000f000fu, a1[2] = w0 & 0x00f000f0u, a1[3] = w1 & 0x00f000f0u;
+          }
           float ks[2];
 #pragma unroll
           for (int u = 0; u < 2; u++) ks[u] = (i & 1) ? f16x2_to_f2(ksw[u][i / 2]).y : f16x2_to_f2(ksw[u][i / 2]).x;
@@ -479,12 +507,12 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
             mma16816(d, a1, qf[nc][i][2], qf[nc][i][3]);
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-              if (TERMS == 2) {
-                x[j][u][nc][0] = fmaf(ks[u], (d[2 * u] + corr[nc][i][0]) + d[2 * u + 1], x[j][u][nc][0]);
-              } else {
 #pragma unroll
-                for (int r = 0; r < NR; r++)
-                  x[j][u][nc][r] = fmaf(ks[u], d[2 * u + r] + corr[nc][i][r], x[j][u][nc][r]);
+              for (int r = 0; r < NR; r++) {
+                float sum = d[2 * u + r];
+                if (!EXACT) sum += corr[nc][i][r];
+                if (TERMS == 2) sum += d[2 * u + 1];
+                x[j][u][nc][r] = fmaf(ks[u], sum, x[j][u][nc][r]);
               }
             }
           }
@@ -500,7 +528,7 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
 #pragma unroll
           for (int u = 0; u < 2; u++) {
             const int at = base + 16 * j + 8 * u + tok;
-            const bool data = (parts >> (subs == 2 ? j : 0)) & 1u;
+            const bool data = (halves >> j) & 1u;
             bool any = false;
 #pragma unroll
             for (int nc = 0; nc < NC; nc++)
@@ -602,7 +630,7 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
           uint32_t z0 = __byte_perm(vw[0][i / 2], vw[1][i / 2], sel), z1 = __byte_perm(vw[2][i / 2], vw[3][i / 2], sel);
 #pragma unroll
           for (int m = 0; m < 2; m++) {
-            if (TERMS == 2) {
+            if (EXACT) {
               const uint32_t av[4] = {codes_f16<false>(z0), codes_f16<true>(z0), codes_f16<false>(z1), codes_f16<true>(z1)};
 #pragma unroll
               for (int nc = 0; nc < NC; nc++) mma16816(O[2 * i + m][nc], av, pb[nc][i][0], pb[nc][i][1]);
@@ -620,23 +648,16 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
           }
         }
       }
-      // ---- the stage is free: the chunk ST rounds on ----
+      // ---- the stage is free for the chunk ST rounds on ----
       __syncwarp();
-      have = (have & ~(3u << (2 * stage))) | issue(c + ST * NW, stage, next_page) << (2 * stage);
-      next_page = page_of(c + (ST + 1) * NW);
-      if (++stage == ST) stage = 0, phase ^= 1;
+      have = (have & ~(3u << (2 * stage))) | fetch(stage) << (2 * stage);
+      stage ^= 1;
     }
-    // Every stage has one phase left (without data after a whole walk): they are waited for before the rings are reused.
-    for (int i = 0; i < ST; i++) {
-      wait_full(stage, phase);
-      if (++stage == ST) stage = 0, phase ^= 1;
-    }
-    __syncthreads();
 
-    // ---- join the warps ----
-    constexpr float kUnscale = TERMS == 2 ? 1.f : 16777216.f;  // subnormal codes carry 2^-24
-    float* buf = reinterpret_cast<float*>(smem);  // [NW][RB][RS]: sums, M, l
-    static_assert((size_t)NW * RB * RS * 4 <= (size_t)NW * ST * SB, "the warps' sums fit the rings");
+    // ---- the segment's sums ----
+    constexpr float kUnscale = EXACT ? 1.f : 16777216.f;  // subnormal codes carry 2^-24
+    const bool complete = begins && ends;
+    float* rec = ends ? buf + warp * RB * RS : reinterpret_cast<float*>(smem + warp * ST * SB);
 #pragma unroll
     for (int nc = 0; nc < NC; nc++)
 #pragma unroll
@@ -644,114 +665,145 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
         float l = L[nc][r];
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        float* w = buf + (warp * RB + nc * RG + t * NR + r) * RS;
+        const int rl = nc * RG + t * NR + r;
+        const float f = complete ? (l > 0.f ? kUnscale / l : (l == 0.f ? 0.f : l)) : kUnscale;  // no token: zeros; NaN stays
+        float* w = rec + rl * RS;
 #pragma unroll
-        for (int i = 0; i < NB; i++)
-#pragma unroll
-          for (int m = 0; m < 2; m++) {
-            const float* o4 = O[2 * i + m][nc];
-            const int d = 32 * i + 4 * g + 2 * m;
-            *reinterpret_cast<float2*>(w + d) =
-                make_float2((TERMS == 2 ? o4[0] + o4[1] : o4[r]) * kUnscale,
-                            (TERMS == 2 ? o4[2] + o4[3] : o4[2 + r]) * (0.0625f * kUnscale));
+        for (int i = 0; i < NB; i++) {  // dimensions 32i + 4g .. + 3
+          const float *o0 = O[2 * i][nc], *o1 = O[2 * i + 1][nc];
+          float4 v;
+          v.x = (TERMS == 2 ? o0[0] + o0[1] : o0[r]) * f;
+          v.y = (TERMS == 2 ? o0[2] + o0[3] : o0[2 + r]) * (0.0625f * f);
+          v.z = (TERMS == 2 ? o1[0] + o1[1] : o1[r]) * f;
+          v.w = (TERMS == 2 ? o1[2] + o1[3] : o1[2 + r]) * (0.0625f * f);
+          if (complete) {
+            if (rl < rows) {
+              const int rr = r0 + rl, s = rr / a.G, h = kvh * a.G + rr % a.G;
+              const float y[4] = {v.x, v.y, v.z, v.w};
+              store4_dt(a.out, (((size_t)b * a.S + s) * a.H + h) * DH + 32 * i + 4 * g, a.dtype, y);
+            }
+          } else {
+            *reinterpret_cast<float4*>(w + 32 * i + 4 * g) = v;
           }
-        if (g == 0) w[DH] = M[nc][r], w[DH + 1] = l;
+        }
+        if (!complete && g == 0) w[DH] = M[nc][r], w[DH + 1] = l;
       }
-    __syncthreads();
-    const int unit = (b * a.kv.KV + kvh) * a.nrb + rb;
-    const int n_parts = unit_last - unit_first + 1;
-    auto out_at = [&](int r, int d) {
-      const int rr = r0 + r, s = rr / a.G, h = kvh * a.G + rr % a.G;
-      return (((size_t)b * a.S + s) * a.H + h) * DH + d;
+    if (!complete && lane == 0) {
+      auto& i = s_rec[2 * warp + (ends ? 0 : 1)];
+      i.u0 = sg.u0, i.n = sg.n, i.b = b, i.kvh = kvh, i.rb = rb, i.begins = begins;
+    }
+  }
+  __syncthreads();
+
+  // ---- join the records: neighbours of the same unit ----
+  for (int k = 0; k < 2 * NW;) {
+    const int u0 = s_rec[k].u0;
+    if (u0 < 0) {
+      k++;
+      continue;
+    }
+    uint32_t members = 0;
+    const int first = k;
+    int last = k;
+    for (; k < 2 * NW && (s_rec[k].u0 == u0 || s_rec[k].u0 < 0); k++)
+      if (s_rec[k].u0 == u0) members |= 1u << k, last = k;
+    const int n = s_rec[first].n, b = s_rec[first].b, kvh = s_rec[first].kvh, rb = s_rec[first].rb;
+    const bool whole = s_rec[first].begins && !(last & 1);  // no other CTA has a part of the unit
+    const int r0 = rb * RB, rows = min(RB, a.R - r0);
+    auto record_at = [&](int m) {
+      return (m & 1) ? reinterpret_cast<const float*>(smem + (m >> 1) * ST * SB) : buf + (m >> 1) * RB * RS;
     };
     auto finish = [&](float (&o)[4], float l, int r, int d) {
-      const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no token: zeros; NaN stays
+      const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
 #pragma unroll
-      for (int k = 0; k < 4; k++) o[k] *= f;
-      store4_dt(a.out, out_at(r, d), a.dtype, o);
+      for (int c = 0; c < 4; c++) o[c] *= f;
+      const int rr = r0 + r, s = rr / a.G, h = kvh * a.G + rr % a.G;
+      store4_dt(a.out, (((size_t)b * a.S + s) * a.H + h) * DH + d, a.dtype, o);
     };
-    // A CTA's segment that begins its unit is its last one (record 1), one that continues a unit its first (record 0).
-    float* mine = a.part + ((size_t)blockIdx.x * 2 + (unit_first == (int)blockIdx.x ? 1 : 0)) * REC;
+    // The unit's first CTA leaves its part in its second record, the others in their first.
+    float* mine = a.part + ((size_t)blockIdx.x * 2 + (u0 >= cta_first ? 1 : 0)) * REC;
     for (int i = threadIdx.x; i < rows * (DH / 4); i += 32 * NW) {
       const int r = i / (DH / 4), d = 4 * (i % (DH / 4));
-      float m = kNoM, wm[NW];
-#pragma unroll
-      for (int w = 0; w < NW; w++) wm[w] = buf[(w * RB + r) * RS + DH], m = fmaxf(m, wm[w]);
+      float m = kNoM;
+      for (uint32_t x = members; x; x &= x - 1) m = fmaxf(m, record_at(__ffs(x) - 1)[r * RS + DH]);
       float o[4] = {}, l = 0.f;
-#pragma unroll
-      for (int w = 0; w < NW; w++) {
-        const float f = exp2f(wm[w] - m);
-        const float4 v = *reinterpret_cast<const float4*>(buf + (w * RB + r) * RS + d);
+      for (uint32_t x = members; x; x &= x - 1) {
+        const float* w = record_at(__ffs(x) - 1) + r * RS;
+        const float f = exp2f(w[DH] - m);
+        const float4 v = *reinterpret_cast<const float4*>(w + d);
         o[0] = fmaf(v.x, f, o[0]), o[1] = fmaf(v.y, f, o[1]), o[2] = fmaf(v.z, f, o[2]), o[3] = fmaf(v.w, f, o[3]);
-        l = fmaf(buf[(w * RB + r) * RS + DH + 1], f, l);
+        l = fmaf(w[DH + 1], f, l);
       }
-      if (n_parts == 1) {
+      if (whole) {
         finish(o, l, r, d);
       } else {
         *reinterpret_cast<float4*>(mine + r * DH + d) = make_float4(o[0], o[1], o[2], o[3]);
         if (d == 0) *reinterpret_cast<float2*>(mine + RB * DH + 2 * r) = make_float2(m, l);
       }
     }
+    if (whole) continue;
 
-    // ---- join the unit's segments: the CTA that draws the last ticket ----
-    if (n_parts > 1) {
+    // ---- the unit's CTAs: the one that draws the last ticket joins them ----
+    const int unit = (b * a.kv.KV + kvh) * a.nrb + rb, unit_first = plan.cta_of(u0);
+    const int n_parts = plan.cta_of(u0 + n - 1) - unit_first + 1;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      s_last = atomicAdd(&a.tickets[unit], 1) == n_parts - 1;
+      if (s_last) a.tickets[unit] = 0;  // re-armed for the next call
+    }
+    __syncthreads();
+    if (s_last) {
       __threadfence();
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        s_last = atomicAdd(&a.tickets[unit], 1) == n_parts - 1;
-        if (s_last) a.tickets[unit] = 0;  // re-armed for the next call
+      auto record = [&](int i) { return a.part + ((size_t)(unit_first + i) * 2 + (i == 0 ? 1 : 0)) * REC; };
+      // Weights of the records first (a warp per row), then the sums: many loads in flight in both.
+      // Row r's weights, then its sum of probabilities: in the second stage of ring r, or an area of their own.
+      static_assert(RB > 8 || (RB * RS * 4 <= SB && (kMaxParts + 1) * 4 <= SB), "records and weights share the rings");
+      auto weights = [&](int r) {
+        return RB > 8 ? buf + NW * RB * RS + r * (kMaxParts + 1) : reinterpret_cast<float*>(smem + r * ST * SB + SB);
+      };
+      for (int r = warp; r < rows; r += NW) {
+        float m = kNoM, l = 0.f;
+        for (int i = lane; i < n_parts; i += 32) m = fmaxf(m, __ldcg(record(i) + RB * DH + 2 * r));
+        m = warp_max(m);
+        for (int i = lane; i < n_parts; i += 32) {
+          const float2 ml = __ldcg(reinterpret_cast<const float2*>(record(i) + RB * DH + 2 * r));
+          const float f = exp2f(ml.x - m);
+          weights(r)[i] = f;
+          l = fmaf(ml.y, f, l);
+        }
+        l = warp_sum(l);
+        if (lane == 0) weights(r)[kMaxParts] = l;
       }
       __syncthreads();
-      if (s_last) {
-        __threadfence();
-        auto record = [&](int i) { return a.part + ((size_t)(unit_first + i) * 2 + (i == 0 ? 1 : 0)) * REC; };
-        // Weights of the records first (a warp per row), then the sums: many loads in flight in both.
-        float* wt = reinterpret_cast<float*>(smem);  // [RB][kParts] weights, then [RB] sums
-        constexpr int kParts = (int)(((size_t)NW * ST * SB / 4 - 64) / RB);
-        for (int r = warp; r < rows; r += NW) {
-          float m = kNoM, l = 0.f;
-          for (int i = lane; i < n_parts; i += 32) m = fmaxf(m, __ldcg(record(i) + RB * DH + 2 * r));
-          m = warp_max(m);
-          for (int i = lane; i < n_parts; i += 32) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(record(i) + RB * DH + 2 * r));
-            const float f = exp2f(ml.x - m);
-            if (i < kParts) wt[r * kParts + i] = f;
-            l = fmaf(ml.y, f, l);
-          }
-          l = warp_sum(l);
-          if (lane == 0) wt[RB * kParts + r] = l;
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < rows * (DH / 4); i += 32 * NW) {
-          const int r = i / (DH / 4), d = 4 * (i % (DH / 4));
-          float o[4] = {};
-          for (int p0 = 0; p0 < n_parts; p0 += 8) {
-            float4 v[8];
+      for (int i = threadIdx.x; i < rows * (DH / 4); i += 32 * NW) {
+        const int r = i / (DH / 4), d = 4 * (i % (DH / 4));
+        float o[4] = {};
+        for (int p0 = 0; p0 < n_parts; p0 += 8) {
+          float4 v[8];
 #pragma unroll
-            for (int k = 0; k < 8; k++)
-              v[k] = __ldcg(reinterpret_cast<const float4*>(record(min(p0 + k, n_parts - 1)) + r * DH + d));
+          for (int c = 0; c < 8; c++)
+            v[c] = __ldcg(reinterpret_cast<const float4*>(record(min(p0 + c, n_parts - 1)) + r * DH + d));
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-              const float f = p0 + k < n_parts ? wt[r * kParts + p0 + k] : 0.f;
-              if (p0 + k < n_parts)
-                o[0] = fmaf(v[k].x, f, o[0]), o[1] = fmaf(v[k].y, f, o[1]), o[2] = fmaf(v[k].z, f, o[2]), o[3] = fmaf(v[k].w, f, o[3]);
-            }
+          for (int c = 0; c < 8; c++) {
+            const float f = p0 + c < n_parts ? weights(r)[p0 + c] : 0.f;
+            if (p0 + c < n_parts)
+              o[0] = fmaf(v[c].x, f, o[0]), o[1] = fmaf(v[c].y, f, o[1]), o[2] = fmaf(v[c].z, f, o[2]), o[3] = fmaf(v[c].w, f, o[3]);
           }
-          finish(o, wt[RB * kParts + r], r, d);
         }
+        finish(o, weights(r)[kMaxParts], r, d);
       }
     }
-    fence_proxy_async();  // this segment's plain writes to the rings come before the next one's copies
-    if (!__syncthreads_and(ok)) return;  // a wait gave up (reported)
+    __syncthreads();
   }
 }
 
-template <int DH, int TERMS, int NC>
+template <int DH, int TERMS, int NC, bool EXACT>
 int launch(hcu_context* h, PagedAttnArgs a) {
   const char* op = "hcu_attention_paged";
   constexpr int RB = 8 * NC / TERMS;
-  constexpr size_t smem = paged_smem(DH), record = (size_t)RB * (DH + 2) * sizeof(float);
-  auto kern = attn_paged_kernel<DH, TERMS, NC>;
+  constexpr size_t smem = paged_smem(DH, RB), record = (size_t)RB * (DH + 2) * sizeof(float);
+  auto kern = attn_paged_kernel<DH, TERMS, NC, EXACT>;
   static std::atomic<uint64_t> attr_done{0};  // per device
   HCU_TRY(once_per_device(attr_done, h->device, [&]() -> int {
     return check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), op);
@@ -759,7 +811,8 @@ int launch(hcu_context* h, PagedAttnArgs a) {
   a.nrb = (a.R + RB - 1) / RB;
   const long long units = (long long)a.batch * a.kv.KV * a.nrb;
   if (units > 0x7fffffffLL) return fail(HCU_EINVAL, "%s: batch x KV x query row blocks too large", op);
-  long long grid = (long long)h->sm_count * paged_ctas(DH, NC);
+  static_assert(smem <= (size_t)(227 * 1024), "shared memory");
+  long long grid = std::min(kMaxParts, h->sm_count * paged_ctas(DH, NC));
   const size_t room = h->workspace_bytes > kTicketBytes ? h->workspace_bytes - kTicketBytes : 0;
   const long long span = a.window > 0 ? std::min<long long>(a.max_context, (long long)a.window + a.S + CHUNK) : a.max_context;
   const long long most = units * (span / CHUNK + 2);  // chunks
@@ -768,7 +821,7 @@ int launch(hcu_context* h, PagedAttnArgs a) {
   if (a.split) {
     grid = std::min(grid, (most + a.min_chunks - 1) / a.min_chunks);
   } else {
-    grid = std::min(grid, units);
+    grid = std::min(grid, (units + NW - 1) / NW);
   }
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(h->workspace) + kTicketBytes);
   a.tickets = static_cast<int*>(h->workspace);
@@ -778,12 +831,17 @@ int launch(hcu_context* h, PagedAttnArgs a) {
 
 template <int DH>
 int launch_dh(hcu_context* h, const PagedAttnArgs& a) {
-  // One f16 number per query where the result is rounded to bf16 anyway and the rows need the columns.
-#ifndef T1
-  if (a.R <= 4) return launch<DH, 2, 1>(h, a);
-#endif
-  if (a.dtype == HCU_DT_BF16) return a.R <= 8 ? launch<DH, 1, 1>(h, a) : launch<DH, 1, 2>(h, a);
-  return launch<DH, 2, 2>(h, a);
+  if (a.dtype == HCU_DT_BF16) {
+    // One f16 number per query where the rows need the columns: its rounding (2^-11) is below the result's (2^-8).
+    if (a.R <= 4) return launch<DH, 2, 1, false>(h, a);
+    if constexpr (DH == 128)
+      if (a.R > 8) return launch<DH, 1, 2, false>(h, a);
+    return launch<DH, 1, 1, false>(h, a);
+  }
+  if (a.dtype == HCU_DT_F16 && a.R <= 4) return launch<DH, 2, 1, false>(h, a);
+  if constexpr (DH == 128)
+    if (a.R > 4) return launch<DH, 2, 2, true>(h, a);
+  return launch<DH, 2, 1, true>(h, a);
 }
 
 }  // namespace
