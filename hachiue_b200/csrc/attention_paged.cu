@@ -33,7 +33,6 @@
 // One CTA per (split of the key axis, KV head, block of query rows, sequence);
 // its eight warps take chunks of 32 tokens in turn, each with its own ring of
 // bulk copies, and never wait for one another until they join their sums.
-// Splits are joined by the CTA that draws the last ticket of its unit.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -52,13 +51,14 @@ struct PagedAttnArgs {
   int split;         // 0: every unit is one warp's (no room for partial sums)
   float scale_log2;  // log2(e) / sqrt(Dh)
   float* part;       // [gridDim.x][2] records of the units at a CTA's two ends: sums [RB][DH], then (M, l) [RB]
-  int* tickets;      // [units], 0 between calls
+  int4* open;        // [gridDim.x] the unit that begins in a CTA and goes on: parts (0: none), sequence, KV head, row block
   uint32_t* status;
   int dtype;
 };
 
 constexpr int NW = 8;          // warps of a CTA
 constexpr int CHUNK = 32;      // tokens a warp takes at a time
+constexpr int kUnitCost = 3;    // chunks that a unit's queries and sums cost a warp besides its chunks
 constexpr float kNoM = -1e30f;  // M of a row that has seen no token
 constexpr float kTop = 14.f, kStart = 4.f;  // weighted probabilities stay below 2^kTop; a moved M leaves the largest near 2^kStart
 
@@ -106,11 +106,29 @@ __device__ __forceinline__ void lds_words(uint32_t addr, uint32_t (&w)[N]) {
   }
 }
 
-// Four consecutive elements of a query row of any type.
-__device__ __forceinline__ void load4_dt(const void* p, size_t at, int dtype, float (&x)[4]) {
-  if (dtype == HCU_DT_F32) load4(static_cast<const float*>(p) + at, x);
-  else if (dtype == HCU_DT_F16) load4(static_cast<const __half*>(p) + at, x);
-  else load4(static_cast<const __nv_bfloat16*>(p) + at, x);
+// A lane's elements of a query row in shared memory: 32i + 8t .. + 7 of each block i.
+template <int NB>
+__device__ __forceinline__ void load_query(uint32_t row, int t, int dtype, float (&q)[NB][8]) {
+#pragma unroll
+  for (int i = 0; i < NB; i++) {
+    uint32_t w[4];
+    if (dtype == HCU_DT_F32) {
+      lds_words<4>(row + (32 * i + 8 * t) * 4, w);
+#pragma unroll
+      for (int c = 0; c < 4; c++) q[i][c] = __uint_as_float(w[c]);
+      lds_words<4>(row + (32 * i + 8 * t + 4) * 4, w);
+#pragma unroll
+      for (int c = 0; c < 4; c++) q[i][4 + c] = __uint_as_float(w[c]);
+    } else {
+      lds_words<4>(row + (32 * i + 8 * t) * 2, w);
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        const float2 h = f16x2_to_f2(w[c]);
+        q[i][2 * c] = dtype == HCU_DT_F16 ? h.x : bf16_lo(w[c]);
+        q[i][2 * c + 1] = dtype == HCU_DT_F16 ? h.y : bf16_hi(w[c]);
+      }
+    }
+  }
 }
 __device__ __forceinline__ void store4_dt(void* p, size_t at, int dtype, const float (&x)[4]) {
   if (dtype == HCU_DT_F32) store4(static_cast<float*>(p) + at, x);
@@ -153,7 +171,7 @@ constexpr int STAGES = 2;
 constexpr int paged_stage_bytes(int dh) { return CHUNK * (dh + dh / 8); }  // codes and scales, keys and values
 constexpr int paged_row_floats(int dh) { return dh + 4; }  // of the warps' sums (a multiple of four)
 constexpr size_t paged_smem(int dh, int rb) {
-  return (size_t)NW * STAGES * paged_stage_bytes(dh) + (size_t)NW * rb * paged_row_floats(dh) * 4 + (rb > 8 ? (size_t)rb * (kMaxParts + 1) * 4 : 0);
+  return (size_t)NW * STAGES * paged_stage_bytes(dh) + (size_t)NW * rb * paged_row_floats(dh) * 4;
 }
 constexpr int paged_ctas(int dh, int nc) { return dh == 128 && nc == 1 ? 2 : 1; }  // per SM
 
@@ -198,13 +216,15 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
   constexpr int RS = paged_row_floats(DH);
   constexpr size_t REC = (size_t)RB * (DH + 2);  // floats of a global record
   static_assert(RB * RS * 4 <= ST * SB, "a record fits a ring");
+  static_assert(RB * DH * (TERMS == 2 ? 4 : 2) <= SB, "a segment's queries fit a stage");
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int scan[NW], s_last, s_b, s_pos;
+  __shared__ int scan[NW], s_b, s_pos;
   // Records of a warp's units that lie only partly in its piece: [2w] the one that ends there, [2w + 1] the one that
   // goes on.  u0 < 0: none.
   __shared__ struct {
     int u0, n, b, kvh, rb, begins;
   } s_rec[2 * NW];
+  asm volatile("griddepcontrol.launch_dependents;");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int tok = (g >> 1) + 4 * (g & 1);  // token of accumulator row g (row g + 8: 8 more)
 
@@ -217,7 +237,7 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
     // Every thread sums a run of sequences; the line position of each run follows from a scan.
     const int run = (a.batch + 32 * NW - 1) / (32 * NW), b0 = threadIdx.x * run, b1 = min(a.batch, b0 + run);
     int sum = 0;
-    for (int b = b0; b < b1; b++) sum += paged_chunks(a, b).y;
+    for (int b = b0; b < b1; b++) sum += paged_chunks(a, b).y + kUnitCost;
     int pre = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -237,7 +257,10 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
     plan.ctas = min((int)gridDim.x, most);
     plan.share = plan.total / plan.ctas;
     plan.more = plan.total % plan.ctas;
-    if ((int)blockIdx.x >= plan.ctas) return;
+    if ((int)blockIdx.x >= plan.ctas) {
+      if (a.split && threadIdx.x == 0) a.open[blockIdx.x] = make_int4(0, 0, 0, 0);
+      return;
+    }
     if (threadIdx.x < 2 * NW) s_rec[threadIdx.x].u0 = -1;
     if (a.split) {
       cta_first = plan.start(blockIdx.x);
@@ -245,7 +268,7 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
       if (cta_first >= lo && cta_first < pre * per_chunk) {  // one thread's run holds the first chunk
         int at = lo, b = b0;
         for (;; b++) {
-          const int n = paged_chunks(a, b).y * per_chunk;
+          const int n = (paged_chunks(a, b).y + kUnitCost) * per_chunk;
           if (cta_first < at + n) break;
           at += n;
         }
@@ -265,10 +288,12 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
     }
   }
 
-  // The segment at line position `at` (or, unsplit, unit number `at`): chunks [c0, c1) of unit (b, kvh, rb), which
-  // begins at position u0 and has n chunks.  seq_b and seq_base walk along.
+  // The segment at line position `at` (or, unsplit, unit number `at`): chunks [c0, c1) of unit (b, kvh, rb), whose n
+  // chunks begin at position u0, and the position behind it.  It may be empty (the position lies in a unit's cost).
+  // seq_b and seq_base walk along.
   struct Segment {
-    int b, kvh, rb, c0, c1, u0, n;
+    int b, kvh, rb, c0, c1, u0, n, next;
+    bool begins, ends;
   };
   auto segment = [&](int at, int& seq_b, int& seq_base) -> Segment {
     Segment s;
@@ -276,33 +301,36 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
     int2 ch;
     if (a.split) {
       ch = paged_chunks(a, seq_b);
-      while (at >= seq_base + ch.y * per_chunk) {
-        seq_base += ch.y * per_chunk;
+      while (at >= seq_base + (ch.y + kUnitCost) * per_chunk) {
+        seq_base += (ch.y + kUnitCost) * per_chunk;
         ch = paged_chunks(a, ++seq_b);
       }
       s.b = seq_b;
-      u = (at - seq_base) / ch.y;
-      s.u0 = seq_base + u * ch.y;
-      s.c0 = ch.x + at - s.u0;
-      s.c1 = ch.x + min(ch.y, end - s.u0);
+      u = (at - seq_base) / (ch.y + kUnitCost);
+      s.u0 = seq_base + u * (ch.y + kUnitCost) + kUnitCost;
+      s.next = min(end, s.u0 + ch.y);
+      s.c0 = ch.x + max(0, at - s.u0);
+      s.c1 = ch.x + max(0, s.next - s.u0);
     } else {
       s.b = at / per_chunk;
       u = at % per_chunk;
       ch = paged_chunks(a, s.b);
       s.u0 = at;
+      s.next = at + gridDim.x * NW;
       s.c0 = ch.x, s.c1 = ch.x + ch.y;
     }
     s.n = ch.y;
+    s.begins = s.c0 == ch.x;
+    s.ends = s.c1 == ch.x + ch.y;
     s.kvh = u / a.nrb, s.rb = u % a.nrb;
     return s;
   };
-  auto after = [&](int at, const Segment& s) { return a.split ? at + s.c1 - s.c0 : at + (int)gridDim.x * NW; };
 
   // ---- this warp's ring: the chunks it will take, fetched ahead across segments ----
   const uint32_t ring = smem_u32(smem) + warp * ST * SB;
   float* buf = reinterpret_cast<float*>(smem + NW * ST * SB);  // [NW][RB][RS]: sums, M, l
   const int page_mask = (1 << a.kv.page_log2) - 1;
-  int f_pos = pos, f_seq = seg_b, f_base = seg_base;  // the segment being fetched begins at f_pos
+  int f_pos = pos, f_seq = seg_b, f_base = seg_base;  // the segment after the one being fetched
   Segment f{};
   int f_c = 0, f_lo, f_hi;
   const int32_t* f_table;
@@ -323,23 +351,34 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
     }
   };
   int f_page[2] = {-2, -2};
-  auto enter = [&]() {  // the segment at f_pos
-    f = segment(f_pos, f_seq, f_base);
-    f_c = f.c0;
+  auto enter = [&]() {  // the next segment with a chunk, from f_pos on
+    do {
+      f = segment(f_pos, f_seq, f_base);
+      f_pos = f.next;
+    } while (f.c0 >= f.c1 && f_pos < end);
+    f_c = f.c0 < f.c1 ? f.c0 - 1 : f.c1;  // its queries come first
     fetch_seq();
-    // its queries will be read soon
-    const char* q = static_cast<const char*>(a.q) + (((size_t)f.b * a.S * a.H + f.kvh * a.G) * DH + lane * 32) * (a.dtype == HCU_DT_F32 ? 4 : 2);
-    if (lane * 32 < min(a.G, RB) * DH) asm volatile("prefetch.global.L2 [%0];" ::"l"(q));
   };
-  if (pos < end) {
-    enter();
-    look_up(f_c, f_page);
-  }
-  // Fetches the next chunk into a stage and looks the one after it up.  Returns which halves hold data.
+  if (pos < end) enter();
+  // Fetches the next item, a segment's queries or a chunk, into a stage and looks the next chunk's pages up.  Returns
+  // which halves of a chunk hold data.
   auto fetch = [&](int st) -> uint32_t {
     uint32_t halves = 0;
-    if (f_c < f.c1) {
-      const uint32_t dst = ring + st * SB;
+    const uint32_t dst = ring + st * SB;
+    if (f_c < f.c0) {
+      const int es = a.dtype == HCU_DT_F32 ? 4 : 2, ppr = DH * es / 16;  // 16-byte pieces of a row
+      const int r0 = f.rb * RB;
+#pragma unroll
+      for (int i = 0; i < RB * DH * (TERMS == 2 ? 4 : 2) / 512; i++) {
+        const int p = 32 * i + lane, r = p / ppr, rr = r0 + r;
+        const bool there = r < RB && rr < a.R;
+        const int sq = there ? rr / a.G : 0, h = f.kvh * a.G + (there ? rr % a.G : 0);
+        const char* src = static_cast<const char*>(a.q) + (((size_t)f.b * a.S + sq) * a.H + h) * DH * es + (p % ppr) * 16;
+        if (r < RB) copy16(dst + p * 16, src, there);
+      }
+      f_c++;
+      look_up(f_c, f_page);
+    } else if (f_c < f.c1) {
       long long row[2];
 #pragma unroll
       for (int p = 0; p < 2; p++) {
@@ -368,7 +407,7 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
         const __half* src = (l / (2 * LH) ? a.kv.vs : a.kv.ks) + (p ? row[1] : row[0]) * NB + (l % LH) * 8;
         copy16(dst + 2 * KB + l * 16, src, p ? there[1] : there[0]);
       }
-      if (++f_c == f.c1 && (f_pos = after(f_pos, f)) < end) enter();
+      if (++f_c == f.c1 && f_pos < end) enter();
       look_up(f_c, f_page);
     }
     copy_commit();
@@ -382,8 +421,9 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
   while (pos < end) {
     const Segment sg = segment(pos, seg_b, seg_base);
     const int b = sg.b, kvh = sg.kvh, rb = sg.rb, c1 = sg.c1;
-    const bool begins = pos == sg.u0, ends = !a.split || sg.u0 + sg.n == pos + c1 - sg.c0;
-    pos = after(pos, sg);
+    const bool begins = sg.begins, ends = sg.ends;
+    pos = sg.next;
+    if (sg.c0 >= c1) continue;
     const int r0 = rb * RB, rows = min(RB, a.R - r0);
     int ctx = a.context[b];
     if (ctx > a.max_context || ctx < 0) {
@@ -394,28 +434,20 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
     const int pos_first = ctx - a.S + r0 / a.G, pos_last = ctx - a.S + (r0 + rows - 1) / a.G;
     const int lo_all = a.window > 0 ? max(0, pos_last + 1 - a.window) : 0, hi_all = max(0, pos_first + 1);
     // ---- query columns: column g of group nc is row / term of this lane's B fragments ----
+    copy_wait<ST - 1>();
+    __syncwarp();
     uint32_t qf[NC][NB][4];
     float corr[NC][NB][NR];  // -8 sum(q) of the block (not EXACT), rows of this thread's accumulator columns 2t, 2t + 1
     float rs[NC][NR];        // score = rs * accumulated sum
 #pragma unroll
     for (int nc = 0; nc < NC; nc++) {
       const int r = nc * RG + (TERMS == 2 ? g >> 1 : g);
-      const bool there = r < rows;
-      const int rr = r0 + (there ? r : 0), s = rr / a.G, h = kvh * a.G + rr % a.G;
-      const size_t at = (((size_t)b * a.S + s) * a.H + h) * DH;
-      float q[NB][8], top = 0.f;
+      float q[NB][8], top = 0.f;  // rows past the last are zeros
+      load_query<NB>(ring + stage * SB + r * (DH * (a.dtype == HCU_DT_F32 ? 4 : 2)), t, a.dtype, q);
 #pragma unroll
-      for (int i = 0; i < NB; i++) {
-        float x[4], y[4];
-        load4_dt(a.q, at + 32 * i + 8 * t, a.dtype, x);
-        load4_dt(a.q, at + 32 * i + 8 * t + 4, a.dtype, y);
+      for (int i = 0; i < NB; i++)
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-          q[i][c] = there ? x[c] : 0.f;
-          q[i][c + 4] = there ? y[c] : 0.f;
-          top = fmaxf(top, fmaxf(fabsf(q[i][c]), fabsf(q[i][c + 4])));
-        }
-      }
+        for (int c = 0; c < 8; c++) top = fmaxf(top, fabsf(q[i][c]));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       // 2^sq brings the row's largest magnitude into [2^13, 2^14)
@@ -451,6 +483,10 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
       rs[nc][0] = __shfl_sync(0xffffffffu, back, 8 * t);
       if (NR == 2) rs[nc][NR - 1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
     }
+
+    __syncwarp();
+    have = (have & ~(3u << (2 * stage))) | fetch(stage) << (2 * stage);
+    stage ^= 1;
 
     float O[2 * NB][NC][4] = {};
     float M[NC][NR], L[NC][NR], T[NC][NR];  // T: the score above which M has to move
@@ -696,106 +732,120 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
   __syncthreads();
 
   // ---- join the records: neighbours of the same unit ----
+  auto finish = [&](const float (&o)[4], float l, int b, int kvh, int rr, int d) {
+    const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    const float y[4] = {o[0] * f, o[1] * f, o[2] * f, o[3] * f};
+    const int s = rr / a.G, h = kvh * a.G + rr % a.G;
+    store4_dt(a.out, (((size_t)b * a.S + s) * a.H + h) * DH + d, a.dtype, y);
+  };
+  int4 open = make_int4(0, 0, 0, 0);
+  constexpr int TPE = DH / 4;  // threads that hold a row
   for (int k = 0; k < 2 * NW;) {
     const int u0 = s_rec[k].u0;
     if (u0 < 0) {
       k++;
       continue;
     }
-    uint32_t members = 0;
     const int first = k;
     int last = k;
+    uint32_t members = 0;
     for (; k < 2 * NW && (s_rec[k].u0 == u0 || s_rec[k].u0 < 0); k++)
       if (s_rec[k].u0 == u0) members |= 1u << k, last = k;
-    const int n = s_rec[first].n, b = s_rec[first].b, kvh = s_rec[first].kvh, rb = s_rec[first].rb;
+    const int b = s_rec[first].b, kvh = s_rec[first].kvh, rb = s_rec[first].rb;
     const bool whole = s_rec[first].begins && !(last & 1);  // no other CTA has a part of the unit
     const int r0 = rb * RB, rows = min(RB, a.R - r0);
-    auto record_at = [&](int m) {
-      return (m & 1) ? reinterpret_cast<const float*>(smem + (m >> 1) * ST * SB) : buf + (m >> 1) * RB * RS;
-    };
-    auto finish = [&](float (&o)[4], float l, int r, int d) {
-      const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-#pragma unroll
-      for (int c = 0; c < 4; c++) o[c] *= f;
-      const int rr = r0 + r, s = rr / a.G, h = kvh * a.G + rr % a.G;
-      store4_dt(a.out, (((size_t)b * a.S + s) * a.H + h) * DH + d, a.dtype, o);
-    };
     // The unit's first CTA leaves its part in its second record, the others in their first.
     float* mine = a.part + ((size_t)blockIdx.x * 2 + (u0 >= cta_first ? 1 : 0)) * REC;
-    for (int i = threadIdx.x; i < rows * (DH / 4); i += 32 * NW) {
-      const int r = i / (DH / 4), d = 4 * (i % (DH / 4));
-      float m = kNoM;
-      for (uint32_t x = members; x; x &= x - 1) m = fmaxf(m, record_at(__ffs(x) - 1)[r * RS + DH]);
-      float o[4] = {}, l = 0.f;
+    for (int i = threadIdx.x; i < rows * TPE; i += 32 * NW) {
+      const int r = i / TPE, d = 4 * (i % TPE);
+      float m = kNoM, l = 0.f, o[4] = {};
+#pragma unroll 1
       for (uint32_t x = members; x; x &= x - 1) {
-        const float* w = record_at(__ffs(x) - 1) + r * RS;
-        const float f = exp2f(w[DH] - m);
-        const float4 v = *reinterpret_cast<const float4*>(w + d);
-        o[0] = fmaf(v.x, f, o[0]), o[1] = fmaf(v.y, f, o[1]), o[2] = fmaf(v.z, f, o[2]), o[3] = fmaf(v.w, f, o[3]);
-        l = fmaf(w[DH + 1], f, l);
+        const int w = __ffs(x) - 1;
+        const float* rec = ((w & 1) ? reinterpret_cast<const float*>(smem + (w >> 1) * ST * SB) : buf + (w >> 1) * RB * RS) + r * RS;
+        const float2 ml = *reinterpret_cast<const float2*>(rec + DH);
+        const float4 v = *reinterpret_cast<const float4*>(rec + d);
+        const float mn = fmaxf(m, ml.x), f0 = ex2_approx(m - mn), f = ex2_approx(ml.x - mn);
+        m = mn;
+        l = fmaf(l, f0, ml.y * f);
+        o[0] = fmaf(o[0], f0, v.x * f), o[1] = fmaf(o[1], f0, v.y * f);
+        o[2] = fmaf(o[2], f0, v.z * f), o[3] = fmaf(o[3], f0, v.w * f);
       }
       if (whole) {
-        finish(o, l, r, d);
+        finish(o, l, b, kvh, r0 + r, d);
       } else {
         *reinterpret_cast<float4*>(mine + r * DH + d) = make_float4(o[0], o[1], o[2], o[3]);
         if (d == 0) *reinterpret_cast<float2*>(mine + RB * DH + 2 * r) = make_float2(m, l);
       }
     }
-    if (whole) continue;
-
-    // ---- the unit's CTAs: the one that draws the last ticket joins them ----
-    const int unit = (b * a.kv.KV + kvh) * a.nrb + rb, unit_first = plan.cta_of(u0);
-    const int n_parts = plan.cta_of(u0 + n - 1) - unit_first + 1;
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      s_last = atomicAdd(&a.tickets[unit], 1) == n_parts - 1;
-      if (s_last) a.tickets[unit] = 0;  // re-armed for the next call
-    }
-    __syncthreads();
-    if (s_last) {
-      __threadfence();
-      auto record = [&](int i) { return a.part + ((size_t)(unit_first + i) * 2 + (i == 0 ? 1 : 0)) * REC; };
-      // Weights of the records first (a warp per row), then the sums: many loads in flight in both.
-      // Row r's weights, then its sum of probabilities: in the second stage of ring r, or an area of their own.
-      static_assert(RB > 8 || (RB * RS * 4 <= SB && (kMaxParts + 1) * 4 <= SB), "records and weights share the rings");
-      auto weights = [&](int r) {
-        return RB > 8 ? buf + NW * RB * RS + r * (kMaxParts + 1) : reinterpret_cast<float*>(smem + r * ST * SB + SB);
-      };
-      for (int r = warp; r < rows; r += NW) {
-        float m = kNoM, l = 0.f;
-        for (int i = lane; i < n_parts; i += 32) m = fmaxf(m, __ldcg(record(i) + RB * DH + 2 * r));
-        m = warp_max(m);
-        for (int i = lane; i < n_parts; i += 32) {
-          const float2 ml = __ldcg(reinterpret_cast<const float2*>(record(i) + RB * DH + 2 * r));
-          const float f = exp2f(ml.x - m);
-          weights(r)[i] = f;
-          l = fmaf(ml.y, f, l);
-        }
-        l = warp_sum(l);
-        if (lane == 0) weights(r)[kMaxParts] = l;
-      }
-      __syncthreads();
-      for (int i = threadIdx.x; i < rows * (DH / 4); i += 32 * NW) {
-        const int r = i / (DH / 4), d = 4 * (i % (DH / 4));
-        float o[4] = {};
-        for (int p0 = 0; p0 < n_parts; p0 += 8) {
-          float4 v[8];
-#pragma unroll
-          for (int c = 0; c < 8; c++)
-            v[c] = __ldcg(reinterpret_cast<const float4*>(record(min(p0 + c, n_parts - 1)) + r * DH + d));
-#pragma unroll
-          for (int c = 0; c < 8; c++) {
-            const float f = p0 + c < n_parts ? weights(r)[p0 + c] : 0.f;
-            if (p0 + c < n_parts)
-              o[0] = fmaf(v[c].x, f, o[0]), o[1] = fmaf(v[c].y, f, o[1]), o[2] = fmaf(v[c].z, f, o[2]), o[3] = fmaf(v[c].w, f, o[3]);
-          }
-        }
-        finish(o, weights(r)[kMaxParts], r, d);
-      }
-    }
-    __syncthreads();
+    if (!whole && u0 >= cta_first)
+      open = make_int4(plan.cta_of(u0 + s_rec[first].n - 1) - (int)blockIdx.x + 1, b, kvh, rb);
   }
+  if (a.split && threadIdx.x == 0) a.open[blockIdx.x] = open;
+}
+
+// Joins the parts of the units that several CTAs share: block (c, r) row r of
+// the unit that begins in CTA c and goes on in the CTAs behind it.  It starts
+// while the CTAs above end and waits for all of them (programmatic dependent
+// launch): joining by the last CTA to arrive instead cost a fence, an atomic
+// and a serial walk, 13 us against 4 us behind the last CTA of one sequence of
+// 131072 keys.
+template <int DH, int RB>
+__global__ void __launch_bounds__(128) attn_paged_join_kernel(const PagedAttnArgs a) {
+  constexpr size_t REC = (size_t)RB * (DH + 2);
+  constexpr int TPE = DH / 4, GROUPS = 128 / TPE;  // threads that hold a row, groups that share the parts
+  __shared__ float w[kMaxParts], red[8];
+  __shared__ __align__(16) float sums[GROUPS][DH];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = blockIdx.y;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 open = a.open[blockIdx.x];
+  const int n_parts = open.x, rr = open.w * RB + r;
+  if (n_parts == 0 || rr >= a.R) return;
+  // the unit's first CTA left its part in its second record, the others in their first
+  auto record = [&](int i) { return a.part + ((size_t)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * REC; };
+  float m = kNoM, l = 0.f;
+  for (int i = tid; i < n_parts; i += 128) {
+    const float2 ml = *reinterpret_cast<const float2*>(record(i) + RB * DH + 2 * r);
+    const float mn = fmaxf(m, ml.x);
+    l = fmaf(l, ex2_approx(m - mn), ml.y * ex2_approx(ml.x - mn));
+    m = mn;
+    w[i] = ml.x;
+  }
+  const float top = warp_max(m);
+  if (lane == 0) red[warp] = top;
+  __syncthreads();
+  const float M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  l = warp_sum(l * ex2_approx(m - M));
+  if (lane == 0) red[4 + warp] = l;
+  const int grp = tid / TPE, d = 4 * (tid % TPE);
+  float o[4] = {};
+  for (int p0 = grp; p0 < n_parts; p0 += 8 * GROUPS) {
+    float4 v[8];
+#pragma unroll
+    for (int c = 0; c < 8; c++)
+      v[c] = *reinterpret_cast<const float4*>(record(min(p0 + c * GROUPS, n_parts - 1)) + r * DH + d);
+#pragma unroll
+    for (int c = 0; c < 8; c++) {
+      const float f = p0 + c * GROUPS < n_parts ? ex2_approx(w[p0 + c * GROUPS] - M) : 0.f;
+      if (p0 + c * GROUPS < n_parts)
+        o[0] = fmaf(v[c].x, f, o[0]), o[1] = fmaf(v[c].y, f, o[1]), o[2] = fmaf(v[c].z, f, o[2]), o[3] = fmaf(v[c].w, f, o[3]);
+    }
+  }
+  *reinterpret_cast<float4*>(&sums[grp][d]) = make_float4(o[0], o[1], o[2], o[3]);
+  __syncthreads();
+  if (grp != 0) return;
+  l = (red[4] + red[5]) + (red[6] + red[7]);
+  const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no token: zeros; NaN stays
+  float y[4];
+#pragma unroll
+  for (int c = 0; c < 4; c++) {
+    y[c] = 0.f;
+#pragma unroll
+    for (int k = 0; k < GROUPS; k++) y[c] += sums[k][d + c];
+    y[c] *= f;
+  }
+  const int s = rr / a.G, h = open.z * a.G + rr % a.G;
+  store4_dt(a.out, (((size_t)open.y * a.S + s) * a.H + h) * DH + d, a.dtype, y);
 }
 
 template <int DH, int TERMS, int NC, bool EXACT>
@@ -808,25 +858,33 @@ int launch(hcu_context* h, PagedAttnArgs a) {
   HCU_TRY(once_per_device(attr_done, h->device, [&]() -> int {
     return check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), op);
   }));
+  static_assert(smem <= (size_t)(227 * 1024), "shared memory");
   a.nrb = (a.R + RB - 1) / RB;
   const long long units = (long long)a.batch * a.kv.KV * a.nrb;
   if (units > 0x7fffffffLL) return fail(HCU_EINVAL, "%s: batch x KV x query row blocks too large", op);
-  static_assert(smem <= (size_t)(227 * 1024), "shared memory");
   long long grid = std::min(kMaxParts, h->sm_count * paged_ctas(DH, NC));
+  // The line must not pass 2^31 and the records must fit the workspace (behind the other ops' tickets).
   const size_t room = h->workspace_bytes > kTicketBytes ? h->workspace_bytes - kTicketBytes : 0;
   const long long span = a.window > 0 ? std::min<long long>(a.max_context, (long long)a.window + a.S + CHUNK) : a.max_context;
-  const long long most = units * (span / CHUNK + 2);  // chunks
-  a.split = units <= kMaxUnits && room >= (size_t)grid * 2 * record && most < 0x7fffffffLL;
+  const long long most = units * (span / CHUNK + 2 + kUnitCost);  // chunks
+  a.split = room >= (size_t)grid * (2 * record + sizeof(int4)) && most < 0x7fffffffLL;
   a.min_chunks = h->opt_attn_chunk > 0 ? (int)std::min<int64_t>(1 << 24, (h->opt_attn_chunk + CHUNK - 1) / CHUNK) : 8;
-  if (a.split) {
-    grid = std::min(grid, (most + a.min_chunks - 1) / a.min_chunks);
-  } else {
-    grid = std::min(grid, (units + NW - 1) / NW);
-  }
-  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(h->workspace) + kTicketBytes);
-  a.tickets = static_cast<int*>(h->workspace);
+  grid = a.split ? std::min(grid, (most + a.min_chunks - 1) / a.min_chunks) : std::min(grid, (units + NW - 1) / NW);
+  a.open = reinterpret_cast<int4*>(static_cast<uint8_t*>(h->workspace) + kTicketBytes);
+  a.part = reinterpret_cast<float*>(a.open + grid);
   kern<<<(unsigned)grid, 32 * NW, smem, h->stream>>>(a);
-  return after_launch("hcu_attention_paged: launch");
+  HCU_TRY(after_launch("hcu_attention_paged: launch"));
+  if (!a.split || grid == 1) return HCU_OK;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(grid - 1), RB);  // no unit goes on behind the last CTA
+  cfg.blockDim = dim3(128);
+  cfg.stream = h->stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, attn_paged_join_kernel<DH, RB>, a), "hcu_attention_paged: join");
 }
 
 template <int DH>
