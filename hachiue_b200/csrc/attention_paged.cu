@@ -136,36 +136,6 @@ __device__ __forceinline__ void store4_dt(void* p, size_t at, int dtype, const f
   else store4(static_cast<__nv_bfloat16*>(p) + at, x);
 }
 
-// Packed f32 pairs: one instruction for two lanes of a 64-bit register pair.
-__device__ __forceinline__ uint64_t f2(float x, float y) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ void f2_get(uint64_t v, float& x, float& y) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
-}
-__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-
-// 16 bytes from global into shared memory by the asynchronous copy unit; nothing is read and zeros are written unless `there`.
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 constexpr int kMaxParts = 320;  // CTAs of a call, and so of a unit
 constexpr int STAGES = 2;
 constexpr int paged_stage_bytes(int dh) { return CHUNK * (dh + dh / 8); }  // codes and scales, keys and values
