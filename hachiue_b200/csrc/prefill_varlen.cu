@@ -13,10 +13,11 @@
 //    tiles) of one sequence and KV head; a small kernel sorts the items by their
 //    number of key tiles, so that the persistent CTAs' shares are near equal
 //    whatever the lengths are.
-//  * Warp roles: K / V by TMA (warp 0), tcgen05.mma (warp 1), Q rows by cp.async
-//    (warps 2, 3), and a softmax warpgroup per tile, one thread per row.  S is in
-//    TMEM, P goes back over its columns, O stays in TMEM across the keys.  While
-//    one tile's softmax runs the tensor cores work on the other tile.
+//  * Warp roles: K / V by TMA (warp 0), tcgen05.mma of each tile (warps 1, 2: one
+//    warp for both spent more time on its barriers than the products take), Q rows
+//    by cp.async (warp 3), and a softmax warpgroup per tile, one thread per row.  S
+//    is in TMEM, P goes back over its columns, O stays in TMEM across the keys.
+//    While one tile's softmax runs the tensor cores work on the other tile.
 //  * Half of the exponentials of a tile without a mask run on the FMA pipe: 2^x =
 //    2^n 2^f with n = round(x) and a cubic minimax polynomial for 2^f (relative
 //    error 7.5e-5, below the 2^-12 of rounding P to f16), so that the SFU takes half the time.
@@ -45,7 +46,7 @@ struct VarlenArgs {
   int batch, H, KV, G, window, total_q, total_k;
   float scale_log2;  // log2(e) / sqrt(D)
   int* blocks;       // [batch + 1]: blocks of 256 rows before each sequence
-  int4* items;       // [2 * blocks]: {first query, queries, first key, keys}, {block of the sequence, 0, 0, 0}
+  int4* items;       // [2 * blocks]: {first query, queries, first key, keys}, {first packed row, first tile's key, tiles, 0}
   uint32_t* status;
 };
 
@@ -113,15 +114,15 @@ __global__ void __launch_bounds__(1024) varlen_items_kernel(const VarlenArgs a) 
         else hi = mid - 1;
       }
       const int q0 = a.cu_q[lo], lq = a.cu_q[lo + 1] - q0, k0 = a.cu_k[lo], lk = a.cu_k[lo + 1] - k0, blk = i - a.blocks[lo];
-      const int r1 = (int)min((long long)lq * a.G, (blk + 1) * 2LL * BM);
-      const int cost = key_tiles(blk * 2 * BM, r1, a.G, lq, lk, a.window).y;
-      const int bin = kBins - 1 - min(cost, kBins - 1);
+      const int r0 = blk * 2 * BM, rows = (int)min((long long)lq * a.G - r0, 2LL * BM);
+      const int2 tiles = key_tiles(r0, r0 + rows, a.G, lq, lk, a.window);
+      const int bin = kBins - 1 - min(tiles.y, kBins - 1);
       if (pass == 0) {
         atomicAdd(&bins[bin], 1);
       } else {
         const int at = atomicAdd(&bins[bin], 1);
         a.items[2 * at] = make_int4(q0, lq, k0, lk);
-        a.items[2 * at + 1] = make_int4(blk, 0, 0, 0);
+        a.items[2 * at + 1] = make_int4(r0, tiles.x, tiles.y, 0);
       }
     }
     __syncthreads();
@@ -256,27 +257,68 @@ __device__ __noinline__ void row_alone(const VarlenArgs& a, int q_row, int head,
   store4(static_cast<T*>(a.out) + ((long long)q_row * a.H + head) * HD + 4 * lane, acc);
 }
 
-// A work item: 256 packed rows of one sequence and KV head.
+// Barriers by their 32-bit shared-memory address (generic pointers to a dozen of them cost the issuing warp its registers).
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool bar_try_sleep(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity), "r"(1000000u)
+      : "memory");
+  return ok != 0;
+}
+// Bounded wait of a whole warp (true on every lane or on none): the MMA warp polls, the others sleep and leave it the
+// issue slots.
+template <bool POLL>
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, uint32_t* status) {
+  bool ok = bar_try(bar, parity);
+  if (!ok) {
+    const uint64_t t0 = globaltimer();
+    for (uint32_t n = 1; !(ok = POLL ? bar_try(bar, parity) : bar_try_sleep(bar, parity)); n++) {
+      if ((!POLL || (n & 63) == 0) && globaltimer() - t0 > HCU_WAIT_NS) {
+        if (status) atomicOr(status, HCU_DEVERR_TIMEOUT);
+        break;
+      }
+    }
+  }
+  return __all_sync(0xffffffffu, ok);
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void bar_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// Barriers of a CTA, in order.
+enum Bar { kQFull = 0, kQEmpty = 3, kKFull = 6, kKEmpty = 8, kVFull = 10, kVEmpty = 12, kSFull = 14, kPVDone = 16, kPHalf = 18, kPFull = 20,
+           kOFree = 22, kSRead = 24, kBars = 26 };
+
+// A work item: 256 packed rows of one sequence and KV head.  A role loads an item's words while it works on the item
+// before and unpacks them when it gets there.
+struct RawItem {
+  int4 x, y;
+  int g;  // KV head; -1: no item
+};
 struct Item {
   int q0, lq, k0, lk, g, r0;  // first query and their number, first key and their number, KV head, first packed row
   int n_first, ntiles;        // first key of the first tile, tiles of the item
-  int nt[2];                  // tiles of each half (0: the half has no row)
 };
-
-__device__ __forceinline__ Item get_item(const VarlenArgs& a, int idx) {
-  const int e = idx / a.KV;
-  const int4 x = a.items[2 * e];
-  Item it;
-  it.q0 = x.x, it.lq = x.y, it.k0 = x.z, it.lk = x.w;
-  it.g = idx % a.KV;
-  it.r0 = a.items[2 * e + 1].x * 2 * BM;
-  const int rows = (int)min((long long)it.lq * a.G - it.r0, 2LL * BM);
-  const int2 both = key_tiles(it.r0, it.r0 + rows, a.G, it.lq, it.lk, a.window);
-  it.n_first = both.x, it.ntiles = both.y;
-  const int last0 = it.lk - it.lq + (it.r0 + min(rows, BM) - 1) / a.G;  // position of the first half's last row
-  it.nt[0] = rows > BM ? (last0 < it.n_first ? 1 : (last0 - it.n_first) / BN + 1) : it.ntiles;
-  it.nt[1] = rows > BM ? it.ntiles : 0;
-  return it;
+__device__ __forceinline__ Item unpack(const RawItem& r) {
+  return Item{r.x.x, r.x.y, r.x.z, r.x.w, r.g, r.y.x, r.y.y, r.y.z};
 }
 
 // The k-th item of this CTA: rounds of gridDim.x items, forwards in even rounds and backwards in odd ones (costs fall
@@ -286,12 +328,22 @@ __device__ __forceinline__ int item_index(int k) {
   return k * P + ((k & 1) ? P - 1 - c : c);
 }
 
-// Barriers run on across items; every role advances the same counters:
-//   q_full / q_empty   per query tile (slot = tiles so far mod 3),
-//   kv_full / kv_empty per key tile of the items (ring),
-//   s_full, p_half, p_full per key tile and half,
-//   o_free             per item and half: O has been read, the next P.V may overwrite it,
-//   o_done             at the end.
+// TMEM (512 columns): O of the two halves, P of the two, and ONE buffer for S.
+// A softmax thread takes its whole row of S into registers at once, so the
+// buffer is free again some 100 cycles after the product is done, and the
+// halves share it in turn: the next scores of a half are computed while it
+// still works on the ones before.  (With a buffer each and P written over S a
+// half's products and its softmax took turns: 1500 of 4200 cycles per tile.)
+constexpr uint32_t kColP = 256, kColS = 384;
+
+// Barriers run on across items; every role advances the same counters.  Tile t
+// is the t-th key tile of this CTA's items; each half takes every tile.
+//   q_full / q_empty          per query tile (slot = tiles so far mod 3),
+//   k_full .. v_empty         per tile (rings of two; each half releases every tile),
+//   s_full, p_half, p_full    per tile and half,
+//   pv_done                   per tile and half: P has been read, O is whole,
+//   s_read                    per tile and half: S is in registers (the buffer is the other half's),
+//   o_free                    per item and half: O has been read, the next P.V may overwrite it.
 template <bool BF16>
 __global__ void __launch_bounds__(384, 1)
     prefill_varlen_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const VarlenArgs a) {
@@ -300,21 +352,13 @@ __global__ void __launch_bounds__(384, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* qsm = smem;                    // [Q_SLOTS][TILE]
   uint8_t* kvsm = qsm + Q_SLOTS * TILE;   // [KV_STAGES][K tile | V tile]
-  __shared__ uint64_t q_full[Q_SLOTS], q_empty[Q_SLOTS], kv_full[KV_STAGES], kv_empty[KV_STAGES];
-  __shared__ uint64_t s_full[2], p_half[2], p_full[2], o_free[2], o_done;
+  __shared__ uint64_t bars[kBars];
   __shared__ uint32_t tmem_slot;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
-    for (int i = 0; i < Q_SLOTS; i++) mbar_init(&q_full[i], 2), mbar_init(&q_empty[i], 1);
-    for (int i = 0; i < KV_STAGES; i++) mbar_init(&kv_full[i], 1), mbar_init(&kv_empty[i], 1);
-    for (int i = 0; i < 2; i++) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_half[i], 4);
-      mbar_init(&p_full[i], 4);
-      mbar_init(&o_free[i], 4);
-    }
-    mbar_init(&o_done, 1);
+    for (int i = 0; i < kBars; i++)
+      mbar_init(&bars[i], i >= kPHalf ? 4 : (i >= kKEmpty && i < kVFull) || (i >= kVEmpty && i < kSFull) ? 2 : 1);
     fence_barrier_init();
   }
   if (warp == 1) {
@@ -324,12 +368,22 @@ __global__ void __launch_bounds__(384, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_slot;
-  // TMEM columns per half: S (P over its first 64 columns), then O.
-  auto s_col = [](int hd) { return (uint32_t)(hd * 256); };
-  auto o_col = [](int hd) { return (uint32_t)(hd * 256 + 128); };
+  const uint32_t tmem = tmem_slot, bar0 = smem_u32(bars);
+  auto bar = [&](int i) { return bar0 + 8 * i; };
+  auto wait = [&](int i, uint32_t parity) { return bar_wait<false>(bar0 + 8 * i, parity, a.status); };
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int n_items = a.blocks[a.batch] * a.KV;
+  auto load_item = [&](int k) {
+    const int idx = item_index(k);
+    RawItem r{make_int4(0, 0, 0, 0), make_int4(0, 0, 0, 0), -1};
+    if (idx < n_items) {
+      const int e = idx / a.KV;
+      r.g = idx - e * a.KV;
+      r.x = a.items[2 * e];
+      r.y = a.items[2 * e + 1];
+    }
+    return r;
+  };
 
   if (warp < 4) {
     warpgroup_reg_dealloc<REG_CTRL>();
@@ -340,84 +394,78 @@ __global__ void __launch_bounds__(384, 1)
         prefetch_tensormap(&tmV);
         int kt = 0;
         bool ok = true;
-        for (int k = 0; ok; k++) {
-          const int idx = item_index(k);
-          if (idx >= n_items) break;
-          const Item it = get_item(a, idx);
+        RawItem next = load_item(0);
+        for (int k = 0; ok && next.g >= 0; k++) {
+          const Item it = unpack(next);
+          next = load_item(k + 1);
           for (int j = 0; j < it.ntiles; j++, kt++) {
             const int s = kt % KV_STAGES;
-            if (kt >= KV_STAGES && !mbar_wait(&kv_empty[s], ((kt - KV_STAGES) / KV_STAGES) & 1, a.status)) {
+            const uint32_t before = ((kt - KV_STAGES) / KV_STAGES) & 1;
+            uint8_t* st = kvsm + s * KV_STAGE;
+            const int row = it.k0 + it.n_first + j * BN;
+            if (kt >= KV_STAGES && !mbar_wait(&bars[kKEmpty + s], before, a.status)) {
               ok = false;
               break;
             }
-            uint8_t* st = kvsm + s * KV_STAGE;
-            const int row = it.k0 + it.n_first + j * BN;
-            mbar_arrive_expect_tx(&kv_full[s], KV_STAGE);
-            tma_load_3d(st, &tmK, &kv_full[s], 0, it.g, row);
-            tma_load_3d(st + BOX, &tmK, &kv_full[s], 64, it.g, row);
-            tma_load_3d(st + TILE, &tmV, &kv_full[s], 0, it.g, row);
-            tma_load_3d(st + TILE + BOX, &tmV, &kv_full[s], 64, it.g, row);
+            mbar_arrive_expect_tx(&bars[kKFull + s], TILE);
+            tma_load_3d(st, &tmK, &bars[kKFull + s], 0, it.g, row);
+            tma_load_3d(st + BOX, &tmK, &bars[kKFull + s], 64, it.g, row);
+            if (kt >= KV_STAGES && !mbar_wait(&bars[kVEmpty + s], before, a.status)) {
+              ok = false;
+              break;
+            }
+            mbar_arrive_expect_tx(&bars[kVFull + s], TILE);
+            tma_load_3d(st + TILE, &tmV, &bars[kVFull + s], 0, it.g, row);
+            tma_load_3d(st + TILE + BOX, &tmV, &bars[kVFull + s], 64, it.g, row);
           }
         }
       }
-    } else if (warp >= 2) {
+    } else if (warp == 3) {
       // ---------------- query tiles: rows of any stride, zeros behind the last ----------------
       int qn = 0;
       bool ok = true;
-      for (int k = 0; ok; k++) {
-        const int idx = item_index(k);
-        if (idx >= n_items) break;
-        const Item it = get_item(a, idx);
-        for (int hd = 0; hd < 2 && it.nt[hd] > 0; hd++, qn++) {
+      RawItem next = load_item(0);
+      for (int k = 0; ok && next.g >= 0; k++) {
+        const Item it = unpack(next);
+        next = load_item(k + 1);
+        for (int hd = 0; hd < 2; hd++, qn++) {
           const int slot = qn % Q_SLOTS;
-          if (qn >= Q_SLOTS && !__all_sync(0xffffffffu, mbar_wait(&q_empty[slot], ((qn - Q_SLOTS) / Q_SLOTS) & 1, a.status))) {
+          if (qn >= Q_SLOTS && !wait(kQEmpty + slot, ((qn - Q_SLOTS) / Q_SLOTS) & 1)) {
             ok = false;
             break;
           }
           const uint32_t dst = smem_u32(qsm + slot * TILE);
           const int piece = lane & 15;  // 16 bytes of a row
+          int q = (it.r0 + hd * BM + (lane >> 4)) / a.G, h = it.r0 + hd * BM + (lane >> 4) - q * a.G;  // row's query and head
 #pragma unroll 4
-          for (int i = 0; i < 32; i++) {
-            const int row = (warp - 2) * 2 + (lane >> 4) + 4 * i, r = it.r0 + hd * BM + row;
-            const int q = r / a.G, h = it.g * a.G + r % a.G;
+          for (int i = 0; i < 64; i++) {
+            const int row = (lane >> 4) + 2 * i;
             const bool there = q < it.lq;
-            const T* src = static_cast<const T*>(a.q) + (long long)(it.q0 + (there ? q : 0)) * a.q_stride + (long long)h * HD + piece * 8;
+            const T* src = static_cast<const T*>(a.q) + (long long)(it.q0 + (there ? q : 0)) * a.q_stride + (long long)(it.g * a.G + h) * HD + piece * 8;
             copy16(dst + (piece >> 3) * BOX + sw128_offset(row, (piece & 7) * 16), src, there);
+            for (h += 2; h >= a.G; h -= a.G) q++;
           }
           copy_commit();
           copy_wait<0>();
           fence_proxy_async();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&q_full[slot]);
+          if (lane == 0) bar_arrive(bar(kQFull + slot));
         }
       }
     } else {
-      // ---------------- MMA issue: the warp walks, one elected lane issues ----------------
+      // ---------------- MMA issue of a half (warps 1 and 2): the warp walks, one elected lane issues ----------------
+      const int hd = warp - 1;
       const bool leader = elect_one_sync();
+      auto wait = [&](int i, uint32_t parity) { return bar_wait<true>(bar0 + 8 * i, parity, a.status); };
       constexpr uint32_t idesc_qk = idesc_f16(BM, BN, BF16, false, false);
       constexpr uint32_t idesc_pv = idesc_f16(BM, HD, BF16, false, true);
-      const uint32_t qb = smem_u32(qsm), kvb = smem_u32(kvsm);
-      auto qk = [&](int hd, int slot, int s) {
-#pragma unroll
-        for (int ks = 0; ks < 8; ks++) {
-          const uint64_t ad = smem_desc_sw128(qb + slot * TILE + (ks >> 2) * BOX + (ks & 3) * 32, 16, 1024);
-          const uint64_t bd = smem_desc_sw128(kvb + s * KV_STAGE + (ks >> 2) * BOX + (ks & 3) * 32, 16, 1024);
-          if (leader) mma_f16_ss(tmem + s_col(hd), ad, bd, idesc_qk, ks > 0);
-        }
-        if (leader) mma_commit(&s_full[hd]);
-      };
-      auto pv_half = [&](int hd, int s, int half, bool acc) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const int ks = 4 * half + i;
-          const uint64_t bd = smem_desc_sw128(kvb + s * KV_STAGE + TILE + ks * 2048, BOX, 1024);  // MN-major V
-          if (leader) mma_f16_ts(tmem + o_col(hd), tmem + s_col(hd) + ks * 8, bd, idesc_pv, (acc || ks > 0) ? 1u : 0u);
-        }
-      };
-      // Value rows behind the sequence's end become zeros (they meet P = 0, but may hold anything).
-      auto clean = [&](const Item& it, int j, int s) {
-        const int valid = max(0, it.lk - it.n_first - j * BN);
-        if (valid >= BN) return;
+      // Descriptors: the first k-step's, to which a constant per k-step is added.
+      const uint64_t dq = smem_desc_sw128(smem_u32(qsm), 16, 1024), dk = smem_desc_sw128(smem_u32(kvsm), 16, 1024);
+      const uint64_t dv = smem_desc_sw128(smem_u32(kvsm) + TILE, BOX, 1024);  // MN-major
+      const uint32_t ts = tmem + kColS, tp = tmem + kColP + hd * 64, to = tmem + hd * HD;
+      // Value rows behind the sequence's end become zeros (they meet P = 0, but may hold anything).  Both halves' warps
+      // write them, each before its own products: the same zeros.
+      auto clean = [&](int valid, int s) {
         uint8_t* v = kvsm + s * KV_STAGE + TILE;
         for (int i = valid * 8 + lane; i < BN * 8; i += 32) {
           *reinterpret_cast<uint4*>(v + i * 16) = make_uint4(0u, 0u, 0u, 0u);
@@ -426,84 +474,91 @@ __global__ void __launch_bounds__(384, 1)
         fence_proxy_async();
         __syncwarp();
       };
-      auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_poll(bar, parity, a.status)); };
-      int kt = 0, qn = 0;        // key tiles and query tiles so far, this item's first
-      int nt[2] = {0, 0};        // key tiles of each half so far
-      int done[2] = {0, 0};      // items of each half so far
-      bool ok = true;
-      int idx = item_index(0);
-      Item it{};
-      if (idx < n_items) {
-        it = get_item(a, idx);
-        ok = wait(&kv_full[0], 0);
-        for (int hd = 0; ok && hd < 2 && it.nt[hd] > 0; hd++) {
-          ok = wait(&q_full[hd], 0);
-          if (!ok) break;
-          tc_fence_after();
-          qk(hd, hd, 0);
-          if (it.nt[hd] == 1 && leader) mma_commit(&q_empty[hd]);
-          if (hd == 0) clean(it, 0, 0);
-        }
+      // S = Q K^T runs one tile ahead of O += P V.  The scores' place: tile st, tile sj of sn in its item, whose query
+      // tile is number sq.
+      int st = 0, sj = 0, sn = 0, sq = hd;
+      RawItem next = load_item(0);
+      int valid = BN;  // keys of the last tile of the item that the scores are in
+      auto enter = [&]() {
+        const Item it = unpack(next);
+        sn = it.ntiles, sj = 0;
+        valid = max(0, it.lk - it.n_first - (it.ntiles - 1) * BN);
+      };
+      bool ok = true, more = next.g >= 0;
+      if (more) {
+        enter();
+        next = load_item(1);
       }
-      for (int k = 0; ok && idx < n_items; k++) {
-        idx = item_index(k + 1);
-        const bool more = idx < n_items;
-        const Item next = more ? get_item(a, idx) : it;
-        const int qn1 = qn + (it.nt[1] > 0 ? 2 : 1);
-        for (int j = 0; ok && j < it.ntiles; j++) {
-          const int s = (kt + j) % KV_STAGES, s1 = (kt + j + 1) % KV_STAGES, last_half = it.nt[1] > 0 ? 1 : 0;
-          const bool last = j + 1 == it.ntiles;
-          bool cleaned = false;
-          for (int hd = 0; hd < 2; hd++) {
-            if (j < it.nt[hd]) {
-              const int t = nt[hd] + j;
-              if (!wait(&p_half[hd], t & 1) || (j == 0 && done[hd] > 0 && !wait(&o_free[hd], (done[hd] - 1) & 1))) {
-                ok = false;
-                break;
-              }
-              tc_fence_after();
-              pv_half(hd, s, 0, j > 0);
-              if (!wait(&p_full[hd], t & 1)) {
-                ok = false;
-                break;
-              }
-              tc_fence_after();
-              pv_half(hd, s, 1, true);
-              if (hd == last_half && leader) mma_commit(&kv_empty[s]);
-            }
-            // The half's next scores overwrite its P: behind the P.V above.  At the item's last tile: the next item's first.
-            const bool here = j + 1 < it.nt[hd], there = last && more && next.nt[hd] > 0;
-            if (here || there) {
-              const int q = here ? qn + hd : qn1 + hd;
-              if (!wait(&kv_full[s1], ((kt + j + 1) / KV_STAGES) & 1) || (there && !wait(&q_full[q % Q_SLOTS], (q / Q_SLOTS) & 1))) {
-                ok = false;
-                break;
-              }
-              tc_fence_after();
-              qk(hd, q % Q_SLOTS, s1);
-              if ((here ? j + 2 == it.nt[hd] : next.nt[hd] == 1) && leader) mma_commit(&q_empty[q % Q_SLOTS]);
-              if (!cleaned) {
-                clean(here ? it : next, here ? j + 1 : 0, s1);
-                cleaned = true;
-              }
-            }
+      int k = 1;  // item that `next` holds
+      auto scores = [&]() -> bool {
+        const int s = st % KV_STAGES, slot = sq % Q_SLOTS;
+        if (!wait(kKFull + s, (st / KV_STAGES) & 1) || (sj == 0 && !wait(kQFull + slot, (sq / Q_SLOTS) & 1)) ||
+            (st + hd > 0 && !wait(kSRead + (hd ^ 1), (st + hd - 1) & 1)))
+          return false;
+        tc_fence_after();
+        const uint64_t ad = dq + slot * (TILE >> 4), bd = dk + s * (KV_STAGE >> 4);
+#pragma unroll
+        for (int ks = 0; ks < 8; ks++) {
+          const uint64_t x = ad + (((ks >> 2) * BOX + (ks & 3) * 32) >> 4), y = bd + (((ks >> 2) * BOX + (ks & 3) * 32) >> 4);
+          if (leader) mma_f16_ss(ts, x, y, idesc_qk, ks > 0);
+        }
+        if (leader) {
+          bar_commit(bar(kSFull + hd));
+          bar_commit(bar(kKEmpty + s));
+          if (sj + 1 == sn) bar_commit(bar(kQEmpty + slot));
+        }
+        st++;
+        if (++sj == sn) {
+          sq += 2;
+          more = next.g >= 0;
+          if (more) {
+            enter();
+            next = load_item(++k);
           }
         }
-        for (int hd = 0; hd < 2; hd++) nt[hd] += it.nt[hd], done[hd] += it.nt[hd] > 0;
-        kt += it.ntiles;
-        qn = qn1;
-        it = next;
+        return true;
+      };
+      int pj = 0, pn = sn, pvalid = valid, items = 0;  // the products' place: tile pj of pn in the items-th item
+      if (more) ok = scores();
+      for (int t = 0; ok && t < st; t++) {  // tile t: its scores have been issued
+        const int sn1 = sn, valid1 = valid;  // of the item of the tile after this one
+        if (more && !scores()) break;
+        const int s = t % KV_STAGES;
+        if (!wait(kVFull + s, (t / KV_STAGES) & 1)) break;
+        if (pj + 1 == pn && pvalid < BN) clean(pvalid, s);
+        // O += P V in two halves of 64 keys: the first runs while the softmax computes the second half of P
+        const uint64_t vd = dv + s * (KV_STAGE >> 4);
+        if (!wait(kPHalf + hd, t & 1) || (pj == 0 && items > 0 && !wait(kOFree + hd, (items - 1) & 1))) break;
+        tc_fence_after();
+#pragma unroll
+        for (int ks = 0; ks < 4; ks++) {
+          const uint64_t y = vd + ks * (2048 >> 4);
+          if (leader) mma_f16_ts(to, tp + ks * 8, y, idesc_pv, (pj > 0 || ks > 0) ? 1u : 0u);
+        }
+        if (!wait(kPFull + hd, t & 1)) break;
+        tc_fence_after();
+#pragma unroll
+        for (int ks = 4; ks < 8; ks++) {
+          const uint64_t y = vd + ks * (2048 >> 4);
+          if (leader) mma_f16_ts(to, tp + ks * 8, y, idesc_pv, 1u);
+        }
+        if (leader) {
+          bar_commit(bar(kPVDone + hd));
+          bar_commit(bar(kVEmpty + s));
+        }
+        if (++pj == pn) {
+          pj = 0, pn = sn1, pvalid = valid1, items++;
+        }
       }
-      if (leader) mma_commit(&o_done);
     }
   } else {
     // ---------------- softmax of one half, one thread per row ----------------
     warpgroup_reg_alloc<REG_SOFTMAX>();
     const int hd = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
-    const uint32_t sc = tmem + lane_off + s_col(hd), oc = tmem + lane_off + o_col(hd);
-    // A finished item's result: out of TMEM and into the output.  It runs after the NEXT item's first P is in TMEM (O
-    // has long been complete by then: the next scores follow the last P.V), so that tile's products cover it.
+    const uint32_t sc = tmem + lane_off + kColS, pc = tmem + lane_off + kColP + hd * 64, oc = tmem + lane_off + hd * HD;
+    // A finished item's result: out of TMEM and into the output.  It runs after the NEXT item's first P is in TMEM, which
+    // waited for the finished item's last product.
     int f_row = -1, f_head = 0, f_k0 = 0, f_lo = 0, f_hi = -1;  // this thread's finished row: query row (-1: none), head, visible keys
     float f_l = 0.f;
     bool fin = false;
@@ -514,7 +569,7 @@ __global__ void __launch_bounds__(384, 1)
       tmem_ld_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&o_free[hd]);
+      if (lane == 0) bar_arrive(bar(kOFree + hd));
       const bool empty = f_lo > f_hi;
       const float inv = empty ? 0.f : 1.f / f_l;
       uint64_t sum = f2(0.f, 0.f);
@@ -531,16 +586,16 @@ __global__ void __launch_bounds__(384, 1)
 #pragma unroll
         for (int c = 0; c < 4; c++)
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            uint4 w;
-            uint32_t* p = &w.x;
+          for (int i = 0; i < 32; i += 16) {
+            uint32_t w[8];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
+            for (int e = 0; e < 8; e++) {
               const float y0 = empty ? 0.f : __uint_as_float(o[c][i + 2 * e]) * inv;
               const float y1 = empty ? 0.f : __uint_as_float(o[c][i + 2 * e + 1]) * inv;
-              p[e] = pack16<BF16>(y0, y1);
+              w[e] = pack16<BF16>(y0, y1);
             }
-            *reinterpret_cast<uint4*>(dst + 32 * c + i) = w;
+            st_global_v8(reinterpret_cast<float*>(dst + 32 * c + i), __uint_as_float(w[0]), __uint_as_float(w[1]), __uint_as_float(w[2]),
+                         __uint_as_float(w[3]), __uint_as_float(w[4]), __uint_as_float(w[5]), __uint_as_float(w[6]), __uint_as_float(w[7]));
           }
       }
       for (uint32_t rows = __ballot_sync(0xffffffffu, bad); rows; rows &= rows - 1) {
@@ -552,21 +607,20 @@ __global__ void __launch_bounds__(384, 1)
     };
     int nt = 0;  // key tiles of this half so far
     bool ok = true;
-    for (int k = 0; ok; k++) {
-      const int idx = item_index(k);
-      if (idx >= n_items) break;
-      const Item it = get_item(a, idx);
-      if (it.nt[hd] == 0) continue;
+    RawItem next = load_item(0);
+    for (int k = 0; ok && next.g >= 0; k++) {
+      const Item it = unpack(next);
+      next = load_item(k + 1);
       const int first = it.r0 + hd * BM, r = first + row, qi = r / a.G, pos = it.lk - it.lq + qi;
       const bool exists = qi < it.lq;
       // every row of the half sees keys [all_lo, all_hi]
-      const int all_hi = it.lk - it.lq + first / a.G;
+      const int all_hi = first / a.G < it.lq ? it.lk - it.lq + first / a.G : -1;
       const int all_lo = a.window > 0 ? it.lk - it.lq + min(it.lq - 1, (first + BM - 1) / a.G) - a.window + 1 : 0;
       const int row_lo = a.window > 0 ? max(0, pos - a.window + 1) : 0, row_hi = exists ? pos : -1;
       float m_use = -INFINITY, l = 0.f;
-      for (int j = 0; j < it.nt[hd]; j++) {
+      for (int j = 0; j < it.ntiles; j++) {
         const int t = nt + j, n0 = it.n_first + j * BN;
-        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[hd], t & 1, a.status))) {
+        if (!wait(kSFull + hd, t & 1)) {
           ok = false;
           break;
         }
@@ -579,6 +633,9 @@ __global__ void __launch_bounds__(384, 1)
         tmem_ld32(sc + 64, s2);
         tmem_ld32(sc + 96, s3);
         tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(bar(kSRead + hd));
         bool e0 = false, e1 = false, e2 = false, e3 = false;
         if (!full) {
           e0 = mask_chunk<0>(s0, lo, hi);
@@ -595,7 +652,13 @@ __global__ void __launch_bounds__(384, 1)
         const bool move = mx > m_use + RESCALE_LOG2 || (j == 0 && mx > m_use);
         const bool rescale_o = move && j > 0 && m_use != -INFINITY;
         const float f = rescale_o ? exp2f(m_use - mx) : 1.f;
-        if (__any_sync(0xffffffffu, rescale_o)) {  // P.V of the tile before has landed (s_full of this tile)
+        // P and O are this thread's again once the product of the tile before is done.
+        if (t > 0 && !wait(kPVDone + hd, (t - 1) & 1)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (__any_sync(0xffffffffu, rescale_o)) {
 #pragma unroll
           for (int c = 0; c < 4; c++) {
             uint32_t r32[32];
@@ -614,7 +677,7 @@ __global__ void __launch_bounds__(384, 1)
         const float neg_m = m_use == -INFINITY ? 0.f : -m_use;
         const uint64_t scale2 = f2(a.scale_log2, a.scale_log2), negm2 = f2(neg_m, neg_m);
         uint64_t ls2[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
-        auto half_p = [&](const uint32_t (&x)[32], bool ex, const uint32_t (&y)[32], bool ey, uint32_t col, uint64_t* bar) {
+        auto half_p = [&](const uint32_t (&x)[32], bool ex, const uint32_t (&y)[32], bool ey, uint32_t col, int done) {
           uint32_t pk[32];
           if (full) {
             chunk_p<BF16, true, 0>(x, false, scale2, negm2, ls2, pk);
@@ -623,14 +686,14 @@ __global__ void __launch_bounds__(384, 1)
             chunk_p<BF16, false, 0>(x, ex, scale2, negm2, ls2, pk);
             chunk_p<BF16, false, 16>(y, ey, scale2, negm2, ls2, pk);
           }
-          tmem_st32(sc + col, pk);
+          tmem_st32(pc + col, pk);
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar);
+          if (lane == 0) bar_arrive(bar(done));
         };
-        half_p(s0, e0, s1, e1, 0, &p_half[hd]);
-        half_p(s2, e2, s3, e3, 32, &p_full[hd]);
+        half_p(s0, e0, s1, e1, 0, kPHalf + hd);
+        half_p(s2, e2, s3, e3, 32, kPFull + hd);
         float a0, a1, b0, b1;
         f2_get(ls2[0], a0, a1);
         f2_get(ls2[1], b0, b1);
@@ -644,9 +707,9 @@ __global__ void __launch_bounds__(384, 1)
       f_k0 = it.k0;
       f_lo = row_lo, f_hi = row_hi;
       f_l = l;
-      nt += it.nt[hd];
+      nt += it.ntiles;
     }
-    if (ok && fin && __all_sync(0xffffffffu, mbar_wait(&o_done, 0, a.status))) {
+    if (ok && fin && wait(kPVDone + hd, (nt - 1) & 1)) {
       tc_fence_after();
       epilogue();
     }
@@ -718,9 +781,9 @@ extern "C" int hcu_prefill_varlen(hcu_handle h, const hcu_prefill_varlen_params*
   if (a.q_stride < (long long)p->H * 128 || a.k_stride < (long long)p->KV * 128 || a.v_stride < (long long)p->KV * 128)
     return fail(HCU_EINVAL, "%s: a row stride is shorter than its row", op);
   if ((a.q_stride | a.k_stride | a.v_stride) >> 32) return fail(HCU_EINVAL, "%s: a row stride is too large", op);
-  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
-       reinterpret_cast<uintptr_t>(out)) % 16)
-    return fail(HCU_EINVAL, "%s: q, k, v and out must be 16-byte aligned", op);
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 ||
+      reinterpret_cast<uintptr_t>(out) % 32)
+    return fail(HCU_EINVAL, "%s: q, k and v must be 16-byte, out 32-byte aligned", op);
   a.q = q;
   a.k = k;
   a.v = v;

@@ -626,7 +626,8 @@ int hcu_attention_paged(hcu_handle h, const hcu_attention_paged_params *p, const
  * (window 0: from 0), scale 1 / sqrt(D), kvh = h / (H / KV).  A query that sees
  * no key (Lk < Lq) gives zeros.  q [total_q, H, D], k and v [total_k, KV, D] of
  * `dtype` (HCU_DT_BF16 or HCU_DT_F16), rows at the given strides in elements
- * (0 = dense), a multiple of 8; out [total_q, H, D] dense, of the same type.
+ * (0 = dense), a multiple of 8; out [total_q, H, D] dense, of the same type,
+ * 32-byte aligned.
  * D = 128.  Tensor cores, f32 accumulation; the probabilities are rounded to
  * `dtype` for their product with the values.
  *
