@@ -18,9 +18,6 @@
 //    by cp.async (warp 3), and a softmax warpgroup per tile, one thread per row.  S
 //    is in TMEM, P goes back over its columns, O stays in TMEM across the keys.
 //    While one tile's softmax runs the tensor cores work on the other tile.
-//  * Half of the exponentials of a tile without a mask run on the FMA pipe: 2^x =
-//    2^n 2^f with n = round(x) and a cubic minimax polynomial for 2^f (relative
-//    error 7.5e-5, below the 2^-12 of rounding P to f16), so that the SFU takes half the time.
 //  * O is rescaled only when a row's maximum grows by more than 2^8: P stays
 //    below 2^8 otherwise and O / l cancels the stale maximum.
 //  * Keys and values behind a sequence's end have no influence: scores are
@@ -47,6 +44,8 @@ struct VarlenArgs {
   float scale_log2;  // log2(e) / sqrt(D)
   int* blocks;       // [batch + 1]: blocks of 256 rows before each sequence
   int4* items;       // [2 * blocks]: {first query, queries, first key, keys}, {first packed row, first tile's key, tiles, 0}
+  uint32_t recip_G, recip_KV;  // for quot()
+  int q_tma;         // G divides 128: a tile's rows are one box of Q
   uint32_t* status;
 };
 
@@ -58,6 +57,14 @@ constexpr int Q_SLOTS = 3;     // tiles of queries: an item's two and the next o
 constexpr float RESCALE_LOG2 = 8.f;
 constexpr uint32_t REG_CTRL = 56, REG_SOFTMAX = 224;
 static_assert(128 * REG_CTRL + 256 * REG_SOFTMAX == 384 * 168, "register split");
+
+// n / d for 0 <= n < 2^31 by the host's recip = min(2^32 - 1, 2^32 / d + 1): the product is off by one at most.
+__device__ __forceinline__ int quot(int n, int d, uint32_t recip) {
+  int q = (int)__umulhi((uint32_t)n, recip);
+  if (q * d > n) q--;
+  if (n - q * d >= d) q++;
+  return q;
+}
 
 // ---- the items, longest first ------------------------------------------------
 constexpr int kBins = 1024;
@@ -160,41 +167,17 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-__device__ __forceinline__ float fmax_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-
-// 2^x for two x <= 127 on the FMA pipe: n = round(x) by adding 1.5 * 2^23, f = x - n in [-1/2, 1/2], a cubic for 2^f
-// (minimax fit of the relative error), and n added to the exponent.  Below -126 the result is near 2^-126; NaN gives
-// something not finite once rounded to 16 bits.
-__device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
-  float x0, x1;
-  f2_get(x, x0, x1);
-  x = f2(fmax_nan(x0, -126.f), fmax_nan(x1, -126.f));
-  const uint64_t magic = f2(12582912.f, 12582912.f), unmagic = f2(-12582912.f, -12582912.f);
-  const uint64_t t = f2_add(x, magic);
-  const uint64_t f = f2_fma(f2_add(t, unmagic), f2(-1.f, -1.f), x);
-  uint64_t p = f2_fma(f2(0.0551716649f, 0.0551716649f), f, f2(0.242611122f, 0.242611122f));
-  p = f2_fma(p, f, f2(0.693260986f, 0.693260986f));
-  p = f2_fma(p, f, f2(0.999928074f, 0.999928074f));
-  float t0, t1, p0, p1;
-  f2_get(t, t0, t1);
-  f2_get(p, p0, p1);
-  return f2(__uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23)),
-            __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23)));
-}
-
-// Scores of columns outside lo..hi (tile columns) become -inf, in one 32-column chunk beginning at column C0.  Returns
-// whether no row of the warp keeps any column of it (warp-uniform; the chunk is then left as it is and skipped).
+// Scores of columns outside lo..hi (tile columns) become -inf, in one 32-column chunk beginning at column C0: a bit per
+// column, tested one by one.  Returns whether no row of the warp keeps any column of it (warp-uniform; the chunk is then left
+// as it is and skipped).
 template <int C0>
 __device__ __forceinline__ bool mask_chunk(uint32_t (&r)[32], int lo, int hi) {
-  if (__all_sync(0xffffffffu, lo <= C0 && hi >= C0 + 31)) return false;
-  if (__all_sync(0xffffffffu, hi < C0 || lo > C0 + 31)) return true;
-  const int a = lo - C0, b = hi - C0;
+  const int a = min(max(lo - C0, 0), 32), b = min(max(hi + 1 - C0, 0), 32);  // columns a .. b - 1 stay
+  const uint32_t keep = (b == 32 ? 0xffffffffu : (1u << b) - 1u) & (a == 32 ? 0u : 0xffffffffu << a);
+  if (__all_sync(0xffffffffu, keep == 0xffffffffu)) return false;
+  if (__all_sync(0xffffffffu, keep == 0u)) return true;
 #pragma unroll
-  for (int i = 0; i < 32; i++) r[i] = (i >= a && i <= b) ? r[i] : 0xff800000u;  // -inf
+  for (int i = 0; i < 32; i++) r[i] = (keep & (1u << i)) ? r[i] : 0xff800000u;  // -inf
   return false;
 }
 __device__ __forceinline__ void chunk_max(const uint32_t (&r)[32], float (&mx)[4]) {
@@ -203,12 +186,8 @@ __device__ __forceinline__ void chunk_max(const uint32_t (&r)[32], float (&mx)[4
     mx[(i >> 1) & 3] = fmax3(mx[(i >> 1) & 3], __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
 }
 
-#ifndef POLY
-#define POLY 2
-#endif
-// P of one 32-column chunk as 16 words pk[OFF..], added to the row's sums.  With FULL (no mask in the tile) every second
-// pair takes the FMA pipe's exponential.
-template <bool BF16, bool FULL, int OFF>
+// P of one 32-column chunk as 16 words pk[OFF..], added to the row's sums.
+template <bool BF16, int OFF>
 __device__ __forceinline__ void chunk_p(const uint32_t (&r)[32], bool empty, uint64_t scale2, uint64_t negm2, uint64_t (&ls2)[2],
                                         uint32_t (&pk)[32]) {
   if (empty) {
@@ -218,18 +197,10 @@ __device__ __forceinline__ void chunk_p(const uint32_t (&r)[32], bool empty, uin
   }
 #pragma unroll
   for (int i = 0; i < 16; i++) {
-    uint64_t x = f2_fma(f2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), scale2, negm2);
-    float p0, p1;
-    if (FULL && POLY > 0 && i % POLY == POLY - 1) {
-      x = exp2_pair(x);
-      f2_get(x, p0, p1);
-    } else {
-      float v0, v1;
-      f2_get(x, v0, v1);
-      p0 = ex2_approx(v0), p1 = ex2_approx(v1);
-      x = f2(p0, p1);
-    }
-    ls2[i & 1] = f2_add(ls2[i & 1], x);
+    float v0, v1;
+    f2_get(f2_fma(f2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), scale2, negm2), v0, v1);
+    const float p0 = ex2_approx(v0), p1 = ex2_approx(v1);
+    ls2[i & 1] = f2_add(ls2[i & 1], f2(p0, p1));
     pk[OFF + i] = pack16<BF16>(p0, p1);
   }
 }
@@ -346,7 +317,8 @@ constexpr uint32_t kColP = 256, kColS = 384;
 //   o_free                    per item and half: O has been read, the next P.V may overwrite it.
 template <bool BF16>
 __global__ void __launch_bounds__(384, 1)
-    prefill_varlen_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const VarlenArgs a) {
+    prefill_varlen_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                          const __grid_constant__ CUtensorMap tmV, const VarlenArgs a) {
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -377,7 +349,7 @@ __global__ void __launch_bounds__(384, 1)
     const int idx = item_index(k);
     RawItem r{make_int4(0, 0, 0, 0), make_int4(0, 0, 0, 0), -1};
     if (idx < n_items) {
-      const int e = idx / a.KV;
+      const int e = quot(idx, a.KV, a.recip_KV);
       r.g = idx - e * a.KV;
       r.x = a.items[2 * e];
       r.y = a.items[2 * e + 1];
@@ -390,6 +362,7 @@ __global__ void __launch_bounds__(384, 1)
     if (warp == 0) {
       // ---------------- K / V tiles ----------------
       if (lane == 0) {
+        prefetch_tensormap(&tmQ);
         prefetch_tensormap(&tmK);
         prefetch_tensormap(&tmV);
         int kt = 0;
@@ -421,7 +394,8 @@ __global__ void __launch_bounds__(384, 1)
         }
       }
     } else if (warp == 3) {
-      // ---------------- query tiles: rows of any stride, zeros behind the last ----------------
+      // ---------------- query tiles: one TMA box, or where 128 rows are no whole queries, row by row ----------------
+      // (rows behind the sequence's last are anything: they stay within themselves and are not stored)
       int qn = 0;
       bool ok = true;
       RawItem next = load_item(0);
@@ -434,9 +408,19 @@ __global__ void __launch_bounds__(384, 1)
             ok = false;
             break;
           }
+          if (a.q_tma) {
+            if (lane == 0) {
+              uint8_t* box = qsm + slot * TILE;
+              const int q = it.q0 + quot(it.r0 + hd * BM, a.G, a.recip_G);
+              mbar_arrive_expect_tx(&bars[kQFull + slot], TILE);
+              tma_load_3d(box, &tmQ, &bars[kQFull + slot], 0, it.g * a.G, q);
+              tma_load_3d(box + BOX, &tmQ, &bars[kQFull + slot], 64, it.g * a.G, q);
+            }
+            continue;
+          }
           const uint32_t dst = smem_u32(qsm + slot * TILE);
           const int piece = lane & 15;  // 16 bytes of a row
-          int q = (it.r0 + hd * BM + (lane >> 4)) / a.G, h = it.r0 + hd * BM + (lane >> 4) - q * a.G;  // row's query and head
+          int q = quot(it.r0 + hd * BM + (lane >> 4), a.G, a.recip_G), h = it.r0 + hd * BM + (lane >> 4) - q * a.G;  // row's query and head
 #pragma unroll 4
           for (int i = 0; i < 64; i++) {
             const int row = (lane >> 4) + 2 * i;
@@ -563,41 +547,39 @@ __global__ void __launch_bounds__(384, 1)
     float f_l = 0.f;
     bool fin = false;
     auto epilogue = [&]() {
-      uint32_t o[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; c++) tmem_ld32(oc + 32 * c, o[c]);
-      tmem_ld_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) bar_arrive(bar(kOFree + hd));
       const bool empty = f_lo > f_hi;
-      const float inv = empty ? 0.f : 1.f / f_l;
+      const float inv = 1.f / f_l;
+      const uint64_t inv2 = f2(inv, inv);
       uint64_t sum = f2(0.f, 0.f);
+      T* dst = static_cast<T*>(a.out) + ((long long)f_row * a.H + f_head) * HD;
+#pragma unroll 1
+      for (int c = 0; c < 4; c++) {
+        uint32_t o[32];
+        tmem_ld32(oc + 32 * c, o);
+        tmem_ld_wait();
+        float w[16];
 #pragma unroll
-      for (int c = 0; c < 4; c++)
-#pragma unroll
-        for (int i = 0; i < 32; i += 2)  // NaN once anything is not finite
-          sum = f2_fma(f2(__uint_as_float(o[c][i]), __uint_as_float(o[c][i + 1])), f2(0.f, 0.f), sum);
+        for (int i = 0; i < 16; i++) {
+          const uint64_t y = f2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]));
+          sum = f2_fma(y, f2(0.f, 0.f), sum);  // NaN once anything is not finite
+          float y0, y1;
+          f2_get(f2_mul(y, inv2), y0, y1);
+          w[i] = __uint_as_float(pack16<BF16>(y0, y1));
+        }
+        if (f_row >= 0 && !empty) {
+          st_global_v8(reinterpret_cast<float*>(dst + 32 * c), w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]);
+          st_global_v8(reinterpret_cast<float*>(dst + 32 * c + 16), w[8], w[9], w[10], w[11], w[12], w[13], w[14], w[15]);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();  // (also: a row's stores come before row_alone's)
+      if (lane == 0) bar_arrive(bar(kOFree + hd));
       float s0, s1;
       f2_get(sum, s0, s1);
       const bool bad = f_row >= 0 && !empty && !(s0 + s1 == 0.f && f_l > 0.f && f_l < INFINITY);
-      if (f_row >= 0 && !bad) {
-        T* dst = static_cast<T*>(a.out) + ((long long)f_row * a.H + f_head) * HD;
-#pragma unroll
-        for (int c = 0; c < 4; c++)
-#pragma unroll
-          for (int i = 0; i < 32; i += 16) {
-            uint32_t w[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-              const float y0 = empty ? 0.f : __uint_as_float(o[c][i + 2 * e]) * inv;
-              const float y1 = empty ? 0.f : __uint_as_float(o[c][i + 2 * e + 1]) * inv;
-              w[e] = pack16<BF16>(y0, y1);
-            }
-            st_global_v8(reinterpret_cast<float*>(dst + 32 * c + i), __uint_as_float(w[0]), __uint_as_float(w[1]), __uint_as_float(w[2]),
-                         __uint_as_float(w[3]), __uint_as_float(w[4]), __uint_as_float(w[5]), __uint_as_float(w[6]), __uint_as_float(w[7]));
-          }
-      }
+      if (f_row >= 0 && empty)
+#pragma unroll 1
+        for (int i = 0; i < HD; i += 16) st_global_v8(reinterpret_cast<float*>(dst + i), 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f);
       for (uint32_t rows = __ballot_sync(0xffffffffu, bad); rows; rows &= rows - 1) {
         const int src = __ffs(rows) - 1;
         row_alone<T>(a, __shfl_sync(0xffffffffu, f_row, src), __shfl_sync(0xffffffffu, f_head, src),
@@ -611,11 +593,12 @@ __global__ void __launch_bounds__(384, 1)
     for (int k = 0; ok && next.g >= 0; k++) {
       const Item it = unpack(next);
       next = load_item(k + 1);
-      const int first = it.r0 + hd * BM, r = first + row, qi = r / a.G, pos = it.lk - it.lq + qi;
+      const int first = it.r0 + hd * BM, r = first + row, qi = quot(r, a.G, a.recip_G), pos = it.lk - it.lq + qi;
+      const int q_first = quot(first, a.G, a.recip_G), q_last = min(it.lq - 1, quot(first + BM - 1, a.G, a.recip_G));
       const bool exists = qi < it.lq;
       // every row of the half sees keys [all_lo, all_hi]
-      const int all_hi = first / a.G < it.lq ? it.lk - it.lq + first / a.G : -1;
-      const int all_lo = a.window > 0 ? it.lk - it.lq + min(it.lq - 1, (first + BM - 1) / a.G) - a.window + 1 : 0;
+      const int all_hi = q_first < it.lq ? it.lk - it.lq + q_first : -1;
+      const int all_lo = a.window > 0 ? it.lk - it.lq + q_last - a.window + 1 : 0;
       const int row_lo = a.window > 0 ? max(0, pos - a.window + 1) : 0, row_hi = exists ? pos : -1;
       float m_use = -INFINITY, l = 0.f;
       for (int j = 0; j < it.ntiles; j++) {
@@ -659,7 +642,7 @@ __global__ void __launch_bounds__(384, 1)
         }
         tc_fence_after();
         if (__any_sync(0xffffffffu, rescale_o)) {
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < 4; c++) {
             uint32_t r32[32];
             tmem_ld32(oc + 32 * c, r32);
@@ -679,13 +662,8 @@ __global__ void __launch_bounds__(384, 1)
         uint64_t ls2[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
         auto half_p = [&](const uint32_t (&x)[32], bool ex, const uint32_t (&y)[32], bool ey, uint32_t col, int done) {
           uint32_t pk[32];
-          if (full) {
-            chunk_p<BF16, true, 0>(x, false, scale2, negm2, ls2, pk);
-            chunk_p<BF16, true, 16>(y, false, scale2, negm2, ls2, pk);
-          } else {
-            chunk_p<BF16, false, 0>(x, ex, scale2, negm2, ls2, pk);
-            chunk_p<BF16, false, 16>(y, ey, scale2, negm2, ls2, pk);
-          }
+          chunk_p<BF16, 0>(x, ex, scale2, negm2, ls2, pk);
+          chunk_p<BF16, 16>(y, ey, scale2, negm2, ls2, pk);
           tmem_st32(pc + col, pk);
           tmem_st_wait();
           tc_fence_before();
@@ -703,7 +681,7 @@ __global__ void __launch_bounds__(384, 1)
       if (!ok) break;
       fin = true;
       f_row = exists ? it.q0 + qi : -1;
-      f_head = it.g * a.G + r % a.G;
+      f_head = it.g * a.G + r - qi * a.G;
       f_k0 = it.k0;
       f_lo = row_lo, f_hi = row_hi;
       f_l = l;
@@ -727,7 +705,7 @@ constexpr size_t kSmem = 1024 + Q_SLOTS * TILE + KV_STAGES * KV_STAGE;
 static_assert(kSmem <= 227 * 1024, "shared memory");
 
 template <bool BF16>
-int launch(hcu_context* h, const VarlenArgs& a, const CUtensorMap& tk, const CUtensorMap& tv, int grid) {
+int launch(hcu_context* h, const VarlenArgs& a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, int grid) {
   const char* op = "hcu_prefill_varlen";
   auto kern = prefill_varlen_kernel<BF16>;
   static std::atomic<uint64_t> attr_done{0};  // per device
@@ -746,7 +724,7 @@ int launch(hcu_context* h, const VarlenArgs& a, const CUtensorMap& tk, const CUt
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return check_cuda(cudaLaunchKernelEx(&cfg, kern, tk, tv, a), "hcu_prefill_varlen: launch");
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, tq, tk, tv, a), "hcu_prefill_varlen: launch");
 }
 
 }  // namespace
@@ -795,6 +773,8 @@ extern "C" int hcu_prefill_varlen(hcu_handle h, const hcu_prefill_varlen_params*
   a.KV = (int)p->KV;
   a.G = a.H / a.KV;
   a.window = (int)p->window;
+  a.recip_G = (uint32_t)std::min<uint64_t>(0xffffffffull, (1ull << 32) / a.G + 1);
+  a.recip_KV = (uint32_t)std::min<uint64_t>(0xffffffffull, (1ull << 32) / a.KV + 1);
   a.total_q = (int)p->total_q;
   a.total_k = (int)p->total_k;
   a.scale_log2 = hcu::kLog2e / sqrtf(128.f);
@@ -802,24 +782,26 @@ extern "C" int hcu_prefill_varlen(hcu_handle h, const hcu_prefill_varlen_params*
   // The item list lives in the workspace, behind the other ops' tickets.
   const long long most = ((long long)a.total_q * a.G + 2 * hcu::BM - 1) / (2 * hcu::BM) + a.batch;  // blocks of 256 rows
   const size_t offsets = ((size_t)(a.batch + 1) * sizeof(int) + 15) / 16 * 16, need = hcu::kTicketBytes + offsets + (size_t)most * 2 * sizeof(int4);
-  if (most * a.KV > 0x7fffffffLL) return fail(HCU_EINVAL, "%s: too many rows", op);
+  if (most * a.KV > 0x3fffffffLL || (long long)a.total_q * a.G > 0x3fffffffLL) return fail(HCU_EINVAL, "%s: too many rows", op);
   if (need > h->workspace_bytes)
     return fail(HCU_ENOMEM, "%s: the list of %lld blocks needs a workspace of %zu bytes (this one has %zu)", op, most, need, h->workspace_bytes);
   uint8_t* ws = static_cast<uint8_t*>(h->workspace) + hcu::kTicketBytes;
   a.blocks = reinterpret_cast<int*>(ws);
   a.items = reinterpret_cast<int4*>(ws + offsets);
-  CUtensorMap tk, tv;
-  for (int i = 0; i < 2; i++) {
-    // Without any key the map covers a row of q (all of whose "keys" are masked).
-    const void* base = a.total_k ? (i ? v : k) : q;
-    const long long stride = i ? a.v_stride : a.k_stride;
-    const uint64_t dims[3] = {128, (uint64_t)a.KV, (uint64_t)(a.total_k ? a.total_k : 1)};
+  // Without any key the K and V maps cover a row of q (all of whose "keys" are masked).
+  CUtensorMap tq, tk, tv;
+  const CUtensorMapDataType dt = p->dtype == HCU_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  auto map = [&](CUtensorMap* m, const void* base, int heads, long long rows, long long stride, uint32_t box_heads, uint32_t box_rows) {
+    const uint64_t dims[3] = {128, (uint64_t)heads, (uint64_t)rows};
     const uint64_t strides[2] = {256, (uint64_t)stride * 2};
-    const uint32_t box[3] = {64, 1, 128};
-    HCU_TRY(hcu::make_tensor_map(i ? &tv : &tk, p->dtype == HCU_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                                 3, const_cast<void*>(base), dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B));
-  }
+    const uint32_t box[3] = {64, box_heads, box_rows};
+    return hcu::make_tensor_map(m, dt, 3, const_cast<void*>(base), dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  };
+  HCU_TRY(map(&tk, a.total_k ? k : q, a.KV, a.total_k ? a.total_k : 1, a.k_stride, 1, 128));
+  HCU_TRY(map(&tv, a.total_k ? v : q, a.KV, a.total_k ? a.total_k : 1, a.v_stride, 1, 128));
+  a.q_tma = a.G <= 128 && 128 % a.G == 0;
+  HCU_TRY(map(&tq, q, a.H, a.total_q, a.q_stride, a.q_tma ? (uint32_t)a.G : 1, a.q_tma ? 128u / a.G : 1));
   int grid = (int)std::min<long long>(h->sm_count, most * a.KV);
   if (h->opt_swa_ctas > 0 && h->opt_swa_ctas < grid) grid = (int)h->opt_swa_ctas;
-  return p->dtype == HCU_DT_BF16 ? hcu::launch<true>(h, a, tk, tv, grid) : hcu::launch<false>(h, a, tk, tv, grid);
+  return p->dtype == HCU_DT_BF16 ? hcu::launch<true>(h, a, tq, tk, tv, grid) : hcu::launch<false>(h, a, tq, tk, tv, grid);
 }
