@@ -634,7 +634,7 @@ __global__ void __launch_bounds__(384, 1)
         const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * a.scale_log2;
         const bool move = mx > m_use + RESCALE_LOG2 || (j == 0 && mx > m_use);
         const bool rescale_o = move && j > 0 && m_use != -INFINITY;
-        const float f = rescale_o ? exp2f(m_use - mx) : 1.f;
+        const float f = rescale_o ? ex2_approx(m_use - mx) : 1.f;
         // P and O are this thread's again once the product of the tile before is done.
         if (t > 0 && !wait(kPVDone + hd, (t - 1) & 1)) {
           ok = false;
