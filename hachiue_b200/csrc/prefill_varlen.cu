@@ -635,13 +635,14 @@ __global__ void __launch_bounds__(384, 1)
         const bool move = mx > m_use + RESCALE_LOG2 || (j == 0 && mx > m_use);
         const bool rescale_o = move && j > 0 && m_use != -INFINITY;
         const float f = rescale_o ? ex2_approx(m_use - mx) : 1.f;
-        // P and O are this thread's again once the product of the tile before is done.
-        if (t > 0 && !wait(kPVDone + hd, (t - 1) & 1)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
+        // P and O are this thread's again once the product of the tile before is done: asked for here, needed when P is there.
+        const bool pv_done = t == 0 || bar_try(bar(kPVDone + hd), (t - 1) & 1);
         if (__any_sync(0xffffffffu, rescale_o)) {
+          if (t > 0 && !wait(kPVDone + hd, (t - 1) & 1)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < 4; c++) {
             uint32_t r32[32];
@@ -664,6 +665,10 @@ __global__ void __launch_bounds__(384, 1)
           uint32_t pk[32];
           chunk_p<BF16, 0>(x, ex, scale2, negm2, ls2, pk);
           chunk_p<BF16, 16>(y, ey, scale2, negm2, ls2, pk);
+          if (col == 0) {
+            if (!__all_sync(0xffffffffu, pv_done) && !wait(kPVDone + hd, (t - 1) & 1)) ok = false;
+            tc_fence_after();
+          }
           tmem_st32(pc + col, pk);
           tmem_st_wait();
           tc_fence_before();
@@ -676,6 +681,7 @@ __global__ void __launch_bounds__(384, 1)
         f2_get(ls2[0], a0, a1);
         f2_get(ls2[1], b0, b1);
         l += (a0 + a1) + (b0 + b1);
+        if (!ok) break;
         if (j == 0 && fin) epilogue();
       }
       if (!ok) break;
