@@ -132,10 +132,12 @@ class PagedKVCache:
     def c_struct(self) -> hcu_paged_kv:
         """The C view of the cache, checked and rebuilt only when a tensor
         changed (a decode step calls this once per layer)."""
-        key = (self.k, self.v, self.k_scale, self.v_scale)
         cached = self.__dict__.get("_c_struct")
-        # the tensors themselves are compared, not their addresses, which a freed cache's successor can have
-        if cached is None or any(a is not b for a, b in zip(cached[0], key)) or cached[2] != self.k.data_ptr():
+        k, v, ks, vs = self.k, self.v, self.k_scale, self.v_scale
+        # the tensors themselves are compared, and their places in memory, which can change under a tensor
+        if (cached is None or cached[0] is not k or cached[1] is not v or cached[2] is not ks or cached[3] is not vs
+                or cached[4] != (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr())):
+            key = (k, v, ks, vs)
             shape, scales = tuple(self.k.shape), (*self.k.shape[:3], self.k.shape[3] // 16)
             if (len(shape) != 4 or self.v.shape != self.k.shape or any(tuple(t.shape) != scales for t in key[2:])
                     or any(t.dtype != torch.uint8 for t in key[:2]) or any(t.dtype != torch.float16 for t in key[2:])
@@ -144,9 +146,9 @@ class PagedKVCache:
                                    "hachiue: a paged cache is contiguous uint8 k / v [n_pages, KV, page_size, Dh / 2] and "
                                    "f16 scales [n_pages, KV, page_size, Dh / 32] on one device")
             st = hcu_paged_kv(KV_Q4_0, shape[2], shape[0], shape[1], 2 * shape[3], *(_ptr(t) for t in key))
-            cached = (key, st, self.k.data_ptr())
+            cached = (*key, tuple(t.data_ptr() for t in key), st)
             self.__dict__["_c_struct"] = cached
-        return cached[1]
+        return cached[5]
 
 
 class CudaBackend:
@@ -162,6 +164,8 @@ class CudaBackend:
         self._h = h
         self._stream = None  # the stream last bound to the handle
         self._attn_params = hcu_attention_params()
+        self._paged_params, self._varlen_params = hcu_attention_paged_params(), hcu_prefill_varlen_params()
+        self._append_params = hcu_rope_append_params()
 
     # -- lifecycle -----------------------------------------------------------
     def close(self) -> None:
@@ -468,8 +472,9 @@ class CudaBackend:
     # -- paged serving ---------------------------------------------------------
     def _on_device(self, op: str, *tensors: torch.Tensor) -> None:
         """Refuses tensors of another device than the handle's."""
+        index = self.device.index
         for t in tensors:
-            if t.device != self.device:
+            if t.get_device() != index:  # -1 on the CPU
                 raise HachiueError(_lib.HCU_EINVAL, f"hachiue: {op}: a tensor is on {t.device}, the handle on {self.device}")
 
     def rope_append_paged(self, k: torch.Tensor, v: torch.Tensor, cache: PagedKVCache, slots: torch.Tensor,
@@ -523,8 +528,10 @@ class CudaBackend:
         if n == 0:
             return
         self._bind_stream()
-        p = hcu_rope_append_params(n, H, _DT[k.dtype], rotary, 0 if cos is None else cos.shape[0],
-                                   0 if q is None else self._row_stride(q), self._row_stride(k), self._row_stride(v))
+        p = self._append_params  # every field is set
+        p.n, p.H, p.dtype, p.rotaryDim, p.table_rows = n, H, _DT[k.dtype], rotary, 0 if cos is None else cos.shape[0]
+        p.q_row_stride = 0 if q is None else self._row_stride(q)
+        p.k_row_stride, p.v_row_stride = self._row_stride(k), self._row_stride(v)
         check(self.lib.hcu_rope_append_paged(self._h, ctypes.byref(p), _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(cos),
                                              _ptr(sin), _ptr(positions), slots.data_ptr(), _ptr(q_out), _ptr(k_out),
                                              ctypes.byref(kv)))
@@ -574,8 +581,10 @@ class CudaBackend:
             return
         pages = block_table.shape[1]
         self._bind_stream()
-        p = hcu_attention_paged_params(B, S, H, window_size, _DT[q.dtype], max_context or pages * kv.page_size, pages,
-                                       block_table.data_ptr(), context.data_ptr())
+        p = self._paged_params  # every field is set
+        p.batch, p.S, p.H, p.windowSize, p.dtype = B, S, H, window_size, _DT[q.dtype]
+        p.max_context, p.table_stride = max_context or pages * kv.page_size, pages
+        p.block_table, p.context = block_table.data_ptr(), context.data_ptr()
         check(self.lib.hcu_attention_paged(self._h, ctypes.byref(p), q.data_ptr(), ctypes.byref(kv), out.data_ptr()))
 
     def prefill_varlen(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor,
@@ -603,7 +612,9 @@ class CudaBackend:
         if nq == 0 or cu_q.shape[0] == 1:
             return
         self._bind_stream()
-        p = hcu_prefill_varlen_params(cu_q.shape[0] - 1, H, KV, D, window, _DT[q.dtype], nq, nk, cu_q.data_ptr(),
-                                      _ptr(cu_k), self._row_stride(q), self._row_stride(k), self._row_stride(v))
+        p = self._varlen_params  # every field is set
+        p.batch, p.H, p.KV, p.D, p.window, p.dtype = cu_q.shape[0] - 1, H, KV, D, window, _DT[q.dtype]
+        p.total_q, p.total_k, p.cu_q, p.cu_k = nq, nk, cu_q.data_ptr(), _ptr(cu_k)
+        p.q_row_stride, p.k_row_stride, p.v_row_stride = self._row_stride(q), self._row_stride(k), self._row_stride(v)
         check(self.lib.hcu_prefill_varlen(self._h, ctypes.byref(p), q.data_ptr(), k.data_ptr(), v.data_ptr(),
                                           out.data_ptr()))

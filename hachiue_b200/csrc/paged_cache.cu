@@ -2,9 +2,15 @@
 // append (hcu_rope_append_paged) and the gather (hcu_read_paged).
 //
 // Both move each row once and are bound by HBM for prompts and by launch
-// latency for single tokens.  One warp takes one row of one head; lane l holds
-// elements 4l .. 4l + 3 of each 128, so a Q4_0 block is eight lanes, a value
-// halfword is one lane's codes and a key word those of two.
+// latency for single tokens.
+//  * Append: a block per token, so that its cos and sin values are loaded once
+//    into registers for all of its rows; eight elements per lane, a row of 128
+//    being half a warp.  A Q4_0 block is then four lanes, a lane's codes one word of
+//    a key row or two halfwords of a value row.
+//  * Read: eight bytes of codes per lane, so that a warp has four rows of 128 of
+//    both tensors in flight, and writes whole 32-byte sectors.
+#include <algorithm>
+
 #include "paged.cuh"
 
 namespace hcu {
@@ -38,114 +44,113 @@ __device__ __forceinline__ uint32_t q4_code(float y, float a, float inv) {
   return (uint32_t)(int)fminf(fmaxf(c, 0.f), 15.f);
 }
 
-// Quantises the four elements of each lane: a block is the eight lanes of
-// equal lane / 8.  Returns the lane's four codes (element 0 lowest) and the
-// block's scale.
-__device__ __forceinline__ uint32_t q4_block(const float (&x)[4], int lane, __half* scale) {
+// Quantises the eight elements of each lane: a block is four lanes.  Returns the
+// lane's codes (element 0 lowest) and the block's scale.  The whole warp calls it.
+__device__ __forceinline__ uint32_t q4_block(const float (&x)[8], int lane, __half* scale) {
   uint32_t top = 0;
   float m = x[0];  // the lane's first element of the lane's largest magnitude
 #pragma unroll
-  for (int c = 0; c < 4; c++) {
+  for (int c = 0; c < 8; c++) {
     const uint32_t b = __float_as_uint(x[c]) & 0x7fffffffu;
     if (b > top) {
       top = b;
       m = x[c];
     }
   }
-  uint32_t all = top;
-#pragma unroll
-  for (int o = 1; o < 8; o <<= 1) all = max(all, __shfl_xor_sync(0xffffffffu, all, o));
+  uint32_t all = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  all = max(all, __shfl_xor_sync(0xffffffffu, all, 2));
   const uint32_t same = __ballot_sync(0xffffffffu, top == all);
-  const int first = (lane & 24) + __ffs((same >> (lane & 24)) & 0xffu) - 1;
+  const int first = (lane & 28) + __ffs((same >> (lane & 28)) & 0xfu) - 1;
   m = __shfl_sync(0xffffffffu, m, first);
   const __half d = __float2half_rn(fminf(fmaxf(m * -0.125f, -65504.f), 65504.f));
   *scale = d;
   const float df = __half2float(d), a = fabsf(df);
-  if (a == 0.f) return 0x8888u;
+  if (a == 0.f) return 0x88888888u;
   const float inv = __fdiv_rn(1.f, a);
   const uint32_t sign = __float_as_uint(df) & 0x80000000u;
   uint32_t code = 0;
 #pragma unroll
-  for (int c = 0; c < 4; c++) code |= q4_code(__uint_as_float(__float_as_uint(x[c]) ^ sign), a, inv) << (4 * c);
+  for (int c = 0; c < 8; c++) code |= q4_code(__uint_as_float(__float_as_uint(x[c]) ^ sign), a, inv) << (4 * c);
   return code;
 }
 
 template <typename T, int DH>
 __global__ void __launch_bounds__(256) rope_append_kernel(const AppendArgs a) {
-  constexpr int NJ = DH / 128, NB = DH / 32;
-  const int lane = threadIdx.x & 31, heads = a.H + 2 * a.kv.KV;
-  const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (row >= (long long)a.n * heads) return;
-  const int i = (int)(row / heads), r = (int)(row % heads);
+  constexpr int LPR = DH / 8, RPB = 256 / LPR, NB = DH / 32;  // lanes per row, rows per pass of the block
+  const int lane = threadIdx.x & 31, l = threadIdx.x % LPR, heads = a.H + 2 * a.kv.KV, i = blockIdx.x;
   const long long slot = a.slots[i];
   if (slot < 0) return;
   const int pos = a.half ? a.positions[i] : 0;
   if (slot >= a.n_slots || (a.half && (pos < 0 || pos >= a.table_rows))) {
-    if (r == 0 && lane == 0) atomicOr(a.status, HCU_DEVERR_BADARG);
+    if (threadIdx.x == 0 && blockIdx.y == 0) atomicOr(a.status, HCU_DEVERR_BADARG);
     return;
   }
-  const int kind = r < a.H ? 0 : (r < a.H + a.kv.KV ? 1 : 2);  // q, k, v
-  const int g = kind == 0 ? r : (kind == 1 ? r - a.H : r - a.H - a.kv.KV);
-  const T* src = kind == 0   ? static_cast<const T*>(a.q) + i * a.q_stride
-                 : kind == 1 ? static_cast<const T*>(a.k) + i * a.k_stride
-                             : static_cast<const T*>(a.v) + i * a.v_stride;
-  src += (long long)g * DH;
-  float x[NJ][4];
+  // The lane's elements 8l .. 8l + 7 in two groups of four, which may lie on different sides of the pairs' halves.
+  float cs[2][4] = {}, sn[2][4] = {};  // sn: negative for the lower half of the pairs
+  int partner[2];
 #pragma unroll
-  for (int j = 0; j < NJ; j++) load4(src + 128 * j + 4 * lane, x[j]);
-  if (kind < 2) {
-    // The partner elements come from memory again (the row is in L1), so any
-    // rotaryDim that is a multiple of 8 takes the same path.
-    const float* ct = a.cos_tab + (long long)pos * a.half;
-    const float* st = a.sin_tab + (long long)pos * a.half;
-    float w[NJ][4];
+  for (int u = 0; u < 2; u++) {
+    const int e = 8 * l + 4 * u;
+    partner[u] = -1;
+    if (e < 2 * a.half) {
+      const bool low = e < a.half;
+      const int at = low ? e : e - a.half;
+      load4(a.cos_tab + (long long)pos * a.half + at, cs[u]);
+      load4(a.sin_tab + (long long)pos * a.half + at, sn[u]);
+      if (low)
 #pragma unroll
-    for (int j = 0; j < NJ; j++) {
-      const int e = 128 * j + 4 * lane;
-      if (e < 2 * a.half) load4(src + (e < a.half ? e + a.half : e - a.half), w[j]);
+        for (int c = 0; c < 4; c++) sn[u][c] = -sn[u][c];
+      partner[u] = low ? e + a.half : e - a.half;
     }
-    __syncwarp();  // in place: the row has been read before any lane writes
-#pragma unroll
-    for (int j = 0; j < NJ; j++) {
-      const int e = 128 * j + 4 * lane;
-      if (e < 2 * a.half) {
-        const bool low = e < a.half;
-        float c[4], s[4];
-        load4(ct + (low ? e : e - a.half), c);
-        load4(st + (low ? e : e - a.half), s);
-#pragma unroll
-        for (int t = 0; t < 4; t++) {
-          const float sg = low ? -s[t] : s[t];
-          if (kind == 0)
-            x[j][t] = fmaf(x[j][t], c[t], w[j][t] * sg);
-          else  // the products of two f32 values are exact in f64
-            x[j][t] = (float)__dadd_rn(__dmul_rn(x[j][t], c[t]), __dmul_rn(w[j][t], sg));
-        }
-      }
-    }
-    T* dst = kind == 0 ? static_cast<T*>(a.q_out) : static_cast<T*>(a.k_out);
-    if (dst) {
-      dst += ((long long)i * (kind == 0 ? a.H : a.kv.KV) + g) * DH;
-#pragma unroll
-      for (int j = 0; j < NJ; j++) store4(dst + 128 * j + 4 * lane, x[j]);
-    }
-    if (kind == 0) return;
   }
-  const long long at = paged_row(a.kv, slot >> a.kv.page_log2, g, (int)(slot & ((1 << a.kv.page_log2) - 1)));
-  uint8_t* codes = (kind == 1 ? a.kv.k : a.kv.v) + at * (DH / 2);
-  __half* scales = (kind == 1 ? a.kv.ks : a.kv.vs) + at * NB;
+  const long long at0 = paged_row(a.kv, slot >> a.kv.page_log2, 0, (int)(slot & ((1 << a.kv.page_log2) - 1)));
+  for (int base = blockIdx.y * RPB; base < heads; base += gridDim.y * RPB) {
+    const int r = base + threadIdx.x / LPR;
+    const bool row = r < heads;
+    const int kind = r < a.H ? 0 : (r < a.H + a.kv.KV ? 1 : 2);  // q, k, v
+    const int g = kind == 0 ? r : (kind == 1 ? r - a.H : r - a.H - a.kv.KV);
+    const T* src = kind == 0   ? static_cast<const T*>(a.q) + i * a.q_stride
+                   : kind == 1 ? static_cast<const T*>(a.k) + i * a.k_stride
+                               : static_cast<const T*>(a.v) + i * a.v_stride;
+    src += (long long)g * DH;
+    float x[8] = {}, w[2][4] = {};
+    if (row) {
+      load8(src + 8 * l, x);
+      if (kind < 2)
 #pragma unroll
-  for (int j = 0; j < NJ; j++) {
-    const int b = 4 * j + (lane >> 3), l = lane & 7;  // block, lane in the block
-    __half d;
-    const uint32_t c = q4_block(x[j], lane, &d);
-    if (kind == 1) {
-      const uint32_t hi = __shfl_xor_sync(0xffffffffu, c, 1);
-      if (!(l & 1)) *reinterpret_cast<uint32_t*>(codes + ((l >> 1) * NB + b) * 4) = c | hi << 16;
-    } else {
-      *reinterpret_cast<uint16_t*>(codes + (l * NB + b) * 2) = (uint16_t)c;
+        for (int u = 0; u < 2; u++)  // the partner elements come from memory again (the row is in L1)
+          if (partner[u] >= 0) load4(src + partner[u], w[u]);
     }
-    if (l == 0) scales[b] = d;
+    __syncwarp();  // in place: a row has been read before any lane writes
+    if (row && kind < 2) {
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+        if (partner[u] >= 0)
+#pragma unroll
+          for (int c = 0; c < 4; c++) {
+            if (kind == 0)
+              x[4 * u + c] = fmaf(x[4 * u + c], cs[u][c], w[u][c] * sn[u][c]);
+            else  // the products of two f32 values are exact in f64
+              x[4 * u + c] = (float)__dadd_rn(__dmul_rn(x[4 * u + c], cs[u][c]), __dmul_rn(w[u][c], sn[u][c]));
+          }
+      T* dst = kind == 0 ? static_cast<T*>(a.q_out) : static_cast<T*>(a.k_out);
+      if (dst) store8(dst + ((long long)i * (kind == 0 ? a.H : a.kv.KV) + g) * DH + 8 * l, x);
+    }
+    if (!__any_sync(0xffffffffu, row && kind > 0)) continue;
+    __half d;
+    const uint32_t code = q4_block(x, lane, &d);
+    if (!row || kind == 0) continue;
+    const long long at = at0 + ((long long)g << a.kv.page_log2);
+    const int b = l >> 2, t = l & 3;  // block, quarter of it
+    if (kind == 1) {
+      *reinterpret_cast<uint32_t*>(a.kv.k + at * (DH / 2) + (t * NB + b) * 4) = code;
+      if (t == 0) a.kv.ks[at * NB + b] = d;
+    } else {
+      uint8_t* v = a.kv.v + at * (DH / 2);
+      *reinterpret_cast<uint16_t*>(v + (2 * t * NB + b) * 2) = (uint16_t)code;
+      *reinterpret_cast<uint16_t*>(v + ((2 * t + 1) * NB + b) * 2) = (uint16_t)(code >> 16);
+      if (t == 0) a.kv.vs[at * NB + b] = d;
+    }
   }
 }
 
@@ -159,35 +164,64 @@ struct ReadArgs {
   uint32_t* status;
 };
 
+// The values of N codes (lowest bits first) with scale d.
+template <int N>
+__device__ __forceinline__ void q4_values(uint32_t codes, float d, float (&x)[N]) {
+#pragma unroll
+  for (int c = 0; c < N; c++) x[c] = (float)((int)((codes >> (4 * c)) & 15u) - 8) * d;
+}
+
 template <typename T, int DH>
 __global__ void __launch_bounds__(256) read_paged_kernel(const ReadArgs a) {
-  constexpr int NJ = DH / 128, NB = DH / 32;
-  const int lane = threadIdx.x & 31;
-  const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (row >= (long long)a.n * a.kv.KV * 2) return;
-  const int i = (int)(row / (2 * a.kv.KV)), r = (int)(row % (2 * a.kv.KV));
-  const long long slot = a.slots[i];
-  if (slot < 0) return;
-  if (slot >= a.n_slots) {
-    if (r == 0 && lane == 0) atomicOr(a.status, HCU_DEVERR_BADARG);
-    return;
+  constexpr int NB = DH / 32, LPR = DH / 16, RPW = 32 / LPR, UNROLL = 2;  // lanes per row, rows per pass of a warp
+  const int lane = threadIdx.x & 31, l = lane % LPR;
+  const long long rows = (long long)a.n * a.kv.KV;
+  const long long row0 = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * (RPW * UNROLL) + lane / LPR;
+  uint2 kc[UNROLL], vc[UNROLL];
+  uint32_t kd[UNROLL];
+  uint2 vd[UNROLL];
+  bool there[UNROLL];
+  const int kb = 2 * l % NB, kt = 2 * l / NB;  // key words 2l, 2l + 1: dimensions 8 kt .. of blocks kb, kb + 1
+  const int vb = 4 * l % NB, vg = 4 * l / NB;  // value halfwords 4l .. 4l + 3: dimensions 4 vg .. of blocks vb .. vb + 3
+#pragma unroll
+  for (int u = 0; u < UNROLL; u++) {
+    const long long row = row0 + u * RPW;
+    there[u] = false;
+    if (row < rows) {
+      const int i = (int)(row / a.kv.KV), g = (int)(row - (long long)i * a.kv.KV);
+      const long long slot = a.slots[i];
+      if (slot >= a.n_slots) {
+        if (l == 0) atomicOr(a.status, HCU_DEVERR_BADARG);
+      } else if (slot >= 0) {
+        const long long at = paged_row(a.kv, slot >> a.kv.page_log2, g, (int)(slot & ((1 << a.kv.page_log2) - 1)));
+        kc[u] = *reinterpret_cast<const uint2*>(a.kv.k + at * (DH / 2) + 8 * l);
+        vc[u] = *reinterpret_cast<const uint2*>(a.kv.v + at * (DH / 2) + 8 * l);
+        kd[u] = *reinterpret_cast<const uint32_t*>(a.kv.ks + at * NB + kb);
+        vd[u] = *reinterpret_cast<const uint2*>(a.kv.vs + at * NB + vb);
+        there[u] = true;
+      }
+    }
   }
-  const bool key = r < a.kv.KV;
-  const int g = key ? r : r - a.kv.KV;
-  const long long at = paged_row(a.kv, slot >> a.kv.page_log2, g, (int)(slot & ((1 << a.kv.page_log2) - 1)));
-  const uint8_t* codes = (key ? a.kv.k : a.kv.v) + at * (DH / 2);
-  const __half* scales = (key ? a.kv.ks : a.kv.vs) + at * NB;
-  T* dst = static_cast<T*>(key ? a.k_out : a.v_out) + ((long long)i * a.kv.KV + g) * DH;
 #pragma unroll
-  for (int j = 0; j < NJ; j++) {
-    const int b = 4 * j + (lane >> 3), l = lane & 7;
-    const uint32_t c = key ? *reinterpret_cast<const uint16_t*>(codes + ((l >> 1) * NB + b) * 4 + (l & 1) * 2)
-                           : *reinterpret_cast<const uint16_t*>(codes + (l * NB + b) * 2);
-    const float d = __half2float(scales[b]);
-    float x[4];
-#pragma unroll
-    for (int t = 0; t < 4; t++) x[t] = (float)((int)((c >> (4 * t)) & 15u) - 8) * d;
-    store4(dst + 128 * j + 4 * lane, x);
+  for (int u = 0; u < UNROLL; u++) {
+    if (!there[u]) continue;
+    const long long out = (row0 + u * RPW) * DH;
+    T* k = static_cast<T*>(a.k_out) + out;
+    T* v = static_cast<T*>(a.v_out) + out;
+    const float2 ds = f16x2_to_f2(kd[u]), d0 = f16x2_to_f2(vd[u].x), d1 = f16x2_to_f2(vd[u].y);
+    float x[8], y[4];
+    q4_values(kc[u].x, ds.x, x);
+    store8(k + 32 * kb + 8 * kt, x);
+    q4_values(kc[u].y, ds.y, x);
+    store8(k + 32 * (kb + 1) + 8 * kt, x);
+    q4_values(vc[u].x, d0.x, y);
+    store4(v + 32 * vb + 4 * vg, y);
+    q4_values(vc[u].x >> 16, d0.y, y);
+    store4(v + 32 * (vb + 1) + 4 * vg, y);
+    q4_values(vc[u].y, d1.x, y);
+    store4(v + 32 * (vb + 2) + 4 * vg, y);
+    q4_values(vc[u].y >> 16, d1.y, y);
+    store4(v + 32 * (vb + 3) + 4 * vg, y);
   }
 }
 
@@ -204,16 +238,18 @@ int with_dtype(const char* op, uint32_t dtype, F&& f) {
 
 template <typename T>
 int launch_append(hcu_context* h, const AppendArgs& a, int dh) {
-  const long long blocks = ((long long)a.n * (a.H + 2 * a.kv.KV) + 7) / 8;
-  if (blocks > 0x7fffffffLL) return fail(HCU_EINVAL, "hcu_rope_append_paged: too many rows");
-  if (dh == 128) rope_append_kernel<T, 128><<<(unsigned)blocks, 256, 0, h->stream>>>(a);
-  else rope_append_kernel<T, 256><<<(unsigned)blocks, 256, 0, h->stream>>>(a);
+  // Few tokens: a block per pass of rows.  Many: one per token, which walks its rows.
+  const int passes = (a.H + 2 * a.kv.KV + 256 / (dh / 8) - 1) / (256 / (dh / 8));
+  const dim3 grid((unsigned)a.n, a.n < 4 * h->sm_count ? (unsigned)std::min(passes, 65535) : 1u);
+  if (dh == 128) rope_append_kernel<T, 128><<<grid, 256, 0, h->stream>>>(a);
+  else rope_append_kernel<T, 256><<<grid, 256, 0, h->stream>>>(a);
   return after_launch("hcu_rope_append_paged: launch");
 }
 
 template <typename T>
 int launch_read(hcu_context* h, const ReadArgs& a, int dh) {
-  const long long blocks = ((long long)a.n * a.kv.KV * 2 + 7) / 8;
+  const int per_block = 8 * 2 * (32 / (dh / 16));  // rows
+  const long long blocks = ((long long)a.n * a.kv.KV + per_block - 1) / per_block;
   if (blocks > 0x7fffffffLL) return fail(HCU_EINVAL, "hcu_read_paged: too many rows");
   if (dh == 128) read_paged_kernel<T, 128><<<(unsigned)blocks, 256, 0, h->stream>>>(a);
   else read_paged_kernel<T, 256><<<(unsigned)blocks, 256, 0, h->stream>>>(a);
@@ -249,14 +285,14 @@ extern "C" int hcu_rope_append_paged(hcu_handle h, const hcu_rope_append_params*
   const uint64_t qs = p->q_row_stride ? p->q_row_stride : (uint64_t)p->H * kv->Dh;
   const uint64_t ks = p->k_row_stride ? p->k_row_stride : (uint64_t)kv->KV * kv->Dh;
   const uint64_t vs = p->v_row_stride ? p->v_row_stride : (uint64_t)kv->KV * kv->Dh;
-  if (qs % 4 || ks % 4 || vs % 4) return fail(HCU_EINVAL, "%s: row strides must be multiples of 4 elements", op);
+  if (qs % 8 || ks % 8 || vs % 8) return fail(HCU_EINVAL, "%s: row strides must be multiples of 8 elements", op);
   if (qs < (uint64_t)p->H * kv->Dh || ks < (uint64_t)kv->KV * kv->Dh || vs < (uint64_t)kv->KV * kv->Dh)
     return fail(HCU_EINVAL, "%s: a row stride is shorter than its row", op);
   if ((qs | ks | vs) >> 40) return fail(HCU_EINVAL, "%s: a row stride is too large", op);
   const uintptr_t rows = reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
                          reinterpret_cast<uintptr_t>(k_out) |
                          (p->H ? reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(q_out) : 0);
-  if (rows % (4 * eb)) return fail(HCU_EINVAL, "%s: rows must be aligned to four elements", op);
+  if (rows % 16) return fail(HCU_EINVAL, "%s: rows must be 16-byte aligned", op);
   if (p->rotaryDim && ((reinterpret_cast<uintptr_t>(cos_tab) | reinterpret_cast<uintptr_t>(sin_tab)) % 16))
     return fail(HCU_EINVAL, "%s: cos and sin must be 16-byte aligned", op);
   if (p->H && q_out == q && qs != (uint64_t)p->H * kv->Dh)
@@ -298,8 +334,8 @@ extern "C" int hcu_read_paged(hcu_handle h, uint32_t n, uint32_t dtype, const in
   if (n > 0x7fffffffu) return fail(HCU_EINVAL, "%s: n too large", op);
   if (n == 0) return HCU_OK;
   if (!slots || !k_out || !v_out) return fail(HCU_EINVAL, "%s: null slots or output", op);
-  if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) % (4 * eb))
-    return fail(HCU_EINVAL, "%s: outputs must be aligned to four elements", op);
+  if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) % 16)
+    return fail(HCU_EINVAL, "%s: outputs must be 16-byte aligned", op);
   a.slots = slots;
   a.n_slots = (long long)kv->n_pages << a.kv.page_log2;
   a.n = (int)n;

@@ -570,7 +570,7 @@ typedef struct {
  * `dtype`, rows at the given strides in elements (0 = dense: views of one fused
  * projection have its width), k_out and q_out dense, of the same type; q_out
  * may be a dense q itself and k_out a dense k (in place).  rotaryDim is a
- * multiple of 8, at most Dh.  Row pointers and strides are multiples of four
+ * multiple of 8, at most Dh.  Rows are 16-byte aligned, strides multiples of 8
  * elements.
  *
  * A negative slot marks padding: nothing of that row is read but its slot, and
@@ -589,7 +589,7 @@ int hcu_rope_append_paged(hcu_handle h, const hcu_rope_append_params *p, const v
 /* Gathers cached rows: k_out and v_out [n, KV, Dh] of `dtype` receive the
  * values that slot slots[i]'s row stands for, rounded once (a shared prefix
  * as dense keys and values for hcu_prefill_varlen).  A slot may be named more
- * than once.  A negative slot leaves its output rows as they were, a slot past
+ * than once.  The outputs are 16-byte aligned.  A negative slot leaves its output rows as they were, a slot past
  * the cache does too and sets bit 2 of the device status. */
 int hcu_read_paged(hcu_handle h, uint32_t n, uint32_t dtype, const int64_t *slots, const hcu_paged_kv *kv,
                    void *k_out, void *v_out);
