@@ -510,36 +510,36 @@ class CudaBackend:
             raise HachiueError(_lib.HCU_EINVAL, "hachiue: rope_append_paged: sin without cos")
         if (q is None) != (q_out is None):
             raise HachiueError(_lib.HCU_EINVAL, "hachiue: rope_append_paged: q and q_out go together")
-        rows = [k, v]
+        strides = self._row_stride(k, "rope_append_paged"), self._row_stride(v, "rope_append_paged")
+        q_stride = 0
         if q is not None:
             self._on_device("rope_append_paged", q, q_out)
             if (q.shape != (n, H, Dh) or q.dtype != k.dtype or q_out.shape != q.shape or q_out.dtype != k.dtype
                     or not q_out.is_contiguous()):
                 raise HachiueError(_lib.HCU_EINVAL, "hachiue: rope_append_paged takes q and a contiguous q_out [n, H, Dh] "
                                                     "of k's dtype")
-            rows.append(q)
+            q_stride = self._row_stride(q, "rope_append_paged")
         if k_out is not None:
             self._on_device("rope_append_paged", k_out)
             if k_out.shape != k.shape or k_out.dtype != k.dtype or not k_out.is_contiguous():
                 raise HachiueError(_lib.HCU_EINVAL, "hachiue: rope_append_paged takes a contiguous k_out like k")
-        for t in rows:
-            if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != Dh):
-                raise HachiueError(_lib.HCU_EINVAL, "hachiue: rope_append_paged: heads must be contiguous")
         if n == 0:
             return
         self._bind_stream()
         p = self._append_params  # every field is set
         p.n, p.H, p.dtype, p.rotaryDim, p.table_rows = n, H, _DT[k.dtype], rotary, 0 if cos is None else cos.shape[0]
-        p.q_row_stride = 0 if q is None else self._row_stride(q)
-        p.k_row_stride, p.v_row_stride = self._row_stride(k), self._row_stride(v)
+        p.q_row_stride, p.k_row_stride, p.v_row_stride = q_stride, *strides
         check(self.lib.hcu_rope_append_paged(self._h, ctypes.byref(p), _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(cos),
                                              _ptr(sin), _ptr(positions), slots.data_ptr(), _ptr(q_out), _ptr(k_out),
                                              ctypes.byref(kv)))
 
     @staticmethod
-    def _row_stride(t: torch.Tensor) -> int:
-        """Elements between the token rows of t [n, heads, D] (0, dense, for a single row)."""
-        return t.stride(0) if t.shape[0] > 1 else 0
+    def _row_stride(t: torch.Tensor, op: str) -> int:
+        """Elements between the token rows of t [n, heads, D], whose heads are contiguous (0, dense, for a single row)."""
+        (n, heads, D), (row, head, one) = t.shape, t.stride()
+        if one != 1 or (head != D and heads > 1):
+            raise HachiueError(_lib.HCU_EINVAL, f"hachiue: {op}: heads must be contiguous")
+        return row if n > 1 else 0
 
     def read_paged(self, cache: PagedKVCache, slots: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor) -> None:
         """The values of cached rows: k_out, v_out [n, KV, Dh] (f32, f16 or
@@ -595,26 +595,26 @@ class CudaBackend:
         [B + 1] offsets of the sequences (cu_k None: the same).  With more
         keys than queries the queries are the last tokens; window 0 = causal."""
         self._on_device("prefill_varlen", q, k, v, out, cu_q)
-        if cu_k is not None:
-            self._on_device("prefill_varlen", cu_k)
         nq, H, D = q.shape
         nk, KV = k.shape[:2]
-        if (q.dtype not in (torch.bfloat16, torch.float16) or any(t.dtype != q.dtype for t in (k, v, out))
+        dtype = q.dtype
+        if (dtype not in (torch.bfloat16, torch.float16) or k.dtype != dtype or v.dtype != dtype or out.dtype != dtype
                 or k.shape != (nk, KV, D) or v.shape != k.shape or out.shape != q.shape or not out.is_contiguous()):
             raise HachiueError(_lib.HCU_EINVAL, "hachiue: prefill_varlen takes q and a contiguous out [total_q, H, D] and "
                                                 "k / v [total_k, KV, D], all bf16 or all f16")
-        for t in (q, k, v):
-            if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != D):
-                raise HachiueError(_lib.HCU_EINVAL, "hachiue: prefill_varlen: heads must be contiguous")
-        for t in (cu_q, cu_k if cu_k is not None else cu_q):
-            if t.dtype != torch.int32 or t.dim() != 1 or t.shape != cu_q.shape or t.shape[0] < 1 or not t.is_contiguous():
+        strides = [self._row_stride(t, "prefill_varlen") for t in (q, k, v)]
+        if cu_k is not None:
+            self._on_device("prefill_varlen", cu_k)
+            if cu_k.dtype != torch.int32 or cu_k.shape != cu_q.shape or not cu_k.is_contiguous():
                 raise HachiueError(_lib.HCU_EINVAL, "hachiue: prefill_varlen takes contiguous int32 offsets [B + 1]")
+        if cu_q.dtype != torch.int32 or cu_q.dim() != 1 or cu_q.shape[0] < 1 or not cu_q.is_contiguous():
+            raise HachiueError(_lib.HCU_EINVAL, "hachiue: prefill_varlen takes contiguous int32 offsets [B + 1]")
         if nq == 0 or cu_q.shape[0] == 1:
             return
         self._bind_stream()
         p = self._varlen_params  # every field is set
-        p.batch, p.H, p.KV, p.D, p.window, p.dtype = cu_q.shape[0] - 1, H, KV, D, window, _DT[q.dtype]
+        p.batch, p.H, p.KV, p.D, p.window, p.dtype = cu_q.shape[0] - 1, H, KV, D, window, _DT[dtype]
         p.total_q, p.total_k, p.cu_q, p.cu_k = nq, nk, cu_q.data_ptr(), _ptr(cu_k)
-        p.q_row_stride, p.k_row_stride, p.v_row_stride = self._row_stride(q), self._row_stride(k), self._row_stride(v)
+        p.q_row_stride, p.k_row_stride, p.v_row_stride = strides
         check(self.lib.hcu_prefill_varlen(self._h, ctypes.byref(p), q.data_ptr(), k.data_ptr(), v.data_ptr(),
                                           out.data_ptr()))

@@ -32,16 +32,18 @@ struct AppendArgs {
   uint32_t* status;
 };
 
-// floor(x / d + 8.5) held within 0..15, exactly, without a division: the f32
-// estimate is off by at most one level next to a border, and the borders
-// (c - 8.5) * d and (c - 7.5) * d of a level are products of an 11-bit and a
-// 5-bit number, exact in f32, so two compares put it right.  y is x times the
-// sign of d, a is |d| (an f16 value above 0), inv about 1 / a.
+// floor(x / d + 8.5) held within 0..15, exactly, without a division: adding
+// 1.5 * 2^23 + 8 rounds y * inv + 8 to the nearest integer, which is off by at
+// most one level next to a border, and the borders (c - 8.5) * d and
+// (c - 7.5) * d of a level are products of an 11-bit and a 5-bit number, exact
+// in f32, so two compares put it right.  y is x times the sign of d, a is |d|
+// (an f16 value above 0), inv about 1 / a.
 __device__ __forceinline__ uint32_t q4_code(float y, float a, float inv) {
-  float c = floorf(fminf(fmaxf(fmaf(y, inv, 8.5f), 0.f), 15.f));
-  if ((c - 8.5f) * a > y) c -= 1.f;
-  if ((c - 7.5f) * a <= y) c += 1.f;
-  return (uint32_t)(int)fminf(fmaxf(c, 0.f), 15.f);
+  float c = fminf(fmaxf(fmaf(y, inv, 12582920.f) - 12582912.f, 0.f), 15.f);
+  const float lower = fmaf(c, a, -8.5f * a);
+  if (lower > y) c -= 1.f;
+  if (lower + a <= y) c += 1.f;
+  return __float_as_uint(fminf(fmaxf(c, 0.f), 15.f) + 8388608.f) & 15u;
 }
 
 // Quantises the eight elements of each lane: a block is four lanes.  Returns the
@@ -75,9 +77,9 @@ __device__ __forceinline__ uint32_t q4_block(const float (&x)[8], int lane, __ha
 }
 
 template <typename T, int DH>
-__global__ void __launch_bounds__(256) rope_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(256, 5) rope_append_kernel(const AppendArgs a) {
   constexpr int LPR = DH / 8, RPB = 256 / LPR, NB = DH / 32;  // lanes per row, rows per pass of the block
-  const int lane = threadIdx.x & 31, l = threadIdx.x % LPR, heads = a.H + 2 * a.kv.KV, i = blockIdx.x;
+  const int lane = threadIdx.x & 31, l = threadIdx.x % LPR, i = blockIdx.x;
   const long long slot = a.slots[i];
   if (slot < 0) return;
   const int pos = a.half ? a.positions[i] : 0;
@@ -86,12 +88,14 @@ __global__ void __launch_bounds__(256) rope_append_kernel(const AppendArgs a) {
     return;
   }
   // The lane's elements 8l .. 8l + 7 in two groups of four, which may lie on different sides of the pairs' halves.
-  float cs[2][4] = {}, sn[2][4] = {};  // sn: negative for the lower half of the pairs
+  float cs[2][4], sn[2][4];  // sn: negative for the lower half of the pairs
   int partner[2];
 #pragma unroll
   for (int u = 0; u < 2; u++) {
     const int e = 8 * l + 4 * u;
     partner[u] = -1;
+#pragma unroll
+    for (int c = 0; c < 4; c++) cs[u][c] = 1.f, sn[u][c] = 0.f;
     if (e < 2 * a.half) {
       const bool low = e < a.half;
       const int at = low ? e : e - a.half;
@@ -103,52 +107,73 @@ __global__ void __launch_bounds__(256) rope_append_kernel(const AppendArgs a) {
       partner[u] = low ? e + a.half : e - a.half;
     }
   }
-  const long long at0 = paged_row(a.kv, slot >> a.kv.page_log2, 0, (int)(slot & ((1 << a.kv.page_log2) - 1)));
-  for (int base = blockIdx.y * RPB; base < heads; base += gridDim.y * RPB) {
-    const int r = base + threadIdx.x / LPR;
-    const bool row = r < heads;
-    const int kind = r < a.H ? 0 : (r < a.H + a.kv.KV ? 1 : 2);  // q, k, v
-    const int g = kind == 0 ? r : (kind == 1 ? r - a.H : r - a.H - a.kv.KV);
-    const T* src = kind == 0   ? static_cast<const T*>(a.q) + i * a.q_stride
-                   : kind == 1 ? static_cast<const T*>(a.k) + i * a.k_stride
-                               : static_cast<const T*>(a.v) + i * a.v_stride;
-    src += (long long)g * DH;
-    float x[8] = {}, w[2][4] = {};
-    if (row) {
-      load8(src + 8 * l, x);
-      if (kind < 2)
+  // Reads a row's eight elements and their partners (from memory again: the row is in L1).
+  auto read = [&](const T* src, float (&x)[8], float (&w)[8]) {
+    load8(src + 8 * l, x);
+    if (a.half % 8 == 0) {
+      if (partner[0] >= 0) load8(src + partner[0], w);
+    } else {
 #pragma unroll
-        for (int u = 0; u < 2; u++)  // the partner elements come from memory again (the row is in L1)
-          if (partner[u] >= 0) load4(src + partner[u], w[u]);
+      for (int u = 0; u < 2; u++) {
+        float y[4] = {};
+        if (partner[u] >= 0) load4(src + partner[u], y);
+#pragma unroll
+        for (int c = 0; c < 4; c++) w[4 * u + c] = y[c];
+      }
     }
+  };
+  const int sub = threadIdx.x / LPR, first = blockIdx.y * RPB, step = gridDim.y * RPB;  // warp-uniform loops
+  // ---- queries ----
+  const T* q = static_cast<const T*>(a.q) + i * a.q_stride;
+  T* q_out = static_cast<T*>(a.q_out) + (long long)i * a.H * DH + 8 * l;
+#pragma unroll 2
+  for (int base = first; base < a.H; base += step) {
+    const int h = base + sub;
+    float x[8], w[8] = {};
+    if (h < a.H) read(q + h * DH, x, w);
     __syncwarp();  // in place: a row has been read before any lane writes
-    if (row && kind < 2) {
+    if (h < a.H) {
 #pragma unroll
-      for (int u = 0; u < 2; u++)
-        if (partner[u] >= 0)
-#pragma unroll
-          for (int c = 0; c < 4; c++) {
-            if (kind == 0)
-              x[4 * u + c] = fmaf(x[4 * u + c], cs[u][c], w[u][c] * sn[u][c]);
-            else  // the products of two f32 values are exact in f64
-              x[4 * u + c] = (float)__dadd_rn(__dmul_rn(x[4 * u + c], cs[u][c]), __dmul_rn(w[u][c], sn[u][c]));
-          }
-      T* dst = kind == 0 ? static_cast<T*>(a.q_out) : static_cast<T*>(a.k_out);
-      if (dst) store8(dst + ((long long)i * (kind == 0 ? a.H : a.kv.KV) + g) * DH + 8 * l, x);
+      for (int c = 0; c < 8; c++)
+        if (partner[c >> 2] >= 0) x[c] = fmaf(x[c], cs[c >> 2][c & 3], w[c] * sn[c >> 2][c & 3]);
+      store8(q_out + h * DH, x);
     }
-    if (!__any_sync(0xffffffffu, row && kind > 0)) continue;
+  }
+  // ---- keys and values: the passes go on where the queries' ended, so that a block per pass (few tokens) shares them ----
+  const long long at0 = paged_row(a.kv, slot >> a.kv.page_log2, 0, (int)(slot & ((1 << a.kv.page_log2) - 1)));
+  const T* k = static_cast<const T*>(a.k) + i * a.k_stride;
+  const T* v = static_cast<const T*>(a.v) + i * a.v_stride;
+  const int q_passes = (a.H + RPB - 1) / RPB, begin = (blockIdx.y + gridDim.y - q_passes % gridDim.y) % gridDim.y;
+  const int b = l >> 2, t = l & 3;  // block, quarter of it
+#pragma unroll 1
+  for (int base = begin * RPB; base < 2 * a.kv.KV; base += step) {
+    const int r = base + sub;
+    const bool row = r < 2 * a.kv.KV, key = r < a.kv.KV;
+    const int g = key ? r : r - a.kv.KV;
+    float x[8] = {}, w[8] = {};
+    if (row && key) read(k + g * DH, x, w);
+    if (row && !key) load8(v + g * DH + 8 * l, x);
+    __syncwarp();
+    if (__any_sync(0xffffffffu, row && key)) {  // a branch of the warp's: it would pay for f64 instructions that its lanes skip
+      if (row && key) {
+#pragma unroll
+        for (int c = 0; c < 8; c++)  // the products of two f32 values are exact in f64
+          if (partner[c >> 2] >= 0)
+            x[c] = (float)__dadd_rn(__dmul_rn(x[c], cs[c >> 2][c & 3]), __dmul_rn(w[c], sn[c >> 2][c & 3]));
+        if (a.k_out) store8(static_cast<T*>(a.k_out) + ((long long)i * a.kv.KV + g) * DH + 8 * l, x);
+      }
+    }
     __half d;
     const uint32_t code = q4_block(x, lane, &d);
-    if (!row || kind == 0) continue;
+    if (!row) continue;
     const long long at = at0 + ((long long)g << a.kv.page_log2);
-    const int b = l >> 2, t = l & 3;  // block, quarter of it
-    if (kind == 1) {
+    if (key) {
       *reinterpret_cast<uint32_t*>(a.kv.k + at * (DH / 2) + (t * NB + b) * 4) = code;
       if (t == 0) a.kv.ks[at * NB + b] = d;
     } else {
-      uint8_t* v = a.kv.v + at * (DH / 2);
-      *reinterpret_cast<uint16_t*>(v + (2 * t * NB + b) * 2) = (uint16_t)code;
-      *reinterpret_cast<uint16_t*>(v + ((2 * t + 1) * NB + b) * 2) = (uint16_t)(code >> 16);
+      uint8_t* dst = a.kv.v + at * (DH / 2);
+      *reinterpret_cast<uint16_t*>(dst + (2 * t * NB + b) * 2) = (uint16_t)code;
+      *reinterpret_cast<uint16_t*>(dst + ((2 * t + 1) * NB + b) * 2) = (uint16_t)(code >> 16);
       if (t == 0) a.kv.vs[at * NB + b] = d;
     }
   }
@@ -239,7 +264,7 @@ int with_dtype(const char* op, uint32_t dtype, F&& f) {
 template <typename T>
 int launch_append(hcu_context* h, const AppendArgs& a, int dh) {
   // Few tokens: a block per pass of rows.  Many: one per token, which walks its rows.
-  const int passes = (a.H + 2 * a.kv.KV + 256 / (dh / 8) - 1) / (256 / (dh / 8));
+  const int rpb = 256 / (dh / 8), passes = (a.H + rpb - 1) / rpb + (2 * a.kv.KV + rpb - 1) / rpb;
   const dim3 grid((unsigned)a.n, a.n < 4 * h->sm_count ? (unsigned)std::min(passes, 65535) : 1u);
   if (dh == 128) rope_append_kernel<T, 128><<<grid, 256, 0, h->stream>>>(a);
   else rope_append_kernel<T, 256><<<grid, 256, 0, h->stream>>>(a);
