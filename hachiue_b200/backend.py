@@ -134,9 +134,10 @@ class PagedKVCache:
         changed (a decode step calls this once per layer)."""
         cached = self.__dict__.get("_c_struct")
         k, v, ks, vs = self.k, self.v, self.k_scale, self.v_scale
-        # the tensors themselves are compared, and their places in memory, which can change under a tensor
+        # the tensors themselves are compared, and their places and shapes, which can change under a tensor
         if (cached is None or cached[0] is not k or cached[1] is not v or cached[2] is not ks or cached[3] is not vs
-                or cached[4] != (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr())):
+                or cached[4] != (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr())
+                or cached[5] != (k.shape, v.shape, ks.shape, vs.shape)):
             key = (k, v, ks, vs)
             shape, scales = tuple(self.k.shape), (*self.k.shape[:3], self.k.shape[3] // 16)
             if (len(shape) != 4 or self.v.shape != self.k.shape or any(tuple(t.shape) != scales for t in key[2:])
@@ -146,9 +147,9 @@ class PagedKVCache:
                                    "hachiue: a paged cache is contiguous uint8 k / v [n_pages, KV, page_size, Dh / 2] and "
                                    "f16 scales [n_pages, KV, page_size, Dh / 32] on one device")
             st = hcu_paged_kv(KV_Q4_0, shape[2], shape[0], shape[1], 2 * shape[3], *(_ptr(t) for t in key))
-            cached = (*key, tuple(t.data_ptr() for t in key), st)
+            cached = (*key, tuple(t.data_ptr() for t in key), tuple(t.shape for t in key), st)
             self.__dict__["_c_struct"] = cached
-        return cached[5]
+        return cached[6]
 
 
 class CudaBackend:
@@ -488,6 +489,8 @@ class CudaBackend:
         (negative: padding, skipped).  q_out and k_out (optional) receive the
         rotated rows; without cos / sin nothing is rotated."""
         kv = cache.c_struct()
+        if k.dim() != 3 or (q is not None and q.dim() != 3):
+            raise HachiueError(_lib.HCU_EINVAL, "hachiue: rope_append_paged takes k / v [n, KV, Dh] and q [n, H, Dh]")
         n, KV, Dh = k.shape
         H = 0 if q is None else q.shape[1]
         self._on_device("rope_append_paged", cache.k, k, v, slots)
@@ -539,13 +542,15 @@ class CudaBackend:
         (n, heads, D), (row, head, one) = t.shape, t.stride()
         if one != 1 or (head != D and heads > 1):
             raise HachiueError(_lib.HCU_EINVAL, f"hachiue: {op}: heads must be contiguous")
+        if n > 1 and row < heads * D:  # an expanded row, whose stride 0 would read as dense
+            raise HachiueError(_lib.HCU_EINVAL, f"hachiue: {op}: token rows must not overlap")
         return row if n > 1 else 0
 
     def read_paged(self, cache: PagedKVCache, slots: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor) -> None:
         """The values of cached rows: k_out, v_out [n, KV, Dh] (f32, f16 or
         bf16, contiguous) receive rows slots[i] (int64 [n]; negative: left as it was)."""
         kv = cache.c_struct()
-        n = slots.shape[0]
+        n = slots.numel()
         self._on_device("read_paged", cache.k, slots, k_out, v_out)
         if (slots.dtype != torch.int64 or slots.dim() != 1 or not slots.is_contiguous() or k_out.shape != (n, kv.KV, kv.Dh)
                 or v_out.shape != k_out.shape or k_out.dtype not in _DT or v_out.dtype != k_out.dtype
@@ -595,6 +600,8 @@ class CudaBackend:
         [B + 1] offsets of the sequences (cu_k None: the same).  With more
         keys than queries the queries are the last tokens; window 0 = causal."""
         self._on_device("prefill_varlen", q, k, v, out, cu_q)
+        if q.dim() != 3 or k.dim() != 3:
+            raise HachiueError(_lib.HCU_EINVAL, "hachiue: prefill_varlen takes q [total_q, H, D] and k / v [total_k, KV, D]")
         nq, H, D = q.shape
         nk, KV = k.shape[:2]
         dtype = q.dtype

@@ -894,7 +894,7 @@ extern "C" int hcu_attention_paged(hcu_handle h, const hcu_attention_paged_param
   if ((uint64_t)p->S * (p->H / kv->KV) > 65535u) return fail(HCU_EINVAL, "%s: S * H / KV > 65535", op);
   if (p->max_context > 0x7fffff00u || p->windowSize > 0x7fffffffu)
     return fail(HCU_EINVAL, "%s: max_context or windowSize too large", op);
-  if (!q || !out || !p->block_table || !p->context) return fail(HCU_EINVAL, "%s: null argument", op);
+  if (!q || !out || (!p->block_table && p->max_context) || !p->context) return fail(HCU_EINVAL, "%s: null argument", op);
   if ((uint64_t)p->table_stride * kv->page_size < p->max_context)
     return fail(HCU_EINVAL, "%s: table_stride (%u) pages of %u tokens cannot hold max_context (%u)", op, p->table_stride,
                 kv->page_size, p->max_context);
