@@ -134,10 +134,10 @@ class PagedKVCache:
         changed (a decode step calls this once per layer)."""
         cached = self.__dict__.get("_c_struct")
         k, v, ks, vs = self.k, self.v, self.k_scale, self.v_scale
-        # the tensors themselves are compared, and their places and shapes, which can change under a tensor
+        # the tensors themselves are compared, and their places and sizes, which can change under a tensor
         if (cached is None or cached[0] is not k or cached[1] is not v or cached[2] is not ks or cached[3] is not vs
                 or cached[4] != (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr())
-                or cached[5] != (k.shape, v.shape, ks.shape, vs.shape)):
+                or cached[5] != k.shape or cached[6] != (v.numel(), ks.numel(), vs.numel())):
             key = (k, v, ks, vs)
             shape, scales = tuple(self.k.shape), (*self.k.shape[:3], self.k.shape[3] // 16)
             if (len(shape) != 4 or self.v.shape != self.k.shape or any(tuple(t.shape) != scales for t in key[2:])
@@ -147,9 +147,9 @@ class PagedKVCache:
                                    "hachiue: a paged cache is contiguous uint8 k / v [n_pages, KV, page_size, Dh / 2] and "
                                    "f16 scales [n_pages, KV, page_size, Dh / 32] on one device")
             st = hcu_paged_kv(KV_Q4_0, shape[2], shape[0], shape[1], 2 * shape[3], *(_ptr(t) for t in key))
-            cached = (*key, tuple(t.data_ptr() for t in key), tuple(t.shape for t in key), st)
+            cached = (*key, tuple(t.data_ptr() for t in key), k.shape, tuple(t.numel() for t in key[1:]), st)
             self.__dict__["_c_struct"] = cached
-        return cached[6]
+        return cached[7]
 
 
 class CudaBackend:
@@ -488,63 +488,69 @@ class CudaBackend:
         [positions, rotary_dim / 2], positions int32 [n], slots int64 [n]
         (negative: padding, skipped).  q_out and k_out (optional) receive the
         rotated rows; without cos / sin nothing is rotated."""
+        op = "rope_append_paged"
         kv = cache.c_struct()
-        if k.dim() != 3 or (q is not None and q.dim() != 3):
-            raise HachiueError(_lib.HCU_EINVAL, "hachiue: rope_append_paged takes k / v [n, KV, Dh] and q [n, H, Dh]")
-        n, KV, Dh = k.shape
-        H = 0 if q is None else q.shape[1]
-        self._on_device("rope_append_paged", cache.k, k, v, slots)
-        if (v.shape != k.shape or KV != kv.KV or Dh != kv.Dh or k.dtype not in _DT or v.dtype != k.dtype
+        shape, dtype = k.shape, k.dtype
+        if len(shape) != 3:
+            raise HachiueError(_lib.HCU_EINVAL, f"hachiue: {op} takes k / v [n, KV, Dh]")
+        n, KV, Dh = shape
+        self._on_device(op, cache.k, k, v, slots)
+        if (KV != kv.KV or Dh != kv.Dh or v.shape != shape or dtype not in _DT or v.dtype != dtype
                 or slots.dtype != torch.int64 or slots.shape != (n,) or not slots.is_contiguous()):
-            raise HachiueError(_lib.HCU_EINVAL, f"hachiue: rope_append_paged takes k / v [n, {kv.KV}, {kv.Dh}] of one float dtype "
-                                                "and contiguous int64 slots [n]")
-        rotary = 0
+            raise HachiueError(_lib.HCU_EINVAL, f"hachiue: {op} takes k / v [n, {kv.KV}, {kv.Dh}] of one float dtype and "
+                                                "contiguous int64 slots [n]")
+        table_rows = half = 0
         if cos is not None:
-            rotary = 2 * cos.shape[-1]
             if sin is None or positions is None:
-                raise HachiueError(_lib.HCU_EINVAL, "hachiue: rope_append_paged: a rotation needs cos, sin and positions")
-            self._on_device("rope_append_paged", cos, sin, positions)
-            if (cos.dim() != 2 or sin.shape != cos.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32
+                raise HachiueError(_lib.HCU_EINVAL, f"hachiue: {op}: a rotation needs cos, sin and positions")
+            self._on_device(op, cos, sin, positions)
+            table = cos.shape
+            if (len(table) != 2 or sin.shape != table or cos.dtype != torch.float32 or sin.dtype != torch.float32
                     or not cos.is_contiguous() or not sin.is_contiguous() or positions.dtype != torch.int32
                     or positions.shape != (n,) or not positions.is_contiguous()):
-                raise HachiueError(_lib.HCU_EINVAL, "hachiue: rope_append_paged takes contiguous f32 cos / sin "
+                raise HachiueError(_lib.HCU_EINVAL, f"hachiue: {op} takes contiguous f32 cos / sin "
                                                     "[positions, rotary_dim / 2] and int32 positions [n]")
+            table_rows, half = table
         elif sin is not None:
-            raise HachiueError(_lib.HCU_EINVAL, "hachiue: rope_append_paged: sin without cos")
-        if (q is None) != (q_out is None):
-            raise HachiueError(_lib.HCU_EINVAL, "hachiue: rope_append_paged: q and q_out go together")
-        strides = self._row_stride(k, "rope_append_paged"), self._row_stride(v, "rope_append_paged")
-        q_stride = 0
-        if q is not None:
-            self._on_device("rope_append_paged", q, q_out)
-            if (q.shape != (n, H, Dh) or q.dtype != k.dtype or q_out.shape != q.shape or q_out.dtype != k.dtype
-                    or not q_out.is_contiguous()):
-                raise HachiueError(_lib.HCU_EINVAL, "hachiue: rope_append_paged takes q and a contiguous q_out [n, H, Dh] "
-                                                    "of k's dtype")
-            q_stride = self._row_stride(q, "rope_append_paged")
+            raise HachiueError(_lib.HCU_EINVAL, f"hachiue: {op}: sin without cos")
+        H = q_stride = 0
+        if q is not None and q_out is not None:
+            self._on_device(op, q, q_out)
+            q_shape = q.shape
+            if (len(q_shape) != 3 or q_shape[0] != n or q_shape[2] != Dh or q.dtype != dtype or q_out.shape != q_shape
+                    or q_out.dtype != dtype or not q_out.is_contiguous()):
+                raise HachiueError(_lib.HCU_EINVAL, f"hachiue: {op} takes q and a contiguous q_out [n, H, Dh] of k's dtype")
+            H = q_shape[1]
+            q_stride = self._row_stride(op, q_shape, q.stride())
+        elif q is not q_out:
+            raise HachiueError(_lib.HCU_EINVAL, f"hachiue: {op}: q and q_out go together")
         if k_out is not None:
-            self._on_device("rope_append_paged", k_out)
-            if k_out.shape != k.shape or k_out.dtype != k.dtype or not k_out.is_contiguous():
-                raise HachiueError(_lib.HCU_EINVAL, "hachiue: rope_append_paged takes a contiguous k_out like k")
+            self._on_device(op, k_out)
+            if k_out.shape != shape or k_out.dtype != dtype or not k_out.is_contiguous():
+                raise HachiueError(_lib.HCU_EINVAL, f"hachiue: {op} takes a contiguous k_out like k")
+        k_stride, v_stride = self._row_stride(op, shape, k.stride()), self._row_stride(op, shape, v.stride())
         if n == 0:
             return
         self._bind_stream()
         p = self._append_params  # every field is set
-        p.n, p.H, p.dtype, p.rotaryDim, p.table_rows = n, H, _DT[k.dtype], rotary, 0 if cos is None else cos.shape[0]
-        p.q_row_stride, p.k_row_stride, p.v_row_stride = q_stride, *strides
+        p.n, p.H, p.dtype, p.rotaryDim, p.table_rows = n, H, _DT[dtype], 2 * half, table_rows
+        p.q_row_stride, p.k_row_stride, p.v_row_stride = q_stride, k_stride, v_stride
         check(self.lib.hcu_rope_append_paged(self._h, ctypes.byref(p), _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(cos),
                                              _ptr(sin), _ptr(positions), slots.data_ptr(), _ptr(q_out), _ptr(k_out),
                                              ctypes.byref(kv)))
 
     @staticmethod
-    def _row_stride(t: torch.Tensor, op: str) -> int:
-        """Elements between the token rows of t [n, heads, D], whose heads are contiguous (0, dense, for a single row)."""
-        (n, heads, D), (row, head, one) = t.shape, t.stride()
+    def _row_stride(op: str, shape: tuple, stride: tuple) -> int:
+        """Elements between the token rows of [n, heads, D], whose heads are contiguous (0, dense, for a single row)."""
+        n, heads, D = shape
+        row, head, one = stride
         if one != 1 or (head != D and heads > 1):
             raise HachiueError(_lib.HCU_EINVAL, f"hachiue: {op}: heads must be contiguous")
-        if n > 1 and row < heads * D:  # an expanded row, whose stride 0 would read as dense
+        if n <= 1:
+            return 0
+        if row < heads * D:  # an expanded row, whose stride 0 would read as dense
             raise HachiueError(_lib.HCU_EINVAL, f"hachiue: {op}: token rows must not overlap")
-        return row if n > 1 else 0
+        return row
 
     def read_paged(self, cache: PagedKVCache, slots: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor) -> None:
         """The values of cached rows: k_out, v_out [n, KV, Dh] (f32, f16 or
@@ -552,15 +558,16 @@ class CudaBackend:
         kv = cache.c_struct()
         n = slots.numel()
         self._on_device("read_paged", cache.k, slots, k_out, v_out)
-        if (slots.dtype != torch.int64 or slots.dim() != 1 or not slots.is_contiguous() or k_out.shape != (n, kv.KV, kv.Dh)
-                or v_out.shape != k_out.shape or k_out.dtype not in _DT or v_out.dtype != k_out.dtype
+        shape, dtype = (n, kv.KV, kv.Dh), k_out.dtype
+        if (slots.dtype != torch.int64 or slots.dim() != 1 or not slots.is_contiguous() or k_out.shape != shape
+                or v_out.shape != shape or dtype not in _DT or v_out.dtype != dtype
                 or not k_out.is_contiguous() or not v_out.is_contiguous()):
             raise HachiueError(_lib.HCU_EINVAL, f"hachiue: read_paged takes contiguous int64 slots [n] and contiguous outputs "
                                                 f"[n, {kv.KV}, {kv.Dh}] of one float dtype")
         if n == 0:
             return
         self._bind_stream()
-        check(self.lib.hcu_read_paged(self._h, n, _DT[k_out.dtype], slots.data_ptr(), ctypes.byref(kv), k_out.data_ptr(),
+        check(self.lib.hcu_read_paged(self._h, n, _DT[dtype], slots.data_ptr(), ctypes.byref(kv), k_out.data_ptr(),
                                       v_out.data_ptr()))
 
     def attention_paged(self, q: torch.Tensor, cache: PagedKVCache, out: torch.Tensor, block_table: torch.Tensor,
@@ -572,22 +579,22 @@ class CudaBackend:
         the split of the key axis fit the call)."""
         kv = cache.c_struct()
         self._on_device("attention_paged", cache.k, q, out, block_table, context)
-        if (q.dim() != 4 or q.shape[3] != kv.Dh or q.dtype not in _DT or out.shape != q.shape or out.dtype != q.dtype
+        shape, dtype, table = q.shape, q.dtype, block_table.shape
+        if (len(shape) != 4 or shape[3] != kv.Dh or dtype not in _DT or out.shape != shape or out.dtype != dtype
                 or not q.is_contiguous() or not out.is_contiguous()):
             raise HachiueError(_lib.HCU_EINVAL, f"hachiue: attention_paged takes contiguous q and out [B, S, H, {kv.Dh}] of one "
                                                 "float dtype")
-        B, S, H = q.shape[:3]
-        if (block_table.dtype != torch.int32 or context.dtype != torch.int32 or block_table.dim() != 2
-                or block_table.shape[0] != B or context.shape != (B,) or not block_table.is_contiguous()
-                or not context.is_contiguous()):
+        B, S, H, _ = shape
+        if (block_table.dtype != torch.int32 or context.dtype != torch.int32 or len(table) != 2 or table[0] != B
+                or context.shape != (B,) or not block_table.is_contiguous() or not context.is_contiguous()):
             raise HachiueError(_lib.HCU_EINVAL, "hachiue: attention_paged takes contiguous int32 block_table [B, pages] and "
                                                 "context [B]")
         if B == 0 or S == 0:
             return
-        pages = block_table.shape[1]
+        pages = table[1]
         self._bind_stream()
         p = self._paged_params  # every field is set
-        p.batch, p.S, p.H, p.windowSize, p.dtype = B, S, H, window_size, _DT[q.dtype]
+        p.batch, p.S, p.H, p.windowSize, p.dtype = B, S, H, window_size, _DT[dtype]
         p.max_context, p.table_stride = max_context or pages * kv.page_size, pages
         p.block_table, p.context = block_table.data_ptr(), context.data_ptr()
         check(self.lib.hcu_attention_paged(self._h, ctypes.byref(p), q.data_ptr(), ctypes.byref(kv), out.data_ptr()))
@@ -599,17 +606,18 @@ class CudaBackend:
         are accepted), out [total_q, H, 128] contiguous; cu_q, cu_k int32
         [B + 1] offsets of the sequences (cu_k None: the same).  With more
         keys than queries the queries are the last tokens; window 0 = causal."""
-        self._on_device("prefill_varlen", q, k, v, out, cu_q)
-        if q.dim() != 3 or k.dim() != 3:
-            raise HachiueError(_lib.HCU_EINVAL, "hachiue: prefill_varlen takes q [total_q, H, D] and k / v [total_k, KV, D]")
-        nq, H, D = q.shape
-        nk, KV = k.shape[:2]
-        dtype = q.dtype
-        if (dtype not in (torch.bfloat16, torch.float16) or k.dtype != dtype or v.dtype != dtype or out.dtype != dtype
-                or k.shape != (nk, KV, D) or v.shape != k.shape or out.shape != q.shape or not out.is_contiguous()):
-            raise HachiueError(_lib.HCU_EINVAL, "hachiue: prefill_varlen takes q and a contiguous out [total_q, H, D] and "
+        op = "prefill_varlen"
+        self._on_device(op, q, k, v, out, cu_q)
+        shape, k_shape, dtype = q.shape, k.shape, q.dtype
+        if (len(shape) != 3 or len(k_shape) != 3 or dtype not in (torch.bfloat16, torch.float16) or k.dtype != dtype
+                or v.dtype != dtype or out.dtype != dtype or k_shape[2] != shape[2] or v.shape != k_shape or out.shape != shape
+                or not out.is_contiguous()):
+            raise HachiueError(_lib.HCU_EINVAL, f"hachiue: {op} takes q and a contiguous out [total_q, H, D] and "
                                                 "k / v [total_k, KV, D], all bf16 or all f16")
-        strides = [self._row_stride(t, "prefill_varlen") for t in (q, k, v)]
+        nq, H, D = shape
+        nk, KV, _ = k_shape
+        strides = (self._row_stride(op, shape, q.stride()), self._row_stride(op, k_shape, k.stride()),
+                   self._row_stride(op, k_shape, v.stride()))
         if cu_k is not None:
             self._on_device("prefill_varlen", cu_k)
             if cu_k.dtype != torch.int32 or cu_k.shape != cu_q.shape or not cu_k.is_contiguous():
