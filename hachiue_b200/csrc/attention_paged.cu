@@ -143,7 +143,7 @@ constexpr int paged_row_floats(int dh) { return dh + 4; }  // of the warps' sums
 constexpr size_t paged_smem(int dh, int rb) {
   return (size_t)NW * STAGES * paged_stage_bytes(dh) + (size_t)NW * rb * paged_row_floats(dh) * 4;
 }
-constexpr int paged_ctas(int dh, int nc) { return dh == 128 && nc == 1 ? 2 : 1; }  // per SM
+constexpr int paged_ctas(int dh, int nc, int mt) { return dh == 128 && nc == 1 && mt == 1 ? 2 : 1; }  // per SM
 
 // The work of a call is a line of chunks: sequence after sequence, in each
 // its KV heads, in each its row blocks, in each the chunks that hold visible tokens
@@ -173,20 +173,27 @@ __device__ __forceinline__ int2 paged_chunks(const PagedAttnArgs& a, int b) {
   return make_int2(c_lo, max(1, c_hi - c_lo));
 }
 
-// TERMS f16 numbers per query, NC groups of eight columns: RB = 8 NC / TERMS
-// rows per warp.  EXACT: code - 8 for both operands (f32 results); otherwise
-// the codes as they are, the offset taken off the sums, whose larger terms
-// the tensor cores' f32 sums truncate (about 3e-6 of the result, measured).
-template <int DH, int TERMS, int NC, bool EXACT>
-__global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel(const PagedAttnArgs a) {
+// A query (a weighted probability) is CT f16 numbers in as many columns, or MT
+// in a column of MT products each; NC groups of eight columns make RB = 8 NC /
+// CT rows per warp.  EXACT: code - 8 for both operands (f32 results), and the
+// sums of 16 tokens are added in f32 outside of the tensor cores, whose own
+// additions truncate: over 8192 tokens that came to 7e-6 of the result.
+// Otherwise the codes as they are, the offset taken off the sums.
+template <int DH, int CT, int MT, int NC, bool EXACT>
+__global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC, MT)) attn_paged_kernel(const PagedAttnArgs a) {
   constexpr int NB = DH / 32, ST = STAGES, SB = paged_stage_bytes(DH);
-  constexpr int RG = 8 / TERMS, RB = RG * NC;  // rows per column group, per warp
-  constexpr int NR = 2 / TERMS;                // rows per thread and column group
+  constexpr int RG = 8 / CT, RB = RG * NC;      // rows per column group, per warp
+  constexpr int NR = 2 / CT;                   // rows per thread and column group
+  static_assert(CT * MT == 1 || (CT * MT == 2 && (MT == 1 || EXACT)), "one f16 number or two");
+  constexpr bool WIDE = CT * MT == 2;          // two f16 numbers: queries may be f32
   constexpr int KB = CHUNK * DH / 2, CB = CHUNK * NB * 2;  // bytes of a stage's codes, of its scales
+  // Steps of 16 tokens in the loop's body: with two of these the code outgrows the instruction cache (bf16, four tokens
+  // of 32 / 8 heads over 16 x 4000 tokens: 58 us unrolled, 54 rolled; one token of 32 / 8 over 64 sequences: 85 and 89).
+  constexpr int kSteps = DH == 256 || NC == 2 ? 1 : 2;
   constexpr int RS = paged_row_floats(DH);
   constexpr size_t REC = (size_t)RB * (DH + 2);  // floats of a global record
   static_assert(RB * RS * 4 <= ST * SB, "a record fits a ring");
-  static_assert(RB * DH * (TERMS == 2 ? 4 : 2) <= SB, "a segment's queries fit a stage");
+  static_assert(RB * DH * (WIDE ? 4 : 2) <= SB, "a segment's queries fit a stage");
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int scan[NW], s_b, s_pos;
   // Records of a warp's units that lie only partly in its piece: [2w] the one that ends there, [2w + 1] the one that
@@ -339,7 +346,7 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
       const int es = a.dtype == HCU_DT_F32 ? 4 : 2, ppr = DH * es / 16;  // 16-byte pieces of a row
       const int r0 = f.rb * RB;
 #pragma unroll
-      for (int i = 0; i < RB * DH * (TERMS == 2 ? 4 : 2) / 512; i++) {
+      for (int i = 0; i < RB * DH * (WIDE ? 4 : 2) / 512; i++) {
         const int p = 32 * i + lane, r = p / ppr, rr = r0 + r;
         const bool there = r < RB && rr < a.R;
         const int sq = there ? rr / a.G : 0, h = f.kvh * a.G + (there ? rr % a.G : 0);
@@ -349,33 +356,52 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
       f_c++;
       look_up(f_c, f_page);
     } else if (f_c < f.c1) {
-      long long row[2];
+      if (a.kv.page_log2 >= 5 && (uint32_t)f_page[0] < (uint32_t)a.kv.n_pages && f_page[1] != -2) {
+        // The whole chunk lies in one page: 32 rows in a piece.
+        halves = 3u;
+        const long long row = paged_row(a.kv, f_page[0], f.kvh, (f_c * CHUNK) & page_mask);
+        const uint8_t* k = a.kv.k + row * (DH / 2) + lane * 16;
+        const uint8_t* v = a.kv.v + row * (DH / 2) + lane * 16;
+        const uint32_t d = dst + lane * 16;
 #pragma unroll
-      for (int p = 0; p < 2; p++) {
-        const bool there = (uint32_t)f_page[p] < (uint32_t)a.kv.n_pages;
-        if (!there && f_page[p] != -2 && lane == 0) atomicOr(a.status, HCU_DEVERR_BADARG);  // the table's entry is no page
-        halves |= (there ? 1u : 0u) << p;
-        row[p] = paged_row(a.kv, there ? f_page[p] : 0, f.kvh, (f_c * CHUNK + 16 * p) & page_mask);
-      }
-      const bool there[2] = {(halves & 1u) != 0, (halves & 2u) != 0};
-#pragma unroll
-      for (int p = 0; p < 2; p++) {
-        const uint8_t* k = a.kv.k + row[p] * (DH / 2) + lane * 16;
-        const uint8_t* v = a.kv.v + row[p] * (DH / 2) + lane * 16;
-        const uint32_t d = dst + p * (KB / 2) + lane * 16;
-#pragma unroll
-        for (int i = 0; i < KB / 1024; i++) {
-          copy16(d + 512 * i, k + 512 * i, there[p]);
-          copy16(d + KB + 512 * i, v + 512 * i, there[p]);
+        for (int i = 0; i < KB / 512; i++) {
+          copy16(d + 512 * i, k + 512 * i);
+          copy16(d + KB + 512 * i, v + 512 * i);
         }
-      }
-      // scales: CB / 32 lanes per half, key scales then value scales
-      constexpr int LH = CB / 32;
 #pragma unroll
-      for (int i = 0; i < 4 * LH; i += 32) {
-        const int l = i + lane, p = (l / LH) & 1;
-        const __half* src = (l / (2 * LH) ? a.kv.vs : a.kv.ks) + (p ? row[1] : row[0]) * NB + (l % LH) * 8;
-        copy16(dst + 2 * KB + l * 16, src, p ? there[1] : there[0]);
+        for (int i = 0; i < 2 * CB / 16; i += 32) {
+          const int l = i + lane;
+          copy16(dst + 2 * KB + l * 16, (l < CB / 16 ? a.kv.ks + l * 8 : a.kv.vs + (l - CB / 16) * 8) + row * NB);
+        }
+      } else {
+        long long row[2];
+#pragma unroll
+        for (int p = 0; p < 2; p++) {
+          const bool there = (uint32_t)f_page[p] < (uint32_t)a.kv.n_pages;
+          if (!there && f_page[p] != -2 && lane == 0) atomicOr(a.status, HCU_DEVERR_BADARG);  // the table's entry is no page
+          halves |= (there ? 1u : 0u) << p;
+          row[p] = paged_row(a.kv, there ? f_page[p] : 0, f.kvh, (f_c * CHUNK + 16 * p) & page_mask);
+        }
+        const bool there[2] = {(halves & 1u) != 0, (halves & 2u) != 0};
+#pragma unroll
+        for (int p = 0; p < 2; p++) {
+          const uint8_t* k = a.kv.k + row[p] * (DH / 2) + lane * 16;
+          const uint8_t* v = a.kv.v + row[p] * (DH / 2) + lane * 16;
+          const uint32_t d = dst + p * (KB / 2) + lane * 16;
+#pragma unroll
+          for (int i = 0; i < KB / 1024; i++) {
+            copy16(d + 512 * i, k + 512 * i, there[p]);
+            copy16(d + KB + 512 * i, v + 512 * i, there[p]);
+          }
+        }
+        // scales: CB / 32 lanes per half, key scales then value scales
+        constexpr int LH = CB / 32;
+#pragma unroll
+        for (int i = 0; i < 4 * LH; i += 32) {
+          const int l = i + lane, p = (l / LH) & 1;
+          const __half* src = (l / (2 * LH) ? a.kv.vs : a.kv.ks) + (p ? row[1] : row[0]) * NB + (l % LH) * 8;
+          copy16(dst + 2 * KB + l * 16, src, p ? there[1] : there[0]);
+        }
       }
       if (++f_c == f.c1 && f_pos < end) enter();
       look_up(f_c, f_page);
@@ -406,12 +432,12 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
     // ---- query columns: column g of group nc is row / term of this lane's B fragments ----
     copy_wait<ST - 1>();
     __syncwarp();
-    uint32_t qf[NC][NB][4];
+    uint32_t qf[NC][MT][NB][4];
     float corr[NC][NB][NR];  // -8 sum(q) of the block (not EXACT), rows of this thread's accumulator columns 2t, 2t + 1
     float rs[NC][NR];        // score = rs * accumulated sum
 #pragma unroll
     for (int nc = 0; nc < NC; nc++) {
-      const int r = nc * RG + (TERMS == 2 ? g >> 1 : g);
+      const int r = nc * RG + (CT == 2 ? g >> 1 : g);
       float q[NB][8], top = 0.f;  // rows past the last are zeros
       load_query<NB>(ring + stage * SB + r * (DH * (a.dtype == HCU_DT_F32 ? 4 : 2)), t, a.dtype, q);
 #pragma unroll
@@ -430,15 +456,18 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
 #pragma unroll
         for (int m = 0; m < 4; m++) {
           // register m: dimensions m and m + 4 of the lane's eight; odd m meets codes times 16
-          __half o[2];
+          __half o[2], low[2];
 #pragma unroll
           for (int c = 0; c < 2; c++) {
+            const float f = (m & 1) ? 0.0625f : 1.f;
             float v = q[i][m + 4 * c] * up;
-            if (TERMS == 2 && (g & 1)) v -= __half2float(__float2half_rn(v));
-            o[c] = __float2half_rn((m & 1) ? v * 0.0625f : v);
+            if (CT == 2 && (g & 1)) v -= __half2float(__float2half_rn(v));
+            o[c] = __float2half_rn(v * f);
+            if (MT == 2) low[c] = __float2half_rn((v - __half2float(__float2half_rn(v))) * f);
             if (!EXACT) sum += __half2float(o[c]) * ((m & 1) ? 16.f : 1.f);
           }
-          qf[nc][i][m] = h2_bits(__halves2half2(o[0], o[1]));
+          qf[nc][0][i][m] = h2_bits(__halves2half2(o[0], o[1]));
+          if (MT == 2) qf[nc][MT - 1][i][m] = h2_bits(__halves2half2(low[0], low[1]));
         }
         if (!EXACT) {
           sum += __shfl_xor_sync(0xffffffffu, sum, 1);
@@ -446,7 +475,7 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
           sum *= -8.f * 5.9604644775390625e-08f;  // -8 * 2^-24
           // column 2t is lane group g = 2t, column 2t + 1 the next
           const float u0 = __shfl_sync(0xffffffffu, sum, 8 * t), u1 = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
-          corr[nc][i][0] = TERMS == 2 ? u0 + u1 : u0;
+          corr[nc][i][0] = CT == 2 ? u0 + u1 : u0;
           if (NR == 2) corr[nc][i][NR - 1] = u1;
         }
       }
@@ -473,22 +502,22 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
       const uint32_t halves = (have >> (2 * stage)) & 3u;
       const int base = c * CHUNK;
       const bool whole = base >= lo_all && base + CHUNK <= hi_all && halves == 3u;
-      // ---- scores of 32 tokens ----
-      float x[2][2][NC][NR];         // [16-token step][accumulator row half][..]: score, log2 units
-      uint32_t vsw[2][2][NB / 2];    // value scales of the thread's tokens, f16 pairs
-#pragma unroll
+#pragma unroll kSteps
       for (int j = 0; j < 2; j++) {
+        // ---- scores of 16 tokens ----
+        float x[2][NC][NR];        // [accumulator row half][..]: score, log2 units
+        uint32_t vsw[2][NB / 2];   // value scales of the thread's tokens, f16 pairs
         uint32_t kw[2][NB], ksw[2][NB / 2];
 #pragma unroll
         for (int u = 0; u < 2; u++) {
           const uint32_t row = 16 * j + 8 * u + tok;
           lds_words<NB>(st + row * (DH / 2) + t * NB * 4, kw[u]);
           lds_words<NB / 2>(st + 2 * KB + row * NB * 2, ksw[u]);
-          lds_words<NB / 2>(st + 2 * KB + CB + row * NB * 2, vsw[j][u]);
+          lds_words<NB / 2>(st + 2 * KB + CB + row * NB * 2, vsw[u]);
 #pragma unroll
           for (int nc = 0; nc < NC; nc++)
 #pragma unroll
-            for (int r = 0; r < NR; r++) x[j][u][nc][r] = 0.f;
+            for (int r = 0; r < NR; r++) x[u][nc][r] = 0.f;
         }
 #pragma unroll
         for (int i = 0; i < NB; i++) {
@@ -509,16 +538,25 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
 #pragma unroll
           for (int nc = 0; nc < NC; nc++) {
             float d[4];
-            mma16816_zero(d, a0, qf[nc][i][0], qf[nc][i][1]);
-            mma16816(d, a1, qf[nc][i][2], qf[nc][i][3]);
+            mma16816_zero(d, a0, qf[nc][0][i][0], qf[nc][0][i][1]);
+            if (MT == 2) {
+              float e[4];
+              mma16816_zero(e, a0, qf[nc][MT - 1][i][0], qf[nc][MT - 1][i][1]);
+              mma16816(d, a1, qf[nc][0][i][2], qf[nc][0][i][3]);
+              mma16816(e, a1, qf[nc][MT - 1][i][2], qf[nc][MT - 1][i][3]);
+              f2_get(f2_add(f2(d[0], d[1]), f2(e[0], e[1])), d[0], d[1]);
+              f2_get(f2_add(f2(d[2], d[3]), f2(e[2], e[3])), d[2], d[3]);
+            } else {
+              mma16816(d, a1, qf[nc][0][i][2], qf[nc][0][i][3]);
+            }
 #pragma unroll
             for (int u = 0; u < 2; u++) {
 #pragma unroll
               for (int r = 0; r < NR; r++) {
                 float sum = d[2 * u + r];
                 if (!EXACT) sum += corr[nc][i][r];
-                if (TERMS == 2) sum += d[2 * u + 1];
-                x[j][u][nc][r] = fmaf(ks[u], sum, x[j][u][nc][r]);
+                if (CT == 2) sum += d[2 * u + 1];
+                x[u][nc][r] = fmaf(ks[u], sum, x[u][nc][r]);
               }
             }
           }
@@ -528,7 +566,7 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
 #pragma unroll
           for (int u = 0; u < 2; u++)
 #pragma unroll
-            for (int r = 0; r < NR; r++) x[j][u][nc][r] *= rs[nc][r];
+            for (int r = 0; r < NR; r++) x[u][nc][r] *= rs[nc][r];
         if (!whole) {
           // Tokens outside a row's range and on missing pages weigh nothing; what their rows hold is not looked at.
 #pragma unroll
@@ -542,115 +580,121 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
               for (int r = 0; r < NR; r++) {
                 const int rl = nc * RG + t * NR + r, p = ctx - a.S + (r0 + rl) / a.G;
                 const bool see = data && rl < rows && at <= p && (a.window == 0 || at > p - a.window);
-                x[j][u][nc][r] = see ? x[j][u][nc][r] : -INFINITY;
+                x[u][nc][r] = see ? x[u][nc][r] : -INFINITY;
                 any = any || see;
               }
             if (!any)
 #pragma unroll
-              for (int i = 0; i < NB / 2; i++) vsw[j][u][i] = 0u;
+              for (int i = 0; i < NB / 2; i++) vsw[u][i] = 0u;
           }
         }
-      }
-      // ---- reference points: they move when a weighted probability could pass 2^kTop ----
-      __half2 vtop = __habs2(bits_h2(vsw[0][0][0]));
+        // ---- reference points: they move when a weighted probability could pass 2^kTop ----
+        __half2 vtop = __habs2(bits_h2(vsw[0][0]));
 #pragma unroll
-      for (int i = 1; i < 2 * NB; i++)
-        vtop = __hmax2(vtop, __habs2(bits_h2(vsw[i / NB][(i / (NB / 2)) & 1][i % (NB / 2)])));
-      const float vmax = fmaxf(__low2float(vtop), __high2float(vtop));
-      bool grow = vmax > cap;
-#pragma unroll
-      for (int nc = 0; nc < NC; nc++)
-#pragma unroll
-        for (int r = 0; r < NR; r++)
-          grow = grow || fmaxf(fmaxf(x[0][0][nc][r], x[0][1][nc][r]), fmaxf(x[1][0][nc][r], x[1][1][nc][r])) > T[nc][r];
-      if (__any_sync(0xffffffffu, grow)) {
-        const float top = warp_max(vmax);
-        if (top > cap) {  // the next power of two
-          cap_log2 = (float)((int)(__float_as_uint(top) >> 23) - 126);
-          cap = exp2f(cap_log2);
-        }
-#pragma unroll
-        for (int nc = 0; nc < NC; nc++) {
-          float f[NR];
-#pragma unroll
-          for (int r = 0; r < NR; r++) {
-            float w = fmaxf(fmaxf(x[0][0][nc][r], x[0][1][nc][r]), fmaxf(x[1][0][nc][r], x[1][1][nc][r]));
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, o));
-            const float m = w + cap_log2 > M[nc][r] + kTop ? w + cap_log2 - kStart : M[nc][r];
-            f[r] = exp2f(M[nc][r] - m);
-            M[nc][r] = m;
-            T[nc][r] = m + kTop - cap_log2;
-            L[nc][r] *= f[r];
-          }
-#pragma unroll
-          for (int i = 0; i < 2 * NB; i++)
-#pragma unroll
-            for (int k = 0; k < 4; k++) O[i][nc][k] *= f[NR == 2 ? (k & 1) : 0];
-        }
-      }
-      // ---- weighted probabilities, values ----
-#pragma unroll
-      for (int j = 0; j < 2; j++) {
-        uint32_t pb[NC][NB][2];  // B fragments: tokens in pairs, column g
+        for (int i = 1; i < NB; i++) vtop = __hmax2(vtop, __habs2(bits_h2(vsw[i / (NB / 2)][i % (NB / 2)])));
+        const float vmax = fmaxf(__low2float(vtop), __high2float(vtop));
+        bool grow = vmax > cap;
 #pragma unroll
         for (int nc = 0; nc < NC; nc++)
 #pragma unroll
-          for (int u = 0; u < 2; u++) {
-            float p[NR];
+          for (int r = 0; r < NR; r++)
+            grow = grow || fmaxf(x[0][nc][r], x[1][nc][r]) > T[nc][r];
+        if (__any_sync(0xffffffffu, grow)) {
+          const float top = warp_max(vmax);
+          if (top > cap) {  // the next power of two
+            cap_log2 = (float)((int)(__float_as_uint(top) >> 23) - 126);
+            cap = exp2f(cap_log2);
+          }
+#pragma unroll
+          for (int nc = 0; nc < NC; nc++) {
+            float f[NR];
 #pragma unroll
             for (int r = 0; r < NR; r++) {
-              p[r] = ex2_approx(x[j][u][nc][r] - M[nc][r]);
-              L[nc][r] += p[r];
+              float w = fmaxf(x[0][nc][r], x[1][nc][r]);
+#pragma unroll
+              for (int o = 4; o < 32; o <<= 1) w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, o));
+              const float m = w + cap_log2 > M[nc][r] + kTop ? w + cap_log2 - kStart : M[nc][r];
+              f[r] = exp2f(M[nc][r] - m);
+              M[nc][r] = m;
+              T[nc][r] = m + kTop - cap_log2;
+              L[nc][r] *= f[r];
             }
 #pragma unroll
-            for (int i = 0; i < NB / 2; i++) {  // two blocks at a time
-              const float2 v = f16x2_to_f2(vsw[j][u][i]);
-              uint32_t w[2];
-              if (TERMS == 2) {
-                const uint64_t y = f2_mul(f2(v.x, v.y), f2(p[0], p[0]));
-                float y0, y1, l0, l1;
-                f2_get(y, y0, y1);
-                const float t0 = __uint_as_float(__float_as_uint(y0) & 0xffffe000u);
-                const float t1 = __uint_as_float(__float_as_uint(y1) & 0xffffe000u);
-                f2_get(f2_fma(f2(t0, t1), f2(-1.f, -1.f), y), l0, l1);
-                w[0] = h2_bits(__floats2half2_rn(t0, l0));
-                w[1] = h2_bits(__floats2half2_rn(t1, l1));
-              } else {
-                float y0, y1, z0, z1;
-                f2_get(f2_mul(f2(v.x, v.y), f2(p[0], p[0])), y0, y1);
-                f2_get(f2_mul(f2(v.x, v.y), f2(p[NR - 1], p[NR - 1])), z0, z1);
-                w[0] = h2_bits(__floats2half2_rn(y0, z0));
-                w[1] = h2_bits(__floats2half2_rn(y1, z1));
-              }
-              pb[nc][2 * i][u] = movmatrix(w[0]);
-              pb[nc][2 * i + 1][u] = movmatrix(w[1]);
-            }
+            for (int i = 0; i < 2 * NB; i++)
+#pragma unroll
+              for (int k = 0; k < 4; k++) O[i][nc][k] *= f[NR == 2 ? (k & 1) : 0];
           }
+        }
+        // ---- weighted probabilities, values ----
+        float p[NC][2][NR];
+#pragma unroll
+        for (int nc = 0; nc < NC; nc++)
+#pragma unroll
+          for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int r = 0; r < NR; r++) {
+              p[nc][u][r] = ex2_approx(x[u][nc][r] - M[nc][r]);
+              L[nc][r] += p[nc][u][r];
+            }
         uint32_t vw[4][NB / 2];  // tokens t, t + 4, t + 8, t + 12: halfwords of the lane's dimensions
 #pragma unroll
         for (int k = 0; k < 4; k++) lds_words<NB / 2>(st + KB + (16 * j + t + 4 * k) * (DH / 2) + g * NB * 2, vw[k]);
 #pragma unroll
-        for (int i = 0; i < NB; i++) {
-          const uint32_t sel = (i & 1) ? 0x7632u : 0x5410u;
-          uint32_t z0 = __byte_perm(vw[0][i / 2], vw[1][i / 2], sel), z1 = __byte_perm(vw[2][i / 2], vw[3][i / 2], sel);
+        for (int i2 = 0; i2 < NB / 2; i2++) {  // two blocks at a time
+          uint32_t pb[2][NC][MT][2];  // [block] B fragments: tokens in pairs, column g
 #pragma unroll
-          for (int m = 0; m < 2; m++) {
-            if (EXACT) {
-              const uint32_t av[4] = {codes_f16<false>(z0), codes_f16<true>(z0), codes_f16<false>(z1), codes_f16<true>(z1)};
+          for (int u = 0; u < 2; u++) {
+            const float2 v = f16x2_to_f2(vsw[u][i2]);
 #pragma unroll
-              for (int nc = 0; nc < NC; nc++) mma16816(O[2 * i + m][nc], av, pb[nc][i][0], pb[nc][i][1]);
-            } else {
-              // as the key codes, f16 subnormals; the offset is a product of its own
-              const uint32_t av[4] = {z0 & 0x000f000fu, z0 & 0x00f000f0u, z1 & 0x000f000fu, z1 & 0x00f000f0u};
-              const uint32_t off[4] = {0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u};  // -8, -128 times 2^-24
+            for (int nc = 0; nc < NC; nc++) {
+              float y[NR][2], l[NR][2];  // a weighted probability's first f16 number (exact in f32) and what is left
 #pragma unroll
-              for (int nc = 0; nc < NC; nc++) {
-                mma16816(O[2 * i + m][nc], av, pb[nc][i][0], pb[nc][i][1]);
-                mma16816(O[2 * i + m][nc], off, pb[nc][i][0], pb[nc][i][1]);
+              for (int r = 0; r < NR; r++) {
+                const uint64_t w = f2_mul(f2(v.x, v.y), f2(p[nc][u][r], p[nc][u][r]));
+                f2_get(w, y[r][0], y[r][1]);
+                if (WIDE) {
+                  y[r][0] = __uint_as_float(__float_as_uint(y[r][0]) & 0xffffe000u);
+                  y[r][1] = __uint_as_float(__float_as_uint(y[r][1]) & 0xffffe000u);
+                  f2_get(f2_fma(f2(y[r][0], y[r][1]), f2(-1.f, -1.f), w), l[r][0], l[r][1]);
+                }
+              }
+#pragma unroll
+              for (int e = 0; e < 2; e++) {
+                pb[e][nc][0][u] = movmatrix(h2_bits(CT == 2 ? __floats2half2_rn(y[0][e], l[0][e]) : __floats2half2_rn(y[0][e], y[NR - 1][e])));
+                if (MT == 2) pb[e][nc][MT - 1][u] = movmatrix(h2_bits(__floats2half2_rn(l[0][e], l[NR - 1][e])));
               }
             }
-            z0 >>= 8, z1 >>= 8;
+          }
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const int i = 2 * i2 + e;
+            const uint32_t sel = e ? 0x7632u : 0x5410u;
+            uint32_t z0 = __byte_perm(vw[0][i2], vw[1][i2], sel), z1 = __byte_perm(vw[2][i2], vw[3][i2], sel);
+#pragma unroll
+            for (int m = 0; m < 2; m++) {
+              if (EXACT) {
+                const uint32_t av[4] = {codes_f16<false>(z0), codes_f16<true>(z0), codes_f16<false>(z1), codes_f16<true>(z1)};
+#pragma unroll
+                for (int nc = 0; nc < NC; nc++) {
+                  float d[4];
+                  mma16816_zero(d, av, pb[e][nc][MT - 1][0], pb[e][nc][MT - 1][1]);
+                  if (MT == 2) mma16816(d, av, pb[e][nc][0][0], pb[e][nc][0][1]);
+                  float(&o)[4] = O[2 * i + m][nc];
+                  f2_get(f2_add(f2(o[0], o[1]), f2(d[0], d[1])), o[0], o[1]);
+                  f2_get(f2_add(f2(o[2], o[3]), f2(d[2], d[3])), o[2], o[3]);
+                }
+              } else {
+                // as the key codes, f16 subnormals; the offset is a product of its own
+                const uint32_t av[4] = {z0 & 0x000f000fu, z0 & 0x00f000f0u, z1 & 0x000f000fu, z1 & 0x00f000f0u};
+                const uint32_t off[4] = {0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u};  // -8, -128 times 2^-24
+#pragma unroll
+                for (int nc = 0; nc < NC; nc++) {
+                  mma16816(O[2 * i + m][nc], av, pb[e][nc][0][0], pb[e][nc][0][1]);
+                  mma16816(O[2 * i + m][nc], off, pb[e][nc][0][0], pb[e][nc][0][1]);
+                }
+              }
+              z0 >>= 8, z1 >>= 8;
+            }
           }
         }
       }
@@ -678,10 +722,10 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC)) attn_paged_kernel
         for (int i = 0; i < NB; i++) {  // dimensions 32i + 4g .. + 3
           const float *o0 = O[2 * i][nc], *o1 = O[2 * i + 1][nc];
           float4 v;
-          v.x = (TERMS == 2 ? o0[0] + o0[1] : o0[r]) * f;
-          v.y = (TERMS == 2 ? o0[2] + o0[3] : o0[2 + r]) * (0.0625f * f);
-          v.z = (TERMS == 2 ? o1[0] + o1[1] : o1[r]) * f;
-          v.w = (TERMS == 2 ? o1[2] + o1[3] : o1[2 + r]) * (0.0625f * f);
+          v.x = (CT == 2 ? o0[0] + o0[1] : o0[r]) * f;
+          v.y = (CT == 2 ? o0[2] + o0[3] : o0[2 + r]) * (0.0625f * f);
+          v.z = (CT == 2 ? o1[0] + o1[1] : o1[r]) * f;
+          v.w = (CT == 2 ? o1[2] + o1[3] : o1[2 + r]) * (0.0625f * f);
           if (complete) {
             if (rl < rows) {
               const int rr = r0 + rl, s = rr / a.G, h = kvh * a.G + rr % a.G;
@@ -818,12 +862,12 @@ __global__ void __launch_bounds__(128) attn_paged_join_kernel(const PagedAttnArg
   store4_dt(a.out, (((size_t)open.y * a.S + s) * a.H + h) * DH + d, a.dtype, y);
 }
 
-template <int DH, int TERMS, int NC, bool EXACT>
+template <int DH, int CT, int MT, int NC, bool EXACT>
 int launch(hcu_context* h, PagedAttnArgs a) {
   const char* op = "hcu_attention_paged";
-  constexpr int RB = 8 * NC / TERMS;
+  constexpr int RB = 8 * NC / CT;
   constexpr size_t smem = paged_smem(DH, RB), record = (size_t)RB * (DH + 2) * sizeof(float);
-  auto kern = attn_paged_kernel<DH, TERMS, NC, EXACT>;
+  auto kern = attn_paged_kernel<DH, CT, MT, NC, EXACT>;
   static std::atomic<uint64_t> attr_done{0};  // per device
   HCU_TRY(once_per_device(attr_done, h->device, [&]() -> int {
     return check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), op);
@@ -832,7 +876,7 @@ int launch(hcu_context* h, PagedAttnArgs a) {
   a.nrb = (a.R + RB - 1) / RB;
   const long long units = (long long)a.batch * a.kv.KV * a.nrb;
   if (units > 0x7fffffffLL) return fail(HCU_EINVAL, "%s: batch x KV x query row blocks too large", op);
-  long long grid = std::min(kMaxParts, h->sm_count * paged_ctas(DH, NC));
+  long long grid = std::min(kMaxParts, h->sm_count * paged_ctas(DH, NC, MT));
   // The line must not pass 2^31 and the records must fit the workspace (behind the other ops' tickets).
   const size_t room = h->workspace_bytes > kTicketBytes ? h->workspace_bytes - kTicketBytes : 0;
   const long long span = a.window > 0 ? std::min<long long>(a.max_context, (long long)a.window + a.S + CHUNK) : a.max_context;
@@ -861,15 +905,14 @@ template <int DH>
 int launch_dh(hcu_context* h, const PagedAttnArgs& a) {
   if (a.dtype == HCU_DT_BF16) {
     // One f16 number per query where the rows need the columns: its rounding (2^-11) is below the result's (2^-8).
-    if (a.R <= 4) return launch<DH, 2, 1, false>(h, a);
+    if (a.R <= 4) return launch<DH, 2, 1, 1, false>(h, a);
     if constexpr (DH == 128)
-      if (a.R > 8) return launch<DH, 1, 2, false>(h, a);
-    return launch<DH, 1, 1, false>(h, a);
+      if (a.R > 8) return launch<DH, 1, 1, 2, false>(h, a);
+    return launch<DH, 1, 1, 1, false>(h, a);
   }
-  if (a.dtype == HCU_DT_F16 && a.R <= 4) return launch<DH, 2, 1, false>(h, a);
-  if constexpr (DH == 128)
-    if (a.R > 4) return launch<DH, 2, 2, true>(h, a);
-  return launch<DH, 2, 1, true>(h, a);
+  if (a.dtype == HCU_DT_F16 && a.R <= 4) return launch<DH, 2, 1, 1, false>(h, a);
+  if (a.R > 4) return launch<DH, 1, 2, 1, true>(h, a);
+  return launch<DH, 2, 1, 1, true>(h, a);
 }
 
 }  // namespace

@@ -98,6 +98,34 @@ def test_little_workspace():
         be.close()
 
 
+@pytest.mark.parametrize("H,KV,Dh", [(8, 8, 128), (16, 2, 128), (4, 2, 256), (16, 2, 256)])
+def test_long_sums_have_no_bias(H, KV, Dh):
+    """f32 sums over 16384 tokens by one warp.  1024 additions that round to nearest are off by u / sqrt(3) of the sum each
+    (u = 2^-24), sqrt(1024 / 3) u / sqrt(3) = 11 u together for values of one sign; three times that, and a few steps for
+    scores of 0.1.  Additions that truncate would be off by some 500 u."""
+    be = CudaBackend(0, workspace_bytes=(1 << 18) + 4096)
+    try:
+        g = gen(H + Dh)
+        n = 16384
+        c = PagedKVCache.allocate(n // 64, 64, KV, Dh)
+        for t in (c.k, c.v):
+            t.copy_(torch.randint(0, 256, t.shape, generator=g, device=dev, dtype=torch.uint8))
+        c.v.bitwise_or_(0x88)  # codes from 8 to 15
+        for t in (c.k_scale, c.v_scale):
+            t.copy_(torch.rand(t.shape, generator=g, device=dev) * 0.2 + 0.05)
+        q = torch.randn((1, 1, H, Dh), generator=g, device=dev) * 0.01
+        out = torch.empty_like(q)
+        table = torch.randperm(n // 64, generator=g, device=dev).int()[None]
+        be.attention_paged(q, c, out, table, i32([n]))
+        t = torch.arange(n, device=dev)
+        slots = table[0].long()[t // 64] * 64 + t % 64
+        k, v = (ref.cache_rows(c, slots, w) for w in "kv")
+        want = ref.attend(q[0].double(), k, v, n - 1)[0]
+        assert float((out[0].double() - want).norm() / want.norm()) < (33 + 8) * 2.0 ** -24
+    finally:
+        be.close()
+
+
 @pytest.mark.parametrize("chunk", [1, 32, 100, 4096, 2 ** 40])
 def test_chunk_option(backend, chunk):
     g = gen(4)
