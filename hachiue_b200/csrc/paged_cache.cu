@@ -6,7 +6,12 @@
 //  * Append: a block per token, so that its cos and sin values are loaded once
 //    into registers for all of its rows; eight elements per lane, a row of 128
 //    being half a warp.  A Q4_0 block is then four lanes, a lane's codes one word of
-//    a key row or two halfwords of a value row.
+//    a key row or two halfwords of a value row.  For prompts four blocks per SM walk
+//    the tokens, each with the next one's rows on their way into L2 (a block per
+//    token spent its life waiting for its slot, then its angles, then its rows: 76
+//    against 65 us below).  8192 tokens of 32 query, 8 key and 8 value heads of 128,
+//    bf16: 65 us, 181 MB at 2.8 TB/s, of which the values' and keys' codes
+//    take 40: 370 instructions per warp and two rows, at 70 % of the issue rate.
 //  * Read: eight bytes of codes per lane, so that a warp has four rows of 128 of
 //    both tensors in flight, and writes whole 32-byte sectors.
 #include <algorithm>
@@ -32,12 +37,17 @@ struct AppendArgs {
   uint32_t* status;
 };
 
-// floor(x / d + 8.5) held within 0..15, exactly, without a division: adding
-// 1.5 * 2^23 + 8 rounds y * inv + 8 to the nearest integer, which is off by at
-// most one level next to a border, and the borders (c - 8.5) * d and
-// (c - 7.5) * d of a level are products of an 11-bit and a 5-bit number, exact
-// in f32, so two compares put it right.  y is x times the sign of d, a is |d|
-// (an f16 value above 0), inv about 1 / a.
+// floor(x / d + 8.5) held within 0..15, exactly, without a division.  d is an
+// f16 value other than 0 and inv about 1 / d; y is x times the sign of d, a is |d|.
+//
+// q4_codes: x * inv + 8 + 2^-18, rounded to the nearest integer.  The sum is
+// off by less than 2^-19 (inv by an ulp, the sum by half of one), so a border
+// goes to the level above it, as it should, and only a y less than 2^-17 a
+// below a border can be taken for it.  There is none among 16-bit inputs: y is a
+// multiple of 2^-12 a there, and so is a border (an 11-bit number times an odd
+// multiple of a half).  Where y is any f32 number such a one is looked for, and
+// q4_code puts it right by comparing with the borders (c - 8.5) a and (c - 7.5) a,
+// products of an 11-bit and a 5-bit number, exact in f32.
 __device__ __forceinline__ uint32_t q4_code(float y, float a, float inv) {
   float c = fminf(fmaxf(fmaf(y, inv, 12582920.f) - 12582912.f, 0.f), 15.f);
   const float lower = fmaf(c, a, -8.5f * a);
@@ -45,10 +55,33 @@ __device__ __forceinline__ uint32_t q4_code(float y, float a, float inv) {
   if (lower + a <= y) c += 1.f;
   return __float_as_uint(fminf(fmaxf(c, 0.f), 15.f) + 8388608.f) & 15u;
 }
+__device__ __forceinline__ uint32_t q4_codes(const float (&x)[8], float d, float inv, bool any_f32) {
+  float v[8], c[8];
+  const uint64_t magic = f2(12582912.f, 12582912.f), unmagic = f2(-12582912.f, -12582912.f);
+  float near = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    f2_get(f2_fma(f2(x[i], x[i + 1]), f2(inv, inv), f2(8.000003814697265625f, 8.000003814697265625f)), v[i], v[i + 1]);
+#pragma unroll
+    for (int u = 0; u < 2; u++) v[i + u] = fminf(fmaxf(v[i + u], 0.f), 15.f);
+    const uint64_t w = f2_add(f2_add(f2(v[i], v[i + 1]), magic), unmagic);
+    f2_get(w, c[i], c[i + 1]);
+    if (any_f32) near = fminf(near, fminf(v[i] - c[i], v[i + 1] - c[i + 1]));
+  }
+  if (any_f32 && near < -0.49999f) {
+    uint32_t code = 0;
+#pragma unroll
+    for (int i = 7; i >= 0; i--) code = code << 4 | q4_code(copysignf(1.f, d) * x[i], fabsf(d), fabsf(inv));
+    return code;
+  }
+  const float lo = fmaf(c[3], 4096.f, fmaf(c[2], 256.f, fmaf(c[1], 16.f, c[0] + 8388608.f)));
+  const float hi = fmaf(c[7], 4096.f, fmaf(c[6], 256.f, fmaf(c[5], 16.f, c[4] + 8388608.f)));
+  return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x5410);
+}
 
 // Quantises the eight elements of each lane: a block is four lanes.  Returns the
 // lane's codes (element 0 lowest) and the block's scale.  The whole warp calls it.
-__device__ __forceinline__ uint32_t q4_block(const float (&x)[8], int lane, __half* scale) {
+__device__ __forceinline__ uint32_t q4_block(const float (&x)[8], int lane, bool any_f32, __half* scale) {
   uint32_t top = 0;
   float m = x[0];  // the lane's first element of the lane's largest magnitude
 #pragma unroll
@@ -66,115 +99,134 @@ __device__ __forceinline__ uint32_t q4_block(const float (&x)[8], int lane, __ha
   m = __shfl_sync(0xffffffffu, m, first);
   const __half d = __float2half_rn(fminf(fmaxf(m * -0.125f, -65504.f), 65504.f));
   *scale = d;
-  const float df = __half2float(d), a = fabsf(df);
-  if (a == 0.f) return 0x88888888u;
-  const float inv = __fdiv_rn(1.f, a);
-  const uint32_t sign = __float_as_uint(df) & 0x80000000u;
-  uint32_t code = 0;
-#pragma unroll
-  for (int c = 0; c < 8; c++) code |= q4_code(__uint_as_float(__float_as_uint(x[c]) ^ sign), a, inv) << (4 * c);
-  return code;
+  const float df = __half2float(d);
+  if (df == 0.f) return 0x88888888u;
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(df));
+  return q4_codes(x, df, inv, any_f32);
 }
 
+constexpr int kAppendBlocks = 4;  // per SM: 64 registers hold a row without spills (3: 69 us, 5: 86)
+
 template <typename T, int DH>
-__global__ void __launch_bounds__(256, 5) rope_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(256, kAppendBlocks) rope_append_kernel(const AppendArgs a) {
   constexpr int LPR = DH / 8, RPB = 256 / LPR, NB = DH / 32;  // lanes per row, rows per pass of the block
-  const int lane = threadIdx.x & 31, l = threadIdx.x % LPR, i = blockIdx.x;
-  const long long slot = a.slots[i];
-  if (slot < 0) return;
-  const int pos = a.half ? a.positions[i] : 0;
-  if (slot >= a.n_slots || (a.half && (pos < 0 || pos >= a.table_rows))) {
-    if (threadIdx.x == 0 && blockIdx.y == 0) atomicOr(a.status, HCU_DEVERR_BADARG);
-    return;
-  }
-  // The lane's elements 8l .. 8l + 7 in two groups of four, which may lie on different sides of the pairs' halves.
-  float cs[2][4], sn[2][4];  // sn: negative for the lower half of the pairs
-  int partner[2];
-#pragma unroll
-  for (int u = 0; u < 2; u++) {
-    const int e = 8 * l + 4 * u;
-    partner[u] = -1;
-#pragma unroll
-    for (int c = 0; c < 4; c++) cs[u][c] = 1.f, sn[u][c] = 0.f;
-    if (e < 2 * a.half) {
-      const bool low = e < a.half;
-      const int at = low ? e : e - a.half;
-      load4(a.cos_tab + (long long)pos * a.half + at, cs[u]);
-      load4(a.sin_tab + (long long)pos * a.half + at, sn[u]);
-      if (low)
-#pragma unroll
-        for (int c = 0; c < 4; c++) sn[u][c] = -sn[u][c];
-      partner[u] = low ? e + a.half : e - a.half;
-    }
-  }
-  // Reads a row's eight elements and their partners (from memory again: the row is in L1).
-  auto read = [&](const T* src, float (&x)[8], float (&w)[8]) {
-    load8(src + 8 * l, x);
-    if (a.half % 8 == 0) {
-      if (partner[0] >= 0) load8(src + partner[0], w);
-    } else {
-#pragma unroll
-      for (int u = 0; u < 2; u++) {
-        float y[4] = {};
-        if (partner[u] >= 0) load4(src + partner[u], y);
-#pragma unroll
-        for (int c = 0; c < 4; c++) w[4 * u + c] = y[c];
+  const int lane = threadIdx.x & 31, l = threadIdx.x % LPR, stride = gridDim.x;
+  int i = blockIdx.x;
+  long long slot = a.slots[i];
+  int pos = a.half ? a.positions[i] : 0;
+  for (; i < a.n; i += stride) {
+    // The block's next token: its slot and position are under way, its rows go into L2.
+    const long long here = slot;
+    const int at_pos = pos;
+    if (i + stride < a.n) {
+      slot = a.slots[i + stride];
+      if (a.half) pos = a.positions[i + stride];
+      constexpr int LINES = DH * (int)sizeof(T) / 128;  // of a row
+      for (int r = threadIdx.x; r < (a.H + 2 * a.kv.KV) * LINES; r += 256) {
+        const int row = r / LINES - a.H;
+        const char* base = reinterpret_cast<const char*>(
+            row < 0 ? static_cast<const T*>(a.q) + (i + stride) * a.q_stride
+                    : row < a.kv.KV ? static_cast<const T*>(a.k) + (i + stride) * a.k_stride : static_cast<const T*>(a.v) + (i + stride) * a.v_stride);
+        const int in = row < 0 ? r : r - (a.H + (row < a.kv.KV ? 0 : a.kv.KV)) * LINES;
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(base + in * 128));
       }
     }
-  };
-  const int sub = threadIdx.x / LPR, first = blockIdx.y * RPB, step = gridDim.y * RPB;  // warp-uniform loops
-  // ---- queries ----
-  const T* q = static_cast<const T*>(a.q) + i * a.q_stride;
-  T* q_out = static_cast<T*>(a.q_out) + (long long)i * a.H * DH + 8 * l;
+    if (here < 0) continue;
+    if (here >= a.n_slots || (a.half && (at_pos < 0 || at_pos >= a.table_rows))) {
+      if (threadIdx.x == 0 && blockIdx.y == 0) atomicOr(a.status, HCU_DEVERR_BADARG);
+      continue;
+    }
+    // The lane's elements 8l .. 8l + 7 in two groups of four, which may lie on different sides of the pairs' halves.
+    float cs[2][4], sn[2][4];  // sn: negative for the lower half of the pairs
+    int partner[2];
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const int e = 8 * l + 4 * u;
+      partner[u] = -1;
+#pragma unroll
+      for (int c = 0; c < 4; c++) cs[u][c] = 1.f, sn[u][c] = 0.f;
+      if (e < 2 * a.half) {
+        const bool low = e < a.half;
+        const int at = low ? e : e - a.half;
+        load4(a.cos_tab + (long long)at_pos * a.half + at, cs[u]);
+        load4(a.sin_tab + (long long)at_pos * a.half + at, sn[u]);
+        if (low)
+#pragma unroll
+          for (int c = 0; c < 4; c++) sn[u][c] = -sn[u][c];
+        partner[u] = low ? e + a.half : e - a.half;
+      }
+    }
+    // Reads a row's eight elements and their partners (from memory again: the row is in L1).
+    auto read = [&](const T* src, float (&x)[8], float (&w)[8]) {
+      load8(src + 8 * l, x);
+      if (a.half % 8 == 0) {
+        if (partner[0] >= 0) load8(src + partner[0], w);
+      } else {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          float y[4] = {};
+          if (partner[u] >= 0) load4(src + partner[u], y);
+#pragma unroll
+          for (int c = 0; c < 4; c++) w[4 * u + c] = y[c];
+        }
+      }
+    };
+    const int sub = threadIdx.x / LPR, first = blockIdx.y * RPB, step = gridDim.y * RPB;  // warp-uniform loops
+    // ---- queries ----
+    const T* q = static_cast<const T*>(a.q) + i * a.q_stride;
+    T* q_out = static_cast<T*>(a.q_out) + (long long)i * a.H * DH + 8 * l;
 #pragma unroll 2
-  for (int base = first; base < a.H; base += step) {
-    const int h = base + sub;
-    float x[8], w[8] = {};
-    if (h < a.H) read(q + h * DH, x, w);
-    __syncwarp();  // in place: a row has been read before any lane writes
-    if (h < a.H) {
+    for (int base = first; base < a.H; base += step) {
+      const int h = base + sub;
+      float x[8], w[8] = {};
+      if (h < a.H) read(q + h * DH, x, w);
+      __syncwarp();  // in place: a row has been read before any lane writes
+      if (h < a.H) {
 #pragma unroll
-      for (int c = 0; c < 8; c++)
-        if (partner[c >> 2] >= 0) x[c] = fmaf(x[c], cs[c >> 2][c & 3], w[c] * sn[c >> 2][c & 3]);
-      store8(q_out + h * DH, x);
-    }
-  }
-  // ---- keys and values: the passes go on where the queries' ended, so that a block per pass (few tokens) shares them ----
-  const long long at0 = paged_row(a.kv, slot >> a.kv.page_log2, 0, (int)(slot & ((1 << a.kv.page_log2) - 1)));
-  const T* k = static_cast<const T*>(a.k) + i * a.k_stride;
-  const T* v = static_cast<const T*>(a.v) + i * a.v_stride;
-  const int q_passes = (a.H + RPB - 1) / RPB, begin = (blockIdx.y + gridDim.y - q_passes % gridDim.y) % gridDim.y;
-  const int b = l >> 2, t = l & 3;  // block, quarter of it
-#pragma unroll 1
-  for (int base = begin * RPB; base < 2 * a.kv.KV; base += step) {
-    const int r = base + sub;
-    const bool row = r < 2 * a.kv.KV, key = r < a.kv.KV;
-    const int g = key ? r : r - a.kv.KV;
-    float x[8] = {}, w[8] = {};
-    if (row && key) read(k + g * DH, x, w);
-    if (row && !key) load8(v + g * DH + 8 * l, x);
-    __syncwarp();
-    if (__any_sync(0xffffffffu, row && key)) {  // a branch of the warp's: it would pay for f64 instructions that its lanes skip
-      if (row && key) {
-#pragma unroll
-        for (int c = 0; c < 8; c++)  // the products of two f32 values are exact in f64
-          if (partner[c >> 2] >= 0)
-            x[c] = (float)__dadd_rn(__dmul_rn(x[c], cs[c >> 2][c & 3]), __dmul_rn(w[c], sn[c >> 2][c & 3]));
-        if (a.k_out) store8(static_cast<T*>(a.k_out) + ((long long)i * a.kv.KV + g) * DH + 8 * l, x);
+        for (int c = 0; c < 8; c++)
+          if (partner[c >> 2] >= 0) x[c] = fmaf(x[c], cs[c >> 2][c & 3], w[c] * sn[c >> 2][c & 3]);
+        store8(q_out + h * DH, x);
       }
     }
-    __half d;
-    const uint32_t code = q4_block(x, lane, &d);
-    if (!row) continue;
-    const long long at = at0 + ((long long)g << a.kv.page_log2);
-    if (key) {
-      *reinterpret_cast<uint32_t*>(a.kv.k + at * (DH / 2) + (t * NB + b) * 4) = code;
-      if (t == 0) a.kv.ks[at * NB + b] = d;
-    } else {
-      uint8_t* dst = a.kv.v + at * (DH / 2);
-      *reinterpret_cast<uint16_t*>(dst + (2 * t * NB + b) * 2) = (uint16_t)code;
-      *reinterpret_cast<uint16_t*>(dst + ((2 * t + 1) * NB + b) * 2) = (uint16_t)(code >> 16);
-      if (t == 0) a.kv.vs[at * NB + b] = d;
+    // ---- keys and values: the passes go on where the queries' ended, so that a block per pass (few tokens) shares them ----
+    const long long at0 = paged_row(a.kv, here >> a.kv.page_log2, 0, (int)(here & ((1 << a.kv.page_log2) - 1)));
+    const T* k = static_cast<const T*>(a.k) + i * a.k_stride;
+    const T* v = static_cast<const T*>(a.v) + i * a.v_stride;
+    const int q_passes = (a.H + RPB - 1) / RPB, begin = (blockIdx.y + gridDim.y - q_passes % gridDim.y) % gridDim.y;
+    const int b = l >> 2, t = l & 3;  // block, quarter of it
+#pragma unroll 1
+    for (int base = begin * RPB; base < 2 * a.kv.KV; base += step) {
+      const int r = base + sub;
+      const bool row = r < 2 * a.kv.KV, key = r < a.kv.KV;
+      const int g = key ? r : r - a.kv.KV;
+      float x[8] = {}, w[8] = {};
+      if (row && key) read(k + g * DH, x, w);
+      if (row && !key) load8(v + g * DH + 8 * l, x);
+      __syncwarp();
+      const bool turned = __any_sync(0xffffffffu, row && key);
+      if (turned) {  // a branch of the warp's: it would pay for f64 instructions that its lanes skip
+        if (row && key) {
+#pragma unroll
+          for (int c = 0; c < 8; c++)  // the products of two f32 values are exact in f64
+            if (partner[c >> 2] >= 0)
+              x[c] = (float)__dadd_rn(__dmul_rn(x[c], cs[c >> 2][c & 3]), __dmul_rn(w[c], sn[c >> 2][c & 3]));
+          if (a.k_out) store8(static_cast<T*>(a.k_out) + ((long long)i * a.kv.KV + g) * DH + 8 * l, x);
+        }
+      }
+      __half d;
+      const uint32_t code = q4_block(x, lane, sizeof(T) == 4 || (a.half && turned), &d);
+      if (!row) continue;
+      const long long at = at0 + ((long long)g << a.kv.page_log2);
+      if (key) {
+        *reinterpret_cast<uint32_t*>(a.kv.k + at * (DH / 2) + (t * NB + b) * 4) = code;
+        if (t == 0) a.kv.ks[at * NB + b] = d;
+      } else {
+        uint8_t* dst = a.kv.v + at * (DH / 2);
+        *reinterpret_cast<uint16_t*>(dst + (2 * t * NB + b) * 2) = (uint16_t)code;
+        *reinterpret_cast<uint16_t*>(dst + ((2 * t + 1) * NB + b) * 2) = (uint16_t)(code >> 16);
+        if (t == 0) a.kv.vs[at * NB + b] = d;
+      }
     }
   }
 }
@@ -265,7 +317,8 @@ template <typename T>
 int launch_append(hcu_context* h, const AppendArgs& a, int dh) {
   // Few tokens: a block per pass of rows.  Many: one per token, which walks its rows.
   const int rpb = 256 / (dh / 8), passes = (a.H + rpb - 1) / rpb + (2 * a.kv.KV + rpb - 1) / rpb;
-  const dim3 grid((unsigned)a.n, a.n < 4 * h->sm_count ? (unsigned)std::min(passes, 65535) : 1u);
+  const bool few = a.n < 4 * h->sm_count;
+  const dim3 grid((unsigned)(few ? a.n : std::min(a.n, kAppendBlocks * h->sm_count)), few ? (unsigned)std::min(passes, 65535) : 1u);
   if (dh == 128) rope_append_kernel<T, 128><<<grid, 256, 0, h->stream>>>(a);
   else rope_append_kernel<T, 256><<<grid, 256, 0, h->stream>>>(a);
   return after_launch("hcu_rope_append_paged: launch");
@@ -298,7 +351,7 @@ extern "C" int hcu_rope_append_paged(hcu_handle h, const hcu_rope_append_params*
   HCU_TRY(hcu::check_paged(op, kv, &a.kv));
   const int eb = hcu::dtype_bytes(p->dtype);
   if (!eb) return fail(HCU_EINVAL, "%s: unknown dtype %u", op, p->dtype);
-  if (p->n > 0x7fffffffu || p->H > 65535u) return fail(HCU_EINVAL, "%s: n or H too large", op);
+  if (p->n > 0x40000000u || p->H > 65535u) return fail(HCU_EINVAL, "%s: n or H too large", op);
   if (p->rotaryDim % 8 || p->rotaryDim > kv->Dh)
     return fail(HCU_EINVAL, "%s: rotaryDim (%u) must be a multiple of 8, at most Dh (%u)", op, p->rotaryDim, kv->Dh);
   if (p->n == 0) return HCU_OK;

@@ -573,8 +573,8 @@ typedef struct {
  * multiple of 8, at most Dh.  Rows are 16-byte aligned, strides multiples of 8
  * elements.
  *
- * A negative slot marks padding: nothing of that row is read but its slot, and
- * nothing is written.  A slot past the cache or a position outside the tables
+ * A negative slot marks padding: what else the row holds, its position too,
+ * makes no difference, and nothing is written.  A slot past the cache or a position outside the tables
  * sets bit 2 of the device status and is skipped the same way.  The slots of
  * one call must differ: a row named twice holds parts of both tokens. */
 typedef struct {

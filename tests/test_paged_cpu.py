@@ -246,6 +246,40 @@ def test_levels_without_a_division():
             assert np.array_equal(got, want), (j, step)
 
 
+@pytest.mark.parametrize("ulp", [-1, 0, 1])
+def test_levels_by_a_biased_rounding(ulp):
+    """paged_cache.cu, q4_codes: x * inv + 8 + 2^-18 rounded, with a reciprocal that is off by an ulp either way.  Right for
+    every 16-bit input next to a border; an f32 input that it takes for the level above is one that it looks for."""
+    a = np.arange(1, 0x7c00, dtype=np.uint16).view(np.float16).astype(np.float32)
+    inv = f32(1.0) / a
+    inv = inv if ulp == 0 else np.nextafter(inv, np.float32(ulp * np.inf))
+    bias = np.float32(8 + 2.0 ** -18)
+    assert float(bias) == 8 + 2.0 ** -18
+    a64 = a.astype(np.float64)
+
+    def levels(y):
+        v = np.clip(f32(y.astype(np.float64) * inv + float(bias)), 0, 15).astype(np.float32)
+        c = (v + np.float32(12582912.0)) - np.float32(12582912.0)
+        return c, v - c
+
+    def exact(y):
+        return sum((y.astype(np.float64) >= (n - 8.5) * a64).astype(np.int64) for n in range(1, 16))
+
+    for j in range(1, 16):
+        border = (j - 8.5) * a64
+        for bits in (8, 11):  # bf16 and f16 inputs: the multiples of an 8- or 11-bit number's last place around the border
+            last = 2.0 ** (np.floor(np.log2(np.abs(border))) - bits + 1)
+            for k in (-2, -1, 0, 1, 2, 3):
+                y = f32((np.floor(border / last) + k) * last)
+                c, _ = levels(y)
+                assert np.array_equal(c.astype(np.int64), exact(y)), (j, bits, k)
+        for k in range(-40, 41, 5):  # f32 inputs within some steps of the border
+            y = (f32(border).view(np.int32) + k).view(np.float32)
+            c, rest = levels(y)
+            wrong = c.astype(np.int64) != exact(y)
+            assert (rest[wrong] < -0.49999).all()
+
+
 def test_codes_as_f16_bits():
     """attention_paged.cu: a code's bits in place are a subnormal f16, and with the exponent of 1024 an integer whose offset
     one subtraction takes off."""
