@@ -1,9 +1,10 @@
 """hachiue_b200 - B200 (sm_100a) backend for hachiue's attention hot path.
 
 GQA decode attention over the KV cache (qwen3 / qwen35 full attention),
-causal sliding-window attention (plamo3) and the Gated DeltaNet gated
-delta-rule recurrence (qwen35), as hand-written CUDA kernels behind the C ABI
-in include/hachiue_cuda.h.  ``CudaBackend`` is the Python host of that ABI and
+causal sliding-window attention (plamo3), the Gated DeltaNet gated delta-rule
+recurrence (qwen35) and paged serving (a 4-bit paged KV cache, its decode
+attention, packed prefill), as hand-written CUDA kernels behind the C ABI in
+include/hachiue_cuda.h.  ``CudaBackend`` is the Python host of that ABI and
 mirrors the reference's attention-dispatch seam (src/engine.ts:1056-1075).
 """
 from ._lib import (KV_BF16, KV_F16, KV_F32, KV_Q4_0, KV_Q8_0, KV_Q8_0_WGSL, HachiueError, LIB_PATH, load)  # noqa: F401

