@@ -161,6 +161,40 @@ def test_long_chains_of_items(backend, H, KV, ctas):
         backend.set_option("swa_ctas", 0)
 
 
+@pytest.mark.parametrize("H,KV", [(130, 1), (256, 1), (400, 2), (128, 1), (64, 1)])
+def test_groups_as_large_as_a_tile(backend, H, KV):
+    """More query heads per KV head than a tile has rows, and as many."""
+    g = gen(H)
+    lens, keys = [3, 1, 0, 9], [200, 1, 5, 9]
+    q, k, v = (torch.randn((n, h, 128), generator=g, device=dev).bfloat16() for n, h in ((13, H), (215, KV), (215, KV)))
+    out = torch.full_like(q, float("nan"))
+    for window in (0, 4):
+        backend.prefill_varlen(q, k, v, out, offsets(lens), offsets(keys), window)
+        check(out, q, k, v, offsets(lens), offsets(keys), window, torch.bfloat16)
+    c, table, slots = paged_batch(g, keys, 16, KV, 128)
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        check_decode(backend, c, table, slots, torch.randn((4, 1, H, 128), generator=g, device=dev).to(dtype), keys, 0)
+    assert backend.device_status() == 0
+
+
+def test_many_prompts(backend):
+    """A batch of 20000 prompts, most of them empty or a single token."""
+    g = gen(11)
+    lens = np.random.default_rng(5).choice([0, 1, 1, 2, 5], 20000).tolist()
+    lens[7777] = 600
+    q, k, v = (torch.randn((sum(lens), h, 128), generator=g, device=dev).half() for h in (2, 1, 1))
+    cu = offsets(lens)
+    out = torch.full_like(q, float("nan"))
+    backend.prefill_varlen(q, k, v, out, cu)
+    assert backend.device_status() == 0 and torch.isfinite(out).all()
+    ones = torch.tensor([n == 1 for n in lens], device=dev)
+    at = cu[:-1][ones].long()
+    assert torch.equal(out[at], v[at].expand(-1, 2, -1))  # one key: its value
+    lo, hi = int(cu[7770]), int(cu[7785])
+    some = cu[7770:7786] - lo
+    check(out[lo:hi], q[lo:hi], k[lo:hi], v[lo:hi], some, some, 0, torch.float16)
+
+
 def test_nothing_to_do(backend):
     c = PagedKVCache.allocate(2, 16, 1, 128)
     q = torch.ones((2, 1, 2, 128), device=dev)
