@@ -83,20 +83,32 @@ __device__ __forceinline__ int2 key_tiles(int r0, int r1, int G, int lq, int lk,
 }
 
 // One block: counts the sequences' blocks of 256 rows, sorts them by their number of key tiles (a counting sort, descending)
-// and writes them out.  Sequences whose offsets are not in order or not within the tensors are reported and left out.
+// and writes them out.  Sequences whose offsets are not in order or not within the tensors are reported and left out; one that
+// begins below any offset before it counts as such, so that the others do not overlap and their blocks fit the list.
 __global__ void __launch_bounds__(1024) varlen_items_kernel(const VarlenArgs a) {
-  __shared__ int bins[kBins], part[32], base;
+  __shared__ int bins[kBins], part[32], top_part[32], base, top_base;
   asm volatile("griddepcontrol.launch_dependents;");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   bins[tid] = 0;
-  if (tid == 0) base = 0;
+  if (tid == 0) base = 0, top_base = 0;
   __syncthreads();
   for (int b0 = 0; b0 < a.batch; b0 += 1024) {
     const int b = b0 + tid;
+    // the largest offset up to this sequence's first
+    int top = b < a.batch ? a.cu_q[b] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, top, o);
+      if (lane >= o) top = max(top, x);
+    }
+    if (lane == 31) top_part[warp] = top;
+    __syncthreads();
+    top = max(top, top_base);
+    for (int w = 0; w < warp; w++) top = max(top, top_part[w]);
     int n = 0;
     if (b < a.batch) {
       const int q0 = a.cu_q[b], q1 = a.cu_q[b + 1], k0 = a.cu_k[b], k1 = a.cu_k[b + 1];
-      if (q0 < 0 || q1 < q0 || q1 > a.total_q || k0 < 0 || k1 < k0 || k1 > a.total_k) atomicOr(a.status, HCU_DEVERR_BADARG);
+      if (q0 < top || q1 < q0 || q1 > a.total_q || k0 < 0 || k1 < k0 || k1 > a.total_k) atomicOr(a.status, HCU_DEVERR_BADARG);
       else n = (int)(((long long)(q1 - q0) * a.G + 2 * BM - 1) / (2 * BM));
     }
     int pre = n;
@@ -111,7 +123,7 @@ __global__ void __launch_bounds__(1024) varlen_items_kernel(const VarlenArgs a) 
     for (int w = 0; w < warp; w++) before += part[w];
     if (b < a.batch) a.blocks[b] = before + pre - n;
     __syncthreads();
-    if (tid == 1023) base = before + pre;
+    if (tid == 1023) base = before + pre, top_base = top;
     __syncthreads();
   }
   const int total = base;

@@ -641,7 +641,8 @@ int hcu_attention_paged(hcu_handle h, const hcu_attention_paged_params *p, const
  * Rows of out that no sequence covers are left as they were, and rows of k and
  * v outside a sequence have no influence on it, whatever they hold.  The
  * offsets must not decrease and must lie within the totals: a sequence whose
- * offsets do not is skipped and sets bit 2 of the device status.  The work list
+ * offsets do not, or whose queries begin below an earlier offset of cu_q, is
+ * skipped and sets bit 2 of the device status.  The work list
  * takes 32 bytes of workspace per 256 packed rows (total_q * H / KV) and
  * sequence; a call whose list does not fit fails with HCU_ENOMEM. */
 typedef struct {

@@ -195,6 +195,23 @@ def test_many_prompts(backend):
     check(out[lo:hi], q[lo:hi], k[lo:hi], v[lo:hi], some, some, 0, torch.float16)
 
 
+def test_offsets_that_begin_again(backend):
+    """Offsets that go back to 0 time and again name the same rows more often than the tensors have rows: all but the first
+    such sequence are skipped, in the first thousand as behind it."""
+    g = gen(12)
+    q, k, v = (torch.randn((300, h, 128), generator=g, device=dev).bfloat16() for h in (4, 2, 2))
+    for cu in ([0, 200] + [0, 0, 200] * 700 + [200, 300], [0] * 1030 + [200, 0, 0, 200, 200, 300]):
+        cu = i32(cu)
+        out = torch.full_like(q, 7.0)
+        backend.prefill_varlen(q, k, v, out, cu)
+        assert backend.device_status() == 2
+        check(out, q, k, v, i32([0, 200, 300]), i32([0, 200, 300]), 0, torch.bfloat16)
+    out = torch.full_like(q, 7.0)
+    backend.prefill_varlen(q, k, v, out, i32([-3, -2, 0, 300]), i32([0, 0, 0, 300]))  # negative ones are out of range
+    assert backend.device_status() == 2
+    check(out, q, k, v, i32([0, 300]), i32([0, 300]), 0, torch.bfloat16)
+
+
 def test_nothing_to_do(backend):
     c = PagedKVCache.allocate(2, 16, 1, 128)
     q = torch.ones((2, 1, 2, 128), device=dev)
