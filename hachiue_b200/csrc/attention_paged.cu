@@ -53,7 +53,8 @@ struct PagedAttnArgs {
   const int32_t* context;
   int batch, S, H, G, R, nrb, window, max_context, table_stride;
   int min_chunks;    // fewest chunks of 32 tokens worth a CTA of their own
-  int split;         // 0: every unit is one warp's (no room for partial sums)
+  int split;         // kWarpUnits, kLine or kCluster
+  int cluster;       // CTAs of a unit (kCluster)
   float scale_log2;  // log2(e) / sqrt(Dh)
   float* part;       // [gridDim.x][2] records of the units at a CTA's two ends: sums [RB][DH], then (M, l) [RB]
   int4* open;        // [gridDim.x] the unit that begins in a CTA and goes on: parts (0: none), sequence, KV head, row block
@@ -62,6 +63,14 @@ struct PagedAttnArgs {
 };
 
 constexpr int NW = 8;          // warps of a CTA
+// How the units (a sequence's KV head and row block) are handed out: each to a
+// warp (no room for partial sums), by equal pieces of the line of all their
+// chunks, or each to a cluster of CTAs, which joins its parts through shared
+// memory without a second kernel.  The host takes clusters for short contexts
+// and few units: up to four chunks per warp, in up to eight CTAs (replayed graphs, f32, 16 / 8
+// heads of 128, cluster / line: one sequence of 256 tokens 9.0 / 11.4 us, of 1024
+// 10.1 / 11.4, 16 of 1024 14.3 / 16.6, 16 of 2048 19.7 / 21.8; one of 4096 13.5 / 12.1).
+constexpr int kWarpUnits = 0, kLine = 1, kCluster = 2;
 constexpr int CHUNK = 32;      // tokens a warp takes at a time
 constexpr int kUnitCost = 3;    // chunks that a unit's queries and sums cost a warp besides its chunks
 constexpr float kNoM = -1e30f;  // M of a row that has seen no token
@@ -90,6 +99,40 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
 
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+
+// Adds a part's sums v and (reference point, sum of weights) to a row's.
+__device__ __forceinline__ void add_part(float& m, float& l, float (&o)[4], float2 ml, float4 v) {
+  const float mn = fmaxf(m, ml.x), f0 = ex2_approx(m - mn), f = ex2_approx(ml.x - mn);
+  m = mn;
+  l = fmaf(l, f0, ml.y * f);
+  o[0] = fmaf(o[0], f0, v.x * f), o[1] = fmaf(o[1], f0, v.y * f);
+  o[2] = fmaf(o[2], f0, v.z * f), o[3] = fmaf(o[3], f0, v.w * f);
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// The shared memory of CTA `rank` of the cluster, by this CTA's address of the same place.
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, int rank) {
+  uint32_t there;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
+  return there;
+}
+__device__ __forceinline__ float4 cluster_load4(uint32_t addr, int rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_addr(addr, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 cluster_load2(uint32_t addr, int rank) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(cluster_addr(addr, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t cluster_load1(uint32_t addr, int rank) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr(addr, rank)) : "memory");
+  return v;
+}
 
 // Two codes (one per 16-bit half, in bits 0-3) as f16 code - 8; HIGH: in bits 4-7, as 16 (code - 8).
 template <bool HIGH>
@@ -141,6 +184,7 @@ __device__ __forceinline__ void store4_dt(void* p, size_t at, int dtype, const f
   else store4(static_cast<__nv_bfloat16*>(p) + at, x);
 }
 
+constexpr int kMaxCluster = 8, kClusterChunks = 4;  // CTAs of a cluster, chunks of a warp in one at most
 constexpr int kMaxParts = 320;  // CTAs of a call, and so of a unit
 constexpr int STAGES = 2;
 constexpr int paged_stage_bytes(int dh) { return CHUNK * (dh + dh / 8); }  // codes and scales, keys and values
@@ -200,6 +244,8 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC, MT)) attn_paged_ke
   static_assert(RB * RS * 4 <= ST * SB, "a record fits a ring");
   static_assert(RB * DH * (WIDE ? 4 : 2) <= SB, "a segment's queries fit a stage");
   extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ __align__(16) float2 s_ml[RB];  // of the CTA's part (kCluster); s_mine: its sums
+  __shared__ __align__(16) uint32_t s_mine;
   __shared__ int scan[NW], s_b, s_pos;
   // Records of a warp's units that lie only partly in its piece: [2w] the one that ends there, [2w + 1] the one that
   // goes on.  u0 < 0: none.
@@ -215,7 +261,15 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC, MT)) attn_paged_ke
   PagedPlan plan;
   int seg_b, seg_base;  // sequence of the next segment, line position of its first chunk
   int pos, end, cta_first;
-  {
+  if (a.split == kCluster) {
+    const int unit = blockIdx.x / a.cluster, part = (blockIdx.x % a.cluster) * NW + warp, parts = a.cluster * NW;
+    seg_b = unit / per_chunk, seg_base = 0;
+    const int n = paged_chunks(a, seg_b).y;
+    cta_first = (unit % per_chunk) * (n + kUnitCost) + kUnitCost;
+    pos = cta_first + (int)((long long)n * part / parts), end = cta_first + (int)((long long)n * (part + 1) / parts);
+    if (threadIdx.x < 2 * NW) s_rec[threadIdx.x].u0 = -1;
+    __syncthreads();
+  } else {
     // Every thread sums a run of sequences; the line position of each run follows from a scan.
     const int run = (a.batch + 32 * NW - 1) / (32 * NW), b0 = threadIdx.x * run, b1 = min(a.batch, b0 + run);
     int sum = 0;
@@ -235,16 +289,16 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC, MT)) attn_paged_ke
       total += scan[w];
     }
     plan.total = total * per_chunk;
-    const int most = a.split ? (plan.total - 1) / a.min_chunks + 1 : (int)gridDim.x;
+    const int most = a.split == kLine ? (plan.total - 1) / a.min_chunks + 1 : (int)gridDim.x;
     plan.ctas = min((int)gridDim.x, most);
     plan.share = plan.total / plan.ctas;
     plan.more = plan.total % plan.ctas;
     if ((int)blockIdx.x >= plan.ctas) {
-      if (a.split && threadIdx.x == 0) a.open[blockIdx.x] = make_int4(0, 0, 0, 0);
+      if (a.split == kLine && threadIdx.x == 0) a.open[blockIdx.x] = make_int4(0, 0, 0, 0);
       return;
     }
     if (threadIdx.x < 2 * NW) s_rec[threadIdx.x].u0 = -1;
-    if (a.split) {
+    if (a.split == kLine) {
       cta_first = plan.start(blockIdx.x);
       const int len = plan.start(blockIdx.x + 1) - cta_first, lo = (pre - sum) * per_chunk;
       if (cta_first >= lo && cta_first < pre * per_chunk) {  // one thread's run holds the first chunk
@@ -281,7 +335,7 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC, MT)) attn_paged_ke
     Segment s;
     int u;
     int2 ch;
-    if (a.split) {
+    if (a.split != kWarpUnits) {
       ch = paged_chunks(a, seq_b);
       while (at >= seq_base + (ch.y + kUnitCost) * per_chunk) {
         seq_base += (ch.y + kUnitCost) * per_chunk;
@@ -711,7 +765,7 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC, MT)) attn_paged_ke
 
     // ---- the segment's sums ----
     constexpr float kUnscale = EXACT ? 1.f : 16777216.f;  // subnormal codes carry 2^-24
-    const bool complete = begins && ends;
+    const bool complete = begins && ends && a.split != kCluster;
     float* rec = ends ? buf + warp * RB * RS : reinterpret_cast<float*>(smem + warp * ST * SB);
 #pragma unroll
     for (int nc = 0; nc < NC; nc++)
@@ -757,8 +811,44 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC, MT)) attn_paged_ke
     const int s = rr / a.G, h = kvh * a.G + rr % a.G;
     store4_dt(a.out, (((size_t)b * a.S + s) * a.H + h) * DH + d, a.dtype, y);
   };
-  int4 open = make_int4(0, 0, 0, 0);
   constexpr int TPE = DH / 4;  // threads that hold a row
+  if (a.split == kCluster) {
+    // The CTA's parts go into one, in the place of the first; then every CTA of the cluster joins a share of the outputs.
+    const int unit = blockIdx.x / a.cluster, b = unit / per_chunk, kvh = unit % per_chunk / a.nrb, rb = unit % per_chunk % a.nrb;
+    const int r0 = rb * RB, rows = min(RB, a.R - r0);
+    uint32_t members = 0;
+    for (int k = 0; k < 2 * NW; k++) members |= (s_rec[k].u0 >= 0 ? 1u : 0u) << k;
+    auto record = [&](int w) { return (w & 1) ? reinterpret_cast<float*>(smem + (w >> 1) * ST * SB) : buf + (w >> 1) * RB * RS; };
+    float* mine = record(members ? __ffs(members) - 1 : 0);
+    for (int i = threadIdx.x; i < rows * TPE; i += 32 * NW) {
+      const int r = i / TPE, d = 4 * (i % TPE);
+      float m = kNoM, l = 0.f, o[4] = {};
+#pragma unroll 1
+      for (uint32_t x = members; x; x &= x - 1) {
+        const float* rec = record(__ffs(x) - 1) + r * RS;
+        add_part(m, l, o, *reinterpret_cast<const float2*>(rec + DH), *reinterpret_cast<const float4*>(rec + d));
+      }
+      *reinterpret_cast<float4*>(mine + r * RS + d) = make_float4(o[0], o[1], o[2], o[3]);
+      if (d == 0) s_ml[r] = make_float2(m, l);
+    }
+    if (threadIdx.x == 0) s_mine = smem_u32(mine);
+    cluster_sync();
+    const int share = a.cluster * 32 * NW;
+    for (int i = (blockIdx.x % a.cluster) * 32 * NW + threadIdx.x; i < rows * TPE; i += share) {
+      const int r = i / TPE, d = 4 * (i % TPE);
+      float m = kNoM, l = 0.f, o[4] = {};
+#pragma unroll 1
+      for (int c = 0; c < a.cluster; c++) {
+        const float2 ml = cluster_load2(smem_u32(&s_ml[r]), c);
+        if (ml.y == 0.f) continue;  // no token: the place may hold anything
+        add_part(m, l, o, ml, cluster_load4(cluster_load1(smem_u32(&s_mine), c) + (r * RS + d) * 4, c));
+      }
+      finish(o, l, b, kvh, r0 + r, d);
+    }
+    cluster_sync();  // the others' reads of this CTA's shared memory are done
+    return;
+  }
+  int4 open = make_int4(0, 0, 0, 0);
   for (int k = 0; k < 2 * NW;) {
     const int u0 = s_rec[k].u0;
     if (u0 < 0) {
@@ -784,11 +874,7 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC, MT)) attn_paged_ke
         const float* rec = ((w & 1) ? reinterpret_cast<const float*>(smem + (w >> 1) * ST * SB) : buf + (w >> 1) * RB * RS) + r * RS;
         const float2 ml = *reinterpret_cast<const float2*>(rec + DH);
         const float4 v = *reinterpret_cast<const float4*>(rec + d);
-        const float mn = fmaxf(m, ml.x), f0 = ex2_approx(m - mn), f = ex2_approx(ml.x - mn);
-        m = mn;
-        l = fmaf(l, f0, ml.y * f);
-        o[0] = fmaf(o[0], f0, v.x * f), o[1] = fmaf(o[1], f0, v.y * f);
-        o[2] = fmaf(o[2], f0, v.z * f), o[3] = fmaf(o[3], f0, v.w * f);
+        add_part(m, l, o, ml, v);
       }
       if (whole) {
         finish(o, l, b, kvh, r0 + r, d);
@@ -800,7 +886,7 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC, MT)) attn_paged_ke
     if (!whole && u0 >= cta_first)
       open = make_int4(plan.cta_of(u0 + s_rec[first].n - 1) - (int)blockIdx.x + 1, b, kvh, rb);
   }
-  if (a.split && threadIdx.x == 0) a.open[blockIdx.x] = open;
+  if (a.split == kLine && threadIdx.x == 0) a.open[blockIdx.x] = open;
 }
 
 // Joins the parts of the units that several CTAs share: block (c, r) row r of
@@ -886,19 +972,39 @@ int launch(hcu_context* h, PagedAttnArgs a) {
   const size_t room = h->workspace_bytes > kTicketBytes ? h->workspace_bytes - kTicketBytes : 0;
   const long long span = a.window > 0 ? std::min<long long>(a.max_context, (long long)a.window + a.S + CHUNK) : a.max_context;
   const long long most = units * (span / CHUNK + 2 + kUnitCost);  // chunks
-  a.split = room >= (size_t)grid * (2 * record + sizeof(int4)) && most < 0x7fffffffLL;
   a.min_chunks = h->opt_attn_chunk > 0 ? (int)std::min<int64_t>(1 << 24, (h->opt_attn_chunk + CHUNK - 1) / CHUNK) : 8;
-  grid = a.split ? std::min(grid, (most + a.min_chunks - 1) / a.min_chunks) : std::min(grid, (units + NW - 1) / NW);
+  // A cluster's CTAs, as many as there are chunks for their warps and slots for all.
+  const long long chunks = (span + CHUNK - 1) / CHUNK + (a.window > 0 ? 1 : 0);
+  a.cluster = 1;
+  while (a.cluster < kMaxCluster && a.cluster * NW < chunks && 2 * a.cluster * units <= grid) a.cluster *= 2;
+  if (chunks <= std::min(kMaxCluster, kClusterChunks * a.cluster) * NW && units <= grid && h->opt_attn_chunk == 0) {
+    a.split = kCluster;
+    grid = units * a.cluster;
+  } else if (room >= (size_t)grid * (2 * record + sizeof(int4)) && most < 0x7fffffffLL) {
+    a.split = kLine;
+    grid = std::min(grid, (most + a.min_chunks - 1) / a.min_chunks);
+  } else {
+    a.split = kWarpUnits;
+    grid = std::min(grid, (units + NW - 1) / NW);
+  }
   a.open = reinterpret_cast<int4*>(static_cast<uint8_t*>(h->workspace) + kTicketBytes);
   a.part = reinterpret_cast<float*>(a.open + grid);
-  kern<<<(unsigned)grid, 32 * NW, smem, h->stream>>>(a);
-  HCU_TRY(after_launch("hcu_attention_paged: launch"));
-  if (!a.split || grid == 1) return HCU_OK;
   cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(32 * NW);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = h->stream;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = a.split == kCluster ? a.cluster : 1;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = a.split == kCluster ? 1 : 0;
+  HCU_TRY(check_cuda(cudaLaunchKernelEx(&cfg, kern, a), "hcu_attention_paged: launch"));
+  if (a.split != kLine || grid == 1) return HCU_OK;
   cfg.gridDim = dim3((unsigned)(grid - 1), RB);  // no unit goes on behind the last CTA
   cfg.blockDim = dim3(128);
-  cfg.stream = h->stream;
-  cudaLaunchAttribute attr[1];
+  cfg.dynamicSmemBytes = 0;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;

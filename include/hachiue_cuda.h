@@ -541,8 +541,8 @@ int hcu_deltanet_chunked_prefill_snap(hcu_handle h, const hcu_gdn_prefill_params
  * hcu_attention_paged and hcu_prefill_varlen keep a call's partial sums and
  * work list in the handle's workspace: calls on one handle, and replays of
  * graphs captured from it, must not overlap (take a handle each).
- * HCU_OPT_ATTN_CHUNK sets the fewest keys that the decode gives a CTA (default
- * 256), HCU_OPT_SWA_CTAS caps the packed prefill's grid.
+ * HCU_OPT_ATTN_CHUNK sets the fewest keys that the decode gives a CTA (unset:
+ * 256, and short contexts go to clusters), HCU_OPT_SWA_CTAS caps the packed prefill's grid.
  *
  * A paged KV cache of one attention layer.  Token rows live in pages of
  * page_size rows (a power of two, 16..256) that any sequence may hold; slot

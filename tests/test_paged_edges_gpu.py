@@ -126,6 +126,20 @@ def test_long_sums_have_no_bias(H, KV, Dh):
         be.close()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("H,KV,Dh,S", [(4, 2, 128, 1), (16, 1, 128, 1), (12, 2, 256, 2)])
+@pytest.mark.parametrize("lens", [[32], [33, 1], [256, 255, 0], [290, 512], [513, 40, 1000], [1024], [1025], [2047], [2048, 5, 31, 32],
+                                  [2049], [1024] * 40 + [0, 7]])
+def test_short_contexts(backend, dtype, H, KV, Dh, S, lens):
+    """Around the lengths at which a unit's cluster grows, and where the work goes over to equal pieces."""
+    g = gen(H + Dh + sum(lens))
+    c, table, slots = paged_batch(g, lens, 32, KV, Dh)
+    q = torch.randn((len(lens), S, H, Dh), generator=g, device=dev).to(dtype)
+    check_decode(backend, c, table, slots, q, lens, 0)
+    check_decode(backend, c, table, slots, q, lens, 77)
+    assert backend.device_status() == 0
+
+
 @pytest.mark.parametrize("chunk", [1, 32, 100, 4096, 2 ** 40])
 def test_chunk_option(backend, chunk):
     g = gen(4)
