@@ -12,7 +12,7 @@
 //    diagonal wastes fewer keys, and any G works.  A work item is 256 rows (two
 //    tiles) of one sequence and KV head; a small kernel sorts the items by their
 //    number of key tiles, so that the persistent CTAs' shares are near equal
-//    whatever the lengths are.
+//    whatever the lengths are.  (A call with no more items than SMs needs no list.)
 //  * Warp roles: K / V by TMA (warp 0), tcgen05.mma of each tile (warps 1, 2: one
 //    warp for both spent more time on its barriers than the products take), Q rows
 //    by cp.async (warp 3), and a softmax warpgroup per tile, one thread per row.  S
@@ -51,6 +51,7 @@ struct VarlenArgs {
   int4* items;       // [2 * blocks]: {first query, queries, first key, keys}, {first packed row, first tile's key, tiles, 0}
   uint32_t recip_G, recip_KV;  // for quot()
   int q_tma;         // G divides 128: a tile's rows are one box of Q
+  int direct;        // every CTA has one item at most and finds it itself
   uint32_t* status;
 };
 
@@ -316,6 +317,52 @@ __device__ __forceinline__ int item_index(int k) {
   return k * P + ((k & 1) ? P - 1 - c : c);
 }
 
+// The item of this CTA where there are no more items than CTAs: each thread takes a sequence (at most kDirectBatch), checks it
+// as varlen_items_kernel does, and the one whose blocks hold the CTA's writes the item.  A launch less: 77 tokens of
+// 16 / 8 heads take 9.5 us in a replayed graph, through the list 10.1.
+constexpr int kDirectBatch = 384;
+__device__ __noinline__ void own_item(const VarlenArgs& a, RawItem* item, int* scan) {
+  const int b = threadIdx.x, lane = b & 31, warp = b >> 5;
+  int q0 = 0, q1 = 0, k0 = 0, k1 = 0;
+  if (b < a.batch) q0 = a.cu_q[b], q1 = a.cu_q[b + 1], k0 = a.cu_k[b], k1 = a.cu_k[b + 1];
+  int top = q0;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, top, o);
+    if (lane >= o) top = max(top, x);
+  }
+  if (lane == 31) scan[warp] = top;
+  if (b == 0) item->g = -1;
+  __syncthreads();
+  top = max(top, 0);
+  for (int w = 0; w < warp; w++) top = max(top, scan[w]);
+  int n = 0;
+  if (b < a.batch) {
+    if (q0 < top || q1 < q0 || q1 > a.total_q || k0 < 0 || k1 < k0 || k1 > a.total_k) {
+      if (blockIdx.x == 0) atomicOr(a.status, HCU_DEVERR_BADARG);
+    } else {
+      n = (int)(((long long)(q1 - q0) * a.G + 2 * BM - 1) / (2 * BM));
+    }
+  }
+  int pre = n;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, pre, o);
+    if (lane >= o) pre += x;
+  }
+  if (lane == 31) scan[12 + warp] = pre;
+  __syncthreads();
+  for (int w = 0; w < warp; w++) pre += scan[12 + w];
+  const int e = blockIdx.x / a.KV;
+  if (e >= pre - n && e < pre) {
+    const int lq = q1 - q0, lk = k1 - k0, r0 = (e - (pre - n)) * 2 * BM, rows = (int)min((long long)lq * a.G - r0, 2LL * BM);
+    const int2 tiles = key_tiles(r0, r0 + rows, a.G, lq, lk, a.window);
+    item->x = make_int4(q0, lq, k0, lk);
+    item->y = make_int4(r0, tiles.x, tiles.y, 0);
+    item->g = blockIdx.x % a.KV;
+  }
+}
+
 // TMEM (512 columns): O of the two halves, P of the two, and ONE buffer for S.
 // A softmax thread takes its whole row of S into registers at once, so the
 // buffer is free again some 100 cycles after the product is done, and the
@@ -343,6 +390,8 @@ __global__ void __launch_bounds__(384, 1)
   uint8_t* kvsm = qsm + Q_SLOTS * TILE;   // [KV_STAGES][K tile | V tile]
   __shared__ uint64_t bars[kBars];
   __shared__ uint32_t tmem_slot;
+  __shared__ RawItem s_item;
+  __shared__ int s_scan[24];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
@@ -354,6 +403,7 @@ __global__ void __launch_bounds__(384, 1)
     tmem_alloc(&tmem_slot, 512);
     tmem_relinquish();
   }
+  if (a.direct) own_item(a, &s_item, s_scan);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -361,10 +411,15 @@ __global__ void __launch_bounds__(384, 1)
   auto bar = [&](int i) { return bar0 + 8 * i; };
   auto wait = [&](int i, uint32_t parity) { return bar_wait<false>(bar0 + 8 * i, parity, a.status); };
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int n_items = a.blocks[a.batch] * a.KV;
+  const int n_items = a.direct ? 0 : a.blocks[a.batch] * a.KV;
   auto load_item = [&](int k) {
     const int idx = item_index(k);
     RawItem r{make_int4(0, 0, 0, 0), make_int4(0, 0, 0, 0), -1};
+    if (a.direct && k == 0) {
+      r.g = s_item.g;
+      r.x = s_item.x;
+      r.y = s_item.y;
+    }
     if (idx < n_items) {
       const int e = quot(idx, a.KV, a.recip_KV);
       r.g = idx - e * a.KV;
@@ -735,8 +790,10 @@ int launch(hcu_context* h, const VarlenArgs& a, const CUtensorMap& tq, const CUt
   HCU_TRY(once_per_device(attr_done, h->device, [&]() -> int {
     return check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem), op);
   }));
-  varlen_items_kernel<<<1, 1024, 0, h->stream>>>(a);
-  HCU_TRY(after_launch("hcu_prefill_varlen: items"));
+  if (!a.direct) {
+    varlen_items_kernel<<<1, 1024, 0, h->stream>>>(a);
+    HCU_TRY(after_launch("hcu_prefill_varlen: items"));
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3(384);
@@ -746,7 +803,7 @@ int launch(hcu_context* h, const VarlenArgs& a, const CUtensorMap& tq, const CUt
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // set up while the items are sorted
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = a.direct ? 0 : 1;
   return check_cuda(cudaLaunchKernelEx(&cfg, kern, tq, tk, tv, a), "hcu_prefill_varlen: launch");
 }
 
@@ -826,5 +883,6 @@ extern "C" int hcu_prefill_varlen(hcu_handle h, const hcu_prefill_varlen_params*
   HCU_TRY(map(&tq, q, a.H, a.total_q, a.q_stride, a.q_tma ? (uint32_t)a.G : 1, a.q_tma ? 128u / a.G : 1));
   int grid = (int)std::min<long long>(h->sm_count, most * a.KV);
   if (h->opt_swa_ctas > 0 && h->opt_swa_ctas < grid) grid = (int)h->opt_swa_ctas;
+  a.direct = most * a.KV <= grid && a.batch <= hcu::kDirectBatch;
   return p->dtype == HCU_DT_BF16 ? hcu::launch<true>(h, a, tq, tk, tv, grid) : hcu::launch<false>(h, a, tq, tk, tv, grid);
 }
