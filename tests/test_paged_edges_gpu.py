@@ -140,6 +140,42 @@ def test_short_contexts(backend, dtype, H, KV, Dh, S, lens):
     assert backend.device_status() == 0
 
 
+@pytest.fixture(scope="module")
+def little():
+    """A handle without room for partial sums."""
+    be = CudaBackend(0, workspace_bytes=(1 << 18) + 4096)
+    yield be
+    be.close()
+
+
+@pytest.mark.parametrize("pieces", ["line", "warps"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("H,KV,Dh,S,window,page,lens", [
+    (16, 8, 128, 1, 0, 16, [1024]),
+    (2, 2, 128, 1, 0, 16, [1, 0, 15, 16, 17, 31, 33]),
+    (8, 2, 128, 1, 0, 64, [700, 64, 1, 65, 0, 129]),
+    (8, 1, 128, 1, 100, 32, [99, 100, 101, 1500, 7]),
+    (6, 3, 128, 5, 0, 128, [300, 4, 5, 1, 0, 6]),
+    (16, 2, 256, 4, 0, 32, [333, 3, 40]),
+    (12, 2, 256, 1, 17, 16, [16, 17, 18, 900]),
+    (32, 1, 128, 3, 40, 256, [257, 39, 2]),
+    (5, 1, 128, 1, 1, 16, [1, 50])])
+def test_short_contexts_in_other_pieces(backend, little, pieces, dtype, H, KV, Dh, S, window, page, lens):
+    """Short contexts by equal pieces of a line (as long ones are), and with whole units for warps."""
+    be = backend if pieces == "line" else little
+    g = gen(H * 5 + Dh + S + sum(lens))
+    c, table, slots = paged_batch(g, lens, page, KV, Dh)
+    q = torch.randn((len(lens), S, H, Dh), generator=g, device=dev).to(dtype)
+    be.set_option("attn_chunk", 64)  # a set one keeps the call from taking clusters
+    try:
+        out = check_decode(be, c, table, slots, q, lens, window)
+    finally:
+        be.set_option("attn_chunk", 0)
+    for b, n in enumerate(lens):
+        assert (out[b, :max(0, S - n)] == 0).all()
+    assert be.device_status() == 0
+
+
 @pytest.mark.parametrize("chunk", [1, 32, 100, 4096, 2 ** 40])
 def test_chunk_option(backend, chunk):
     g = gen(4)
