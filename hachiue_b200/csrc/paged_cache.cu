@@ -81,7 +81,9 @@ __device__ __forceinline__ uint32_t q4_codes(const float (&x)[8], float d, float
 }
 
 // Quantises the eight elements of each lane: a block is four lanes.  Returns the
-// lane's codes (element 0 lowest) and the block's scale.  The whole warp calls it.
+// lane's codes (element 0 lowest) and the block's scale.  A NaN's bits are the
+// largest, so a block that holds one is found by its maximum; its scale is NaN, and
+// so is every value that it stands for.  The whole warp calls it.
 __device__ __forceinline__ uint32_t q4_block(const float (&x)[8], int lane, bool any_f32, __half* scale) {
   uint32_t top = 0;
   float m = x[0];  // the lane's first element of the lane's largest magnitude
@@ -98,10 +100,11 @@ __device__ __forceinline__ uint32_t q4_block(const float (&x)[8], int lane, bool
   const uint32_t same = __ballot_sync(0xffffffffu, top == all);
   const int first = (lane & 28) + __ffs((same >> (lane & 28)) & 0xfu) - 1;
   m = __shfl_sync(0xffffffffu, m, first);
-  const __half d = __float2half_rn(fminf(fmaxf(m * -0.125f, -65504.f), 65504.f));
+  // (the limits alone would make a NaN the lower one)
+  const __half d = __float2half_rn(all > 0x7f800000u ? m : fminf(fmaxf(m * -0.125f, -65504.f), 65504.f));
   *scale = d;
   const float df = __half2float(d);
-  if (df == 0.f) return 0x88888888u;
+  if (!(fabsf(df) > 0.f)) return 0x88888888u;  // zero or NaN
   float inv;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(df));
   return q4_codes(x, df, inv, any_f32);

@@ -68,7 +68,8 @@ extern "C" {
  * of the largest magnitude (the first of equals); its scale is
  * d = f16(m / -8), held within +-65504, the code of an element is
  * floor(x / d + 8.5) held within 0..15 (8 where d is 0), found exactly, and the
- * element then stands for (code - 8) * d. */
+ * element then stands for (code - 8) * d.  A block that holds a NaN has a NaN
+ * scale: all of its elements stand for NaN. */
 #define HCU_KV_Q4_0 5
 
 /* Element types of activations: the tensor-core prefill inputs and outputs,
