@@ -39,6 +39,7 @@
 // chunk at 56 % of the slots, of which the masks and shifts of the codes are a quarter;
 // 128 registers allow 16 warps per SM.
 #include <algorithm>
+#include <cfloat>
 
 #include "paged.cuh"
 
@@ -73,7 +74,7 @@ constexpr int NW = 8;          // warps of a CTA
 constexpr int kWarpUnits = 0, kLine = 1, kCluster = 2;
 constexpr int CHUNK = 32;      // tokens a warp takes at a time
 constexpr int kUnitCost = 3;    // chunks that a unit's queries and sums cost a warp besides its chunks
-constexpr float kNoM = -1e30f;  // M of a row that has seen no token
+constexpr float kNoM = -FLT_MAX;  // M of a row that has seen no token: below every finite score
 constexpr float kTop = 14.f, kStart = 4.f;  // weighted probabilities stay below 2^kTop; a moved M leaves the largest near 2^kStart
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
