@@ -494,7 +494,8 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC, MT)) attn_paged_ke
     __syncwarp();
     uint32_t qf[NC][MT][NB][4];
     float corr[NC][NB][NR];  // -8 sum(q) of the block (not EXACT), rows of this thread's accumulator columns 2t, 2t + 1
-    float rs[NC][NR];        // score = rs * accumulated sum
+    float rs[NC][NR];        // score = rs * (kCodes * accumulated sum): together the factors can pass f32's range
+    constexpr float kCodes = EXACT ? 1.f : 16777216.f;  // subnormal codes carry 2^-24
 #pragma unroll
     for (int nc = 0; nc < NC; nc++) {
       const int r = nc * RG + (CT == 2 ? g >> 1 : g);
@@ -509,7 +510,7 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC, MT)) attn_paged_ke
       // 2^sq brings the row's largest magnitude into [2^13, 2^14)
       const int sq = top > 0.f ? max(-126, min(127, 140 - (int)(__float_as_uint(top) >> 23))) : 0;
       const float up = __uint_as_float((uint32_t)(sq + 127) << 23);
-      const float back = ldexpf(a.scale_log2, (EXACT ? 0 : 24) - sq);
+      const float back = ldexpf(a.scale_log2, -sq);
 #pragma unroll
       for (int i = 0; i < NB; i++) {
         float sum = 0.f;
@@ -626,7 +627,7 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC, MT)) attn_paged_ke
 #pragma unroll
           for (int u = 0; u < 2; u++)
 #pragma unroll
-            for (int r = 0; r < NR; r++) x[u][nc][r] *= rs[nc][r];
+            for (int r = 0; r < NR; r++) x[u][nc][r] = x[u][nc][r] * kCodes * rs[nc][r];
         if (!whole) {
           // Tokens outside a row's range and on missing pages weigh nothing; what their rows hold is not looked at.
 #pragma unroll
@@ -765,7 +766,6 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC, MT)) attn_paged_ke
     }
 
     // ---- the segment's sums ----
-    constexpr float kUnscale = EXACT ? 1.f : 16777216.f;  // subnormal codes carry 2^-24
     const bool complete = begins && ends && a.split != kCluster;
     float* rec = ends ? buf + warp * RB * RS : reinterpret_cast<float*>(smem + warp * ST * SB);
 #pragma unroll
@@ -776,7 +776,7 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC, MT)) attn_paged_ke
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
         const int rl = nc * RG + t * NR + r;
-        const float f = complete ? (l > 0.f ? kUnscale / l : (l == 0.f ? 0.f : l)) : kUnscale;  // no token: zeros; NaN stays
+        const float f = complete ? (l > 0.f ? kCodes / l : (l == 0.f ? 0.f : l)) : kCodes;  // no token: zeros; NaN stays
         float* w = rec + rl * RS;
 #pragma unroll
         for (int i = 0; i < NB; i++) {  // dimensions 32i + 4g .. + 3

@@ -86,3 +86,22 @@ def test_negative_scores_alone(backend, little, H, Dh, S):
                     # weights of 2^-11 (bf16, more than four rows) or 2^-22, the sum of n tokens and the division
                     step = 2.0 ** -11 if dtype == torch.bfloat16 and S * H > 4 else 2.0 ** -18
                     assert ((out[b, s].double() - mean).abs() <= step * size + 1.01 * ref.HALF_STEP[dtype] * mean.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("H", [2, 8, 12])
+def test_largest_queries(backend, dtype, H):
+    """Queries of 2^126 over the smallest scales that f16 holds: finite scores, the largest take all."""
+    g = gen(H + 1)
+    c, table, slots = paged_batch(g, [90], 16, 1, 128)
+    page, off = slots[0] // 16, slots[0] % 16
+    c.k_scale[page, :, off] = torch.randint(1, 6, (90, 1, 4), generator=g, device=dev).half() * 2.0 ** -24
+    q = torch.zeros((1, 1, H, 128), device=dev)
+    q[..., 3] = 2.0 ** 126
+    q = q.to(dtype)
+    out = torch.empty_like(q)
+    backend.attention_paged(q, c, out, table, i32([90]))
+    x = ref.cache_rows(c, slots[0], "k")[:, 0, 3]
+    v = ref.cache_rows(c, slots[0], "v")[:, 0][x == x.max()]
+    bound = ref.HALF_STEP[dtype] * 1.01 * v.mean(0).abs() + (2.0 ** -11 if dtype == torch.bfloat16 else 2.0 ** -20) * v.abs().mean(0)
+    assert ((out[0, 0].double() - v.mean(0)).abs() <= bound).all()
