@@ -25,10 +25,14 @@
 //    for up to four rows.  bf16 calls with more rows use one f16 number, whose
 //    rounding (2^-11) stays below the result's own.  Queries are scaled by a power
 //    of two per row, so bf16 and f32 exponents fit f16.
-//  * Softmax: log2 domain, one pass, per warp.  The reference point M of a row
-//    takes in the exponent of the token's largest value scale, so that the
-//    weighted probabilities stay within f16's range whatever the scales are; it
-//    moves only when one would pass 2^14.
+//  * Softmax: log2 domain, one pass, per warp, p = 2^(x - M) with a whole number M
+//    for each row.  The weighted probabilities of a row and block of 32 dimensions
+//    are held times a power of two E of their own, so that the largest lies between
+//    2^8 and 2^15 whatever the scales of other blocks and of tokens without weight
+//    are: one below 2^-22 of the largest loses bits (f16's smallest number is 2^-24).
+//    (With one exponent for all blocks, that of the largest scale, values 2^-18 of
+//    another block's were off by 1e-4.)  M and the E move only when a number would
+//    pass 2^15.
 //
 // The work is cut by chunks of 32 tokens, not by sequences: see PagedPlan.  A
 // warp fetches its chunks into a ring of its own, two ahead, and never waits for
@@ -75,7 +79,8 @@ constexpr int kWarpUnits = 0, kLine = 1, kCluster = 2;
 constexpr int CHUNK = 32;      // tokens a warp takes at a time
 constexpr int kUnitCost = 3;    // chunks that a unit's queries and sums cost a warp besides its chunks
 constexpr float kNoM = -FLT_MAX;  // M of a row that has seen no token: below every finite score
-constexpr float kTop = 14.f, kStart = 4.f;  // weighted probabilities stay below 2^kTop; a moved M leaves the largest near 2^kStart
+constexpr int kTop = 15, kStart = 8;  // weighted probabilities stay below 2^kTop; a moved E leaves the largest near 2^kStart
+constexpr uint32_t kMostE = 253;      // exponent bits of the largest E, 2^126: that of a block without a weight
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -100,6 +105,16 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
 
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+
+// 2^n for n up to 127; 0 below 2^-126.
+__device__ __forceinline__ float pow2(int n) { return __uint_as_float((uint32_t)max(n + 127, 0) << 23); }
+
+// max(a, |b|, |c|); a NaN counts for nothing.
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(fabsf(b)), "f"(fabsf(c)));
+  return d;
+}
 
 // Adds a part's sums v and (reference point, sum of weights) to a row's.
 __device__ __forceinline__ void add_part(float& m, float& l, float (&o)[4], float2 ml, float4 v) {
@@ -193,7 +208,8 @@ constexpr int paged_row_floats(int dh) { return dh + 4; }  // of the warps' sums
 constexpr size_t paged_smem(int dh, int rb) {
   return (size_t)NW * STAGES * paged_stage_bytes(dh) + (size_t)NW * rb * paged_row_floats(dh) * 4;
 }
-constexpr int paged_ctas(int dh, int nc, int mt) { return dh == 128 && nc == 1 && mt == 1 ? 2 : 1; }  // per SM
+// Per SM.  One row per thread fits 128 registers; two (bf16, eight rows) do not: two CTAs 67 us, one 59 (32 sequences, 64 / 8 heads).
+constexpr int paged_ctas(int dh, int ct) { return dh == 128 && ct == 2 ? 2 : 1; }
 
 // The work of a call is a line of chunks: sequence after sequence, in each
 // its KV heads, in each its row blocks, in each the chunks that hold visible tokens
@@ -230,7 +246,7 @@ __device__ __forceinline__ int2 paged_chunks(const PagedAttnArgs& a, int b) {
 // additions truncate: over 8192 tokens that came to 7e-6 of the result.
 // Otherwise the codes as they are, the offset taken off the sums.
 template <int DH, int CT, int MT, int NC, bool EXACT>
-__global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC, MT)) attn_paged_kernel(const PagedAttnArgs a) {
+__global__ void __launch_bounds__(32 * NW, paged_ctas(DH, CT)) attn_paged_kernel(const PagedAttnArgs a) {
   constexpr int NB = DH / 32, ST = STAGES, SB = paged_stage_bytes(DH);
   constexpr int RG = 8 / CT, RB = RG * NC;      // rows per column group, per warp
   constexpr int NR = 2 / CT;                   // rows per thread and column group
@@ -549,12 +565,15 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC, MT)) attn_paged_ke
     stage ^= 1;
 
     float O[2 * NB][NC][4] = {};
-    float M[NC][NR], L[NC][NR], T[NC][NR];  // T: the score above which M has to move
-    float cap = 0.f, cap_log2 = -25.f;      // every value scale so far is at most cap <= 2^cap_log2
+    float M[NC][NR], L[NC][NR], E[NC][NR][NB];
 #pragma unroll
     for (int nc = 0; nc < NC; nc++)
 #pragma unroll
-      for (int r = 0; r < NR; r++) M[nc][r] = T[nc][r] = kNoM, L[nc][r] = 0.f;
+      for (int r = 0; r < NR; r++) {
+        M[nc][r] = kNoM, L[nc][r] = 0.f;
+#pragma unroll
+        for (int i = 0; i < NB; i++) E[nc][r][i] = __uint_as_float(kMostE << 23);
+      }
 
     for (int c = sg.c0; c < c1; c++) {
       copy_wait<ST - 1>();
@@ -649,54 +668,78 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC, MT)) attn_paged_ke
               for (int i = 0; i < NB / 2; i++) vsw[u][i] = 0u;
           }
         }
-        // ---- reference points: they move when a weighted probability could pass 2^kTop ----
-        __half2 vtop = __habs2(bits_h2(vsw[0][0]));
+        // ---- probabilities, and weighted by the blocks' value scales ----
+        float p[NC][2][NR] = {};
+        auto weight = [&](int nc, int u, int r, int i2) {  // of two blocks, without E
+          const float2 v = f16x2_to_f2(vsw[u][i2]);
+          return f2_mul(f2(v.x, v.y), f2(p[nc][u][r], p[nc][u][r]));
+        };
+        uint64_t w[NC][2][NR][NB / 2];
+        auto weigh = [&]() {
+          float most = 0.f;
 #pragma unroll
-        for (int i = 1; i < NB; i++) vtop = __hmax2(vtop, __habs2(bits_h2(vsw[i / (NB / 2)][i % (NB / 2)])));
-        const float vmax = fmaxf(__low2float(vtop), __high2float(vtop));
-        bool grow = vmax > cap;
+          for (int nc = 0; nc < NC; nc++)
 #pragma unroll
-        for (int nc = 0; nc < NC; nc++)
+            for (int u = 0; u < 2; u++)
 #pragma unroll
-          for (int r = 0; r < NR; r++)
-            grow = grow || fmaxf(x[0][nc][r], x[1][nc][r]) > T[nc][r];
-        if (__any_sync(0xffffffffu, grow)) {
-          const float top = warp_max(vmax);
-          if (top > cap) {  // the next power of two
-            cap_log2 = (float)((int)(__float_as_uint(top) >> 23) - 126);
-            cap = exp2f(cap_log2);
-          }
+              for (int r = 0; r < NR; r++) {
+                p[nc][u][r] = ex2_approx(x[u][nc][r] - M[nc][r]);
+                most = fmaxf(most, p[nc][u][r]);
 #pragma unroll
-          for (int nc = 0; nc < NC; nc++) {
-            float f[NR];
+                for (int i2 = 0; i2 < NB / 2; i2++) {
+                  w[nc][u][r][i2] = f2_mul(weight(nc, u, r, i2), f2(E[nc][r][2 * i2], E[nc][r][2 * i2 + 1]));
+                  float w0, w1;
+                  f2_get(w[nc][u][r][i2], w0, w1);
+                  most = max_abs(most, w0, w1);
+                }
+              }
+          return most;
+        };
+        if (__any_sync(0xffffffffu, weigh() > (float)(1 << kTop))) {
+#pragma unroll
+          for (int nc = 0; nc < NC; nc++)
 #pragma unroll
             for (int r = 0; r < NR; r++) {
-              float w = fmaxf(x[0][nc][r], x[1][nc][r]);
+              float m = fmaxf(x[0][nc][r], x[1][nc][r]);
 #pragma unroll
-              for (int o = 4; o < 32; o <<= 1) w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, o));
-              const float m = w + cap_log2 > M[nc][r] + kTop ? w + cap_log2 - kStart : M[nc][r];
-              f[r] = exp2f(M[nc][r] - m);
+              for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+              m = fmaxf(M[nc][r], ceilf(m));
+              const int n = (int)fminf(m - M[nc][r], 300.f);  // whole: M moves by multiplying every E by 2^n, the sums stay
               M[nc][r] = m;
-              T[nc][r] = m + kTop - cap_log2;
-              L[nc][r] *= f[r];
+              L[nc][r] *= pow2(-n);
+#pragma unroll
+              for (int u = 0; u < 2; u++) p[nc][u][r] = ex2_approx(x[u][nc][r] - m);
+#pragma unroll
+              for (int i2 = 0; i2 < NB / 2; i2++) {
+                float a0, a1, b0, b1;
+                f2_get(weight(nc, 0, r, i2), a0, a1);
+                f2_get(weight(nc, 1, r, i2), b0, b1);
+                // the largest weights of both blocks, by their upper 16 bits
+                uint32_t top = __byte_perm(__float_as_uint(fmaxf(fabsf(a0), fabsf(b0))), __float_as_uint(fmaxf(fabsf(a1), fabsf(b1))), 0x7632u);
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                  const int i = 2 * i2 + e, big = (int)(top >> (16 * e + 7)) & 0xff;  // exponent bits
+                  const int old = (int)(__float_as_uint(E[nc][r][i]) >> 23) + n;
+                  const int now = min(min(old, (int)kMostE), 254 + kStart - big);  // the largest becomes 2^kStart, unless it is less
+                  E[nc][r][i] = __uint_as_float((uint32_t)now << 23);
+                  const float f = pow2(now - old);
+#pragma unroll
+                  for (int k = 0; k < 4; k++)
+                    if (NR == 1 || (k & 1) == r) O[2 * i][nc][k] *= f, O[2 * i + 1][nc][k] *= f;
+                }
+              }
             }
-#pragma unroll
-            for (int i = 0; i < 2 * NB; i++)
-#pragma unroll
-              for (int k = 0; k < 4; k++) O[i][nc][k] *= f[NR == 2 ? (k & 1) : 0];
-          }
+          weigh();
         }
-        // ---- weighted probabilities, values ----
-        float p[NC][2][NR];
 #pragma unroll
         for (int nc = 0; nc < NC; nc++)
 #pragma unroll
           for (int u = 0; u < 2; u++)
 #pragma unroll
-            for (int r = 0; r < NR; r++) {
-              p[nc][u][r] = ex2_approx(x[u][nc][r] - M[nc][r]);
-              L[nc][r] += p[nc][u][r];
-            }
+            for (int r = 0; r < NR; r++) L[nc][r] += p[nc][u][r];
+        // ---- values ----
         uint32_t vw[4][NB / 2];  // tokens t, t + 4, t + 8, t + 12: halfwords of the lane's dimensions
 #pragma unroll
         for (int k = 0; k < 4; k++) lds_words<NB / 2>(st + KB + (16 * j + t + 4 * k) * (DH / 2) + g * NB * 2, vw[k]);
@@ -705,18 +748,16 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC, MT)) attn_paged_ke
           uint32_t pb[2][NC][MT][2];  // [block] B fragments: tokens in pairs, column g
 #pragma unroll
           for (int u = 0; u < 2; u++) {
-            const float2 v = f16x2_to_f2(vsw[u][i2]);
 #pragma unroll
             for (int nc = 0; nc < NC; nc++) {
               float y[NR][2], l[NR][2];  // a weighted probability's first f16 number (exact in f32) and what is left
 #pragma unroll
               for (int r = 0; r < NR; r++) {
-                const uint64_t w = f2_mul(f2(v.x, v.y), f2(p[nc][u][r], p[nc][u][r]));
-                f2_get(w, y[r][0], y[r][1]);
+                f2_get(w[nc][u][r][i2], y[r][0], y[r][1]);
                 if (WIDE) {
                   y[r][0] = __uint_as_float(__float_as_uint(y[r][0]) & 0xffffe000u);
                   y[r][1] = __uint_as_float(__float_as_uint(y[r][1]) & 0xffffe000u);
-                  f2_get(f2_fma(f2(y[r][0], y[r][1]), f2(-1.f, -1.f), w), l[r][0], l[r][1]);
+                  f2_get(f2_fma(f2(y[r][0], y[r][1]), f2(-1.f, -1.f), w[nc][u][r][i2]), l[r][0], l[r][1]);
                 }
               }
 #pragma unroll
@@ -777,15 +818,16 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC, MT)) attn_paged_ke
         for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
         const int rl = nc * RG + t * NR + r;
         const float f = complete ? (l > 0.f ? kCodes / l : (l == 0.f ? 0.f : l)) : kCodes;  // no token: zeros; NaN stays
-        float* w = rec + rl * RS;
+        float* row = rec + rl * RS;
 #pragma unroll
         for (int i = 0; i < NB; i++) {  // dimensions 32i + 4g .. + 3
           const float *o0 = O[2 * i][nc], *o1 = O[2 * i + 1][nc];
           float4 v;
-          v.x = (CT == 2 ? o0[0] + o0[1] : o0[r]) * f;
-          v.y = (CT == 2 ? o0[2] + o0[3] : o0[2 + r]) * (0.0625f * f);
-          v.z = (CT == 2 ? o1[0] + o1[1] : o1[r]) * f;
-          v.w = (CT == 2 ? o1[2] + o1[3] : o1[2 + r]) * (0.0625f * f);
+          const float fe = f * __uint_as_float((254u << 23) - __float_as_uint(E[nc][r][i]));  // f / E
+          v.x = (CT == 2 ? o0[0] + o0[1] : o0[r]) * fe;
+          v.y = (CT == 2 ? o0[2] + o0[3] : o0[2 + r]) * (0.0625f * fe);
+          v.z = (CT == 2 ? o1[0] + o1[1] : o1[r]) * fe;
+          v.w = (CT == 2 ? o1[2] + o1[3] : o1[2 + r]) * (0.0625f * fe);
           if (complete) {
             if (rl < rows) {
               const int rr = r0 + rl, s = rr / a.G, h = kvh * a.G + rr % a.G;
@@ -793,10 +835,10 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, NC, MT)) attn_paged_ke
               store4_dt(a.out, (((size_t)b * a.S + s) * a.H + h) * DH + 32 * i + 4 * g, a.dtype, y);
             }
           } else {
-            *reinterpret_cast<float4*>(w + 32 * i + 4 * g) = v;
+            *reinterpret_cast<float4*>(row + 32 * i + 4 * g) = v;
           }
         }
-        if (!complete && g == 0) w[DH] = M[nc][r], w[DH + 1] = l;
+        if (!complete && g == 0) row[DH] = M[nc][r], row[DH + 1] = l;
       }
     if (!complete && lane == 0) {
       auto& i = s_rec[2 * warp + (ends ? 0 : 1)];
@@ -968,7 +1010,7 @@ int launch(hcu_context* h, PagedAttnArgs a) {
   a.nrb = (a.R + RB - 1) / RB;
   const long long units = (long long)a.batch * a.kv.KV * a.nrb;
   if (units > 0x7fffffffLL) return fail(HCU_EINVAL, "%s: batch x KV x query row blocks too large", op);
-  long long grid = std::min(kMaxParts, h->sm_count * paged_ctas(DH, NC, MT));
+  long long grid = std::min(kMaxParts, h->sm_count * paged_ctas(DH, CT));
   // The line must not pass 2^31 and the records must fit the workspace (behind the other ops' tickets).
   const size_t room = h->workspace_bytes > kTicketBytes ? h->workspace_bytes - kTicketBytes : 0;
   const long long span = a.window > 0 ? std::min<long long>(a.max_context, (long long)a.window + a.S + CHUNK) : a.max_context;

@@ -614,8 +614,11 @@ int hcu_read_paged(hcu_handle h, uint32_t n, uint32_t dtype, const int64_t *slot
  * with it); a longer sequence sets bit 2 of the device status and its outputs
  * are zeros.  A page index outside the cache sets bit 2 too and that page's
  * tokens are left out; only the pages that hold visible tokens are looked up.
- * f32 outputs keep f32 accuracy; bf16 and f16 ones are rounded once, and bf16
- * calls with S * H / KV above 4 hold queries and weighted probabilities in f16. */
+ * f32 calls hold queries and weighted probabilities in 22 bits and sum in f32,
+ * whatever the scales of other blocks and tokens are: an element's error is that
+ * of f32 arithmetic on the values of its block of 32 dimensions.  bf16 and f16
+ * results are rounded once, and bf16 calls with S * H / KV above 4 hold queries
+ * and weighted probabilities in f16. */
 typedef struct {
   uint32_t batch, S, H, windowSize, dtype, max_context;
   uint32_t table_stride;      /* block_table entries per sequence */

@@ -1,10 +1,11 @@
-"""The decode over the 4-bit pages where its numbers are far apart."""
+"""The decode over the 4-bit pages where its numbers are far apart: scores and queries near the ends of f32, value scales that
+differ between the blocks of a row and between tokens."""
 import pytest
 import torch
 
 from hachiue_b200 import CudaBackend
 from tests import paged_reference as ref
-from tests.test_paged_gpu import dev, gen, paged_batch
+from tests.test_paged_gpu import DTYPES, dev, gen, paged_batch
 
 pytestmark = pytest.mark.gpu
 
@@ -30,6 +31,38 @@ def runs(backend, little):
     finally:
         backend.set_option("attn_chunk", 0)
     yield little
+
+
+def check(be, c, table, slots, q, lens, window=0, without=None, blocks=False):
+    """As check_decode, with the step of f16's smallest numbers; token `without` has no weight, so that its own score's
+    error says nothing about the others'.
+
+    `blocks`: an element is held to the size of its block, sum_j p_j 8 |d_j|, not to its own, sum_j p_j |v_j|.  Where the
+    token that takes nearly all has code 8 (a zero) the second one is the sum of the others alone, which the arithmetic does
+    not resolve to 22 bits: a weight w is two f16 numbers, off by 2^-22 w or, below 2^-2, by up to 2^-24, and the largest
+    weight W of the row and block is at least 2^8: T weights are off by at most T 2^-32 W (times 8, their largest code),
+    below the T / 16 steps of 2^-24 of the bound.  16-bit calls add codes and their offset inside the tensor cores, of which
+    each sum of 16 tokens truncates twice, by 2^-23 of at most 15 / 8 of the block's size: T / 16 * 7.5 steps, below the
+    2 (D + 8) mag steps of a bound whose scores reach 40."""
+    out = torch.full_like(q, float("nan"))
+    be.attention_paged(q, c, out, table, i32(lens), window_size=window)
+    S, D = q.shape[1], q.shape[3]
+    for b, n in enumerate(lens):
+        k, v = (ref.cache_rows(c, slots[b], w) for w in "kv")
+        want, spread, mag = ref.attend(q[b].double(), k, v, n - S, window)
+        if blocks:
+            page, off = slots[b] // c.page_size, slots[b] % c.page_size
+            size = 8 * c.v_scale[page, :, off].double().abs().repeat_interleave(32, -1)
+            spread = ref.attend(q[b].double(), k, size, n - S, window)[0]
+            assert n / 16 * 7.5 < 2 * (D + 8) * float(mag.min())
+        if without is not None:
+            k[without] = 0
+            mag = ref.attend(q[b].double(), k, v, n - S, window)[2]
+        rows = S * q.shape[2] // c.kv_heads
+        p_step = 2.0 ** -11 if q.dtype == torch.bfloat16 and rows > 4 else 2.0 ** -22
+        bound = ref.attention_bound(want, spread, mag, D, n, q.dtype, p_step) + (2.0 ** -25 if q.dtype == torch.float16 else 0)
+        err = (out[b].double() - want).abs()
+        assert (err <= bound).all(), (b, n, float((err / bound).max()), float(err.max()))
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -105,3 +138,67 @@ def test_largest_queries(backend, dtype, H):
     v = ref.cache_rows(c, slots[0], "v")[:, 0][x == x.max()]
     bound = ref.HALF_STEP[dtype] * 1.01 * v.mean(0).abs() + (2.0 ** -11 if dtype == torch.bfloat16 else 2.0 ** -20) * v.abs().mean(0)
     assert ((out[0, 0].double() - v.mean(0)).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,KV,Dh,S", [(4, 2, 128, 1), (16, 2, 128, 1), (24, 2, 128, 1), (6, 2, 256, 1), (16, 2, 256, 2)])
+@pytest.mark.parametrize("apart", [10, 18, 24])
+def test_value_scales_of_blocks(backend, little, dtype, H, KV, Dh, S, apart):
+    """One block of every value row is 2^apart times as large as the others, another 2^-8 of those: each block's results
+    keep the accuracy of their own size."""
+    g = gen(H + Dh + apart)
+    lens = [900, 33, 1]
+    c, table, slots = paged_batch(g, lens, 32, KV, Dh)
+    every = torch.cat(slots)
+    page, off = every // 32, every % 32
+    size = torch.full((Dh // 32,), 2.0 ** (8 - apart), device=dev)
+    size[1], size[2] = 2.0 ** 8, 2.0 ** -apart
+    c.v_scale[page, :, off] = ((torch.rand((len(every), KV, Dh // 32), generator=g, device=dev) + 0.5) * size).half()
+    q = torch.randn((3, S, H, Dh), generator=g, device=dev).to(dtype)
+    for be in runs(backend, little):
+        check(be, c, table, slots, q, lens)
+        check(be, c, table, slots, q, lens, 100)
+    assert backend.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,KV,Dh", [(4, 2, 128), (16, 2, 128), (24, 2, 128), (6, 2, 256), (16, 2, 256)])
+@pytest.mark.parametrize("at", [0, 17, 450, 899])
+@pytest.mark.parametrize("blocks", [slice(None), 1], ids=["all", "one"])
+def test_a_large_token_of_no_weight(backend, little, dtype, H, KV, Dh, at, blocks):
+    """A token whose values (all, or those of one block) are 2^27 times the others' has a probability near 2^-50: it adds
+    nothing, wherever it lies, and takes nothing from the accuracy of the rest."""
+    g = gen(H + Dh + at)
+    lens = [900]
+    c, table, slots = paged_batch(g, lens, 32, KV, Dh)
+    page, off = slots[0] // 32, slots[0] % 32
+    c.v_scale[page, :, off] = ((torch.rand((900, KV, Dh // 32), generator=g, device=dev) + 0.5) * 2.0 ** -12).half()
+    c.v_scale[page[at], :, off[at], blocks] = 2.0 ** 15
+    k = ref.cache_rows(c, slots[0], "k")
+    G = H // KV
+    q = torch.empty((1, 1, H, Dh), device=dev)
+    for h in range(H):  # a score near -35 with that token, and a random one with the others
+        u = k[at, h // G].float()
+        q[0, 0, h] = torch.randn(Dh, generator=g, device=dev) * 0.3 - 35 * Dh ** 0.5 * u / (u * u).sum()
+    for be in runs(backend, little):
+        check(be, c, table, slots, q.to(dtype), lens, without=at)
+    assert backend.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,KV,Dh", [(4, 2, 128), (16, 2, 128), (24, 2, 128), (16, 2, 256)])
+def test_scales_and_scores_that_grow(backend, little, dtype, H, KV, Dh):
+    """Scores and value scales that grow along the context, each block's at its own pace, so that references move often."""
+    g = gen(H + Dh + 5)
+    n = 1500
+    c, table, slots = paged_batch(g, [n], 32, KV, Dh)
+    page, off = slots[0] // 32, slots[0] % 32
+    t = torch.arange(n, device=dev)[:, None, None] / n
+    pace = torch.linspace(-20, 20, Dh // 32, device=dev)
+    c.v_scale[page, :, off] = torch.exp2(pace * t - 10 - pace.clamp_min(0) / 2).expand(-1, KV, -1).half()
+    c.k_scale[page, :, off] = (c.k_scale[page, :, off].float() * (0.1 + 4 * t)).half()
+    q = torch.randn((1, 1, H, Dh), generator=g, device=dev)
+    q[0, 0, 1:] += ref.cache_rows(c, slots[0], "k")[n - 1, 0].float() * 0.3
+    for be in runs(backend, little):
+        check(be, c, table, slots, q.to(dtype), [n], blocks=True)
+    assert backend.device_status() == 0
