@@ -693,6 +693,16 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, CT)) attn_paged_kernel
                   most = max_abs(most, w0, w1);
                 }
               }
+          // A token that one of the thread's rows sees and another does not: its scale, which may be NaN, is the first one's alone.
+          if (NR * NC > 1 && !whole)
+#pragma unroll
+            for (int nc = 0; nc < NC; nc++)
+#pragma unroll
+              for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int r = 0; r < NR; r++)
+#pragma unroll
+                  for (int i2 = 0; i2 < NB / 2; i2++) w[nc][u][r][i2] = x[u][nc][r] == -INFINITY ? 0 : w[nc][u][r][i2];
           return most;
         };
         if (__any_sync(0xffffffffu, weigh() > (float)(1 << kTop))) {
@@ -712,8 +722,8 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, CT)) attn_paged_kernel
 #pragma unroll
               for (int i2 = 0; i2 < NB / 2; i2++) {
                 float a0, a1, b0, b1;
-                f2_get(weight(nc, 0, r, i2), a0, a1);
-                f2_get(weight(nc, 1, r, i2), b0, b1);
+                f2_get(x[0][nc][r] == -INFINITY ? 0 : weight(nc, 0, r, i2), a0, a1);
+                f2_get(x[1][nc][r] == -INFINITY ? 0 : weight(nc, 1, r, i2), b0, b1);
                 // the largest weights of both blocks, by their upper 16 bits
                 uint32_t top = __byte_perm(__float_as_uint(fmaxf(fabsf(a0), fabsf(b0))), __float_as_uint(fmaxf(fabsf(a1), fabsf(b1))), 0x7632u);
 #pragma unroll

@@ -60,3 +60,41 @@ def test_append_keeps_nan(backend, dtype, Dh, rotary, n):
     assert nan[:2].all()  # a NaN key of their head
     assert torch.equal(nan[2:], (bad_v[0, 1] | bad_v[n - 1, 1]).repeat_interleave(32, -1).expand(2, -1))
     assert backend.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,KV,Dh,S,n", [(2, 2, 128, 2, 40), (8, 2, 128, 2, 300), (8, 1, 128, 4, 100), (2, 2, 128, 8, 70), (6, 2, 128, 3, 50), (16, 2, 256, 4, 333),
+                                         (3, 1, 256, 5, 2500)])
+@pytest.mark.parametrize("window", [0, 20])
+def test_a_draft_that_is_nan(backend, dtype, H, KV, Dh, S, n, window):
+    """The last drafted token's key or value row is NaN: the drafts before it do not see it, and with a window the ones
+    behind a NaN row do not either."""
+    g = gen(H + Dh + S + n + window)
+    pages = -(-n // 16)
+    c = PagedKVCache.allocate(pages, 16, KV, Dh)
+    k, v = (torch.randn((n, KV, Dh), generator=g, device=dev) for _ in range(2))
+    slots = torch.arange(n, device=dev)
+    q = torch.randn((1, S, H, Dh), generator=g, device=dev).to(dtype)
+    table, ctx = torch.arange(pages, device=dev, dtype=torch.int32)[None], torch.tensor([n], dtype=torch.int32, device=dev)
+    clean, out = torch.empty_like(q), torch.empty_like(q)
+    backend.rope_append_paged(k, v, c, slots)
+    backend.attention_paged(q, c, clean, table, ctx, window_size=window)
+    at = [n - 1] if not window else [n - 1, n - window - 1]  # the first query's window begins at n - S + 1 - window
+    saved = snapshot(c)
+    for scales in ("v_scale", "k_scale"):
+        rows = getattr(c, scales)
+        for i in at:
+            rows[i // 16, :, i % 16, 1 if scales == "v_scale" else 0] = float("nan")
+        backend.attention_paged(q, c, out, table, ctx, window_size=window)
+        for s in range(S):
+            pos = n - S + s
+            sees = [i for i in at if i <= pos and (not window or i > pos - window)]
+            nan = torch.isnan(out[0, s])
+            if not sees:
+                assert torch.equal(out[0, s], clean[0, s]), (scales, s)
+            elif scales == "v_scale":
+                assert nan[:, 32:64].all() and not nan[:, :32].any() and not nan[:, 64:].any(), s
+            else:
+                assert nan.all(), s
+        rows.copy_(saved[scales])
+    assert backend.device_status() == 0
