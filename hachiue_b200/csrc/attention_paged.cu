@@ -395,12 +395,13 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, CT)) attn_paged_kernel
     f_lo = a.window > 0 ? max(0, ctx - a.S + 1 - a.window) : 0;
     f_table = a.table + (size_t)f.b * a.table_stride;
   };
-  // The pages of chunk c's two halves of 16 tokens: -2 where no query sees a token of the half (not looked up).
+  // The pages of chunk c's two halves of 16 tokens: -2 where no query sees a token of the half (not looked up), -1 for
+  // every negative entry.
   auto look_up = [&](int c, int (&pg)[2]) {
 #pragma unroll
     for (int p = 0; p < 2; p++) {
       const int t0 = c * CHUNK + 16 * p;
-      pg[p] = c < f.c1 && t0 < f_hi && t0 + 16 > f_lo ? f_table[t0 >> a.kv.page_log2] : -2;
+      pg[p] = c < f.c1 && t0 < f_hi && t0 + 16 > f_lo ? max(f_table[t0 >> a.kv.page_log2], -1) : -2;
     }
   };
   int f_page[2] = {-2, -2};

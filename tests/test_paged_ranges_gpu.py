@@ -5,7 +5,7 @@ import torch
 
 from hachiue_b200 import CudaBackend
 from tests import paged_reference as ref
-from tests.test_paged_gpu import DTYPES, dev, gen, paged_batch
+from tests.test_paged_gpu import DTYPES, check_decode, dev, gen, paged_batch
 
 pytestmark = pytest.mark.gpu
 
@@ -202,3 +202,16 @@ def test_scales_and_scores_that_grow(backend, little, dtype, H, KV, Dh):
     for be in runs(backend, little):
         check(be, c, table, slots, q.to(dtype), [n], blocks=True)
     assert backend.device_status() == 0
+
+
+@pytest.mark.parametrize("bad", [-1, -2, -3, -(2 ** 31), 2 ** 31 - 1])
+@pytest.mark.parametrize("page", [16, 64])
+def test_every_bad_page_is_reported(backend, bad, page):
+    g = gen(page)
+    c, table, slots = paged_batch(g, [200], page, 2, 128)
+    q = torch.randn((1, 1, 4, 128), generator=g, device=dev)
+    table[0, 1] = bad
+    missing = torch.zeros(200, dtype=torch.bool, device=dev)
+    missing[page:2 * page] = True
+    check_decode(backend, c, table, slots, q, [200], 0, missing=[missing])
+    assert backend.device_status() == 2
