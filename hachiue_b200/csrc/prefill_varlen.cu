@@ -852,7 +852,8 @@ extern "C" int hcu_prefill_varlen(hcu_handle h, const hcu_prefill_varlen_params*
   a.H = (int)p->H;
   a.KV = (int)p->KV;
   a.G = a.H / a.KV;
-  a.window = (int)p->window;
+  // A window as long as the longest sequence hides nothing (and the first key's index minus a larger one could pass 2^31).
+  a.window = p->window >= p->total_k ? 0 : (int)p->window;
   a.recip_G = (uint32_t)std::min<uint64_t>(0xffffffffull, (1ull << 32) / a.G + 1);
   a.recip_KV = (uint32_t)std::min<uint64_t>(0xffffffffull, (1ull << 32) / a.KV + 1);
   a.total_q = (int)p->total_q;
