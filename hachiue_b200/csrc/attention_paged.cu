@@ -229,12 +229,15 @@ struct PagedPlan {
   }
 };
 
+// First token that a query at position pos sees (pos may be negative: pos + 1 - window could then pass int's range).
+__device__ __forceinline__ int first_seen(int pos, int window) { return window > 0 && pos >= window ? pos + 1 - window : 0; }
+
 // Chunk range of sequence b over all its queries: first chunk, count (at least 1).
 __device__ __forceinline__ int2 paged_chunks(const PagedAttnArgs& a, int b) {
   int ctx = a.context[b];
   if (ctx > a.max_context || ctx < 0) ctx = 0;
   const int first = ctx - a.S;
-  const int lo = a.window > 0 ? max(0, first + 1 - a.window) : 0;
+  const int lo = first_seen(first, a.window);
   const int c_lo = lo / CHUNK, c_hi = (ctx + CHUNK - 1) / CHUNK;
   return make_int2(c_lo, max(1, c_hi - c_lo));
 }
@@ -392,7 +395,7 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, CT)) attn_paged_kernel
     int ctx = a.context[f.b];
     if (ctx > a.max_context || ctx < 0) ctx = 0;
     f_hi = ctx;
-    f_lo = a.window > 0 ? max(0, ctx - a.S + 1 - a.window) : 0;
+    f_lo = first_seen(ctx - a.S, a.window);
     f_table = a.table + (size_t)f.b * a.table_stride;
   };
   // The pages of chunk c's two halves of 16 tokens: -2 where no query sees a token of the half (not looked up), -1 for
@@ -505,7 +508,7 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, CT)) attn_paged_kernel
     }
     // The tokens that every row of this block sees: [lo_all, hi_all).
     const int pos_first = ctx - a.S + r0 / a.G, pos_last = ctx - a.S + (r0 + rows - 1) / a.G;
-    const int lo_all = a.window > 0 ? max(0, pos_last + 1 - a.window) : 0, hi_all = max(0, pos_first + 1);
+    const int lo_all = first_seen(pos_last, a.window), hi_all = max(0, pos_first + 1);
     // ---- query columns: column g of group nc is row / term of this lane's B fragments ----
     copy_wait<ST - 1>();
     __syncwarp();
@@ -660,7 +663,7 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, CT)) attn_paged_kernel
 #pragma unroll
               for (int r = 0; r < NR; r++) {
                 const int rl = nc * RG + t * NR + r, p = ctx - a.S + (r0 + rl) / a.G;
-                const bool see = data && rl < rows && at <= p && (a.window == 0 || at > p - a.window);
+                const bool see = data && rl < rows && at <= p && at >= first_seen(p, a.window);
                 x[u][nc][r] = see ? x[u][nc][r] : -INFINITY;
                 any = any || see;
               }

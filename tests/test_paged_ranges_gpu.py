@@ -215,3 +215,25 @@ def test_every_bad_page_is_reported(backend, bad, page):
     missing[page:2 * page] = True
     check_decode(backend, c, table, slots, q, [200], 0, missing=[missing])
     assert backend.device_status() == 2
+
+
+@pytest.mark.parametrize("window", [0, 2 ** 31 - 500, 2 ** 31 - 257, 2 ** 31 - 1])
+def test_windows_near_the_largest_context(backend, window):
+    """A table of 2^31 - 256 tokens a row (its one page again and again), whose sequences hold fewer tokens than the call has
+    queries: a window near 2^31 hides nothing, and what there is is seen."""
+    g = gen(window % 97)
+    S, page = 700, 256
+    c, table, slots = paged_batch(g, [200, 256], page, 1, 128, spare=0)
+    wide = table[:, :1].expand(2, 2 ** 31 // page - 1).contiguous()
+    q = torch.randn((2, S, 2, 128), generator=g, device=dev)
+    out = torch.full_like(q, float("nan"))
+    backend.attention_paged(q, c, out, wide, i32([200, 256]), 2 ** 31 - 256, window)
+    plain = torch.full_like(q, float("nan"))
+    backend.attention_paged(q, c, plain, table, i32([200, 256]))
+    assert backend.device_status() == 0
+    for b, n in enumerate((200, 256)):
+        assert (out[b, :S - n] == 0).all()
+        k, v = (ref.cache_rows(c, slots[b], w) for w in "kv")
+        want, spread, mag = ref.attend(q[b].double(), k, v, n - S)
+        for got in (out, plain):
+            assert ((got[b].double() - want).abs() <= ref.attention_bound(want, spread, mag, 128, n, torch.float32)).all()
