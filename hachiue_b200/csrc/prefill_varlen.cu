@@ -22,8 +22,11 @@
 //    below 2^8 otherwise and O / l cancels the stale maximum.
 //  * Keys and values behind a sequence's end have no influence: scores are
 //    selected, value rows are zeroed in shared memory.  Masked keys inside the sequence
-//    meet P = 0; where such a value is not finite the row's result is not either, and
-//    the row is computed again over its visible keys alone (slow, exact, never taken by finite inputs).
+//    meet P = 0; where such a value is not finite the row's result is not either.  A CTA
+//    that stored such a row (or one that overflowed: P reaches 2^8, so values of bf16's
+//    last 2^9 may) goes over its items once more when all of them are done and no wait
+//    is open, and computes again, over their visible keys alone, the rows whose result
+//    no visible value explains (mend_rows: slow and exact).
 //
 // Measured, bf16, D = 128: 8192 tokens in eight prompts of 1 to 3001, 32 / 8 heads,
 // 146 us, 955 TFLOP/s (0.57 of the library's dense rate); 32772 tokens, 16 / 4 heads,
@@ -223,29 +226,6 @@ __device__ __forceinline__ void chunk_p(const uint32_t (&r)[32], bool empty, uin
   }
 }
 
-// One row over its visible keys [lo, hi], by a warp: for rows that a value outside them made not finite.
-template <typename T>
-__device__ __noinline__ void row_alone(const VarlenArgs& a, int q_row, int head, int k0, int lo, int hi) {
-  const int lane = threadIdx.x & 31, g = head / a.G;
-  float q[4], acc[4] = {}, m = -INFINITY, l = 0.f;
-  load4(static_cast<const T*>(a.q) + (long long)q_row * a.q_stride + head * HD + 4 * lane, q);
-  for (int t = lo; t <= hi; t++) {
-    float k[4], v[4];
-    load4(static_cast<const T*>(a.k) + (long long)(k0 + t) * a.k_stride + g * HD + 4 * lane, k);
-    load4(static_cast<const T*>(a.v) + (long long)(k0 + t) * a.v_stride + g * HD + 4 * lane, v);
-    float x = fmaf(q[0], k[0], fmaf(q[1], k[1], fmaf(q[2], k[2], q[3] * k[3])));
-    x = warp_sum(x) * a.scale_log2;
-    const float mn = fmaxf(m, x), f = exp2f(m - mn), p = exp2f(x - mn);
-    m = mn;
-    l = fmaf(l, f, p);
-#pragma unroll
-    for (int c = 0; c < 4; c++) acc[c] = fmaf(acc[c], f, p * v[c]);
-  }
-#pragma unroll
-  for (int c = 0; c < 4; c++) acc[c] /= l;
-  store4(static_cast<T*>(a.out) + ((long long)q_row * a.H + head) * HD + 4 * lane, acc);
-}
-
 // Barriers by their 32-bit shared-memory address (generic pointers to a dozen of them cost the issuing warp its registers).
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
   uint32_t ok;
@@ -363,6 +343,160 @@ __device__ __noinline__ void own_item(const VarlenArgs& a, RawItem* item, int* s
   }
 }
 
+// ---- rows to be computed again -------------------------------------------------
+struct Mend {
+  int any;             // a row of the half was stored with a result that is not finite
+  int late;            // a wait of the half ran out: its results are not all there
+  int rows[4];         // per warp: some row of the present item's is one
+  // Dimensions, a bit each.  need: of such results, the infinite ones (words 0 .. 3) and the NaN ones (4 .. 7).  seen: where a
+  // value that every row of the half sees is infinite or NaN (0 .. 3), is NaN (4 .. 7).
+  uint32_t need[8], seen[8];
+};
+constexpr uint32_t kNoSum = 0xffffffffu;  // a stored row without a sum (NaN, infinite or zero): NaN for good (no conversion gives this one)
+
+// Two elements: bits 0, 1 infinite or NaN; bits 4, 5 NaN.
+template <bool BF16>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+  constexpr uint32_t E = BF16 ? 0x7f80u : 0x7c00u;
+  const uint32_t a = w & 0x7fffu, b = w >> 16 & 0x7fffu;
+  return (a >= E ? 1u : 0u) | (b >= E ? 2u : 0u) | (a > E ? 16u : 0u) | (b > E ? 32u : 0u);
+}
+// Four: bits 0 .. 3 and 4 .. 7.
+template <bool BF16>
+__device__ __forceinline__ uint32_t not_finite4(uint2 w) { return not_finite<BF16>(w.x) | not_finite<BF16>(w.y) << 2; }
+
+__device__ __forceinline__ void half_sync(int hd) { asm volatile("bar.sync %0, 128;" ::"r"(1 + hd) : "memory"); }
+
+// One row over its visible keys lo .. hi, by a warp: a lane's keys are lo + lane, 32 apart.  Two passes, so that the weights are
+// divided by their sum before they meet the values.
+template <bool BF16>
+__device__ __noinline__ void row_alone(const VarlenArgs& a, int q_row, int head, int k0, int lo, int hi) {
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  const int lane = threadIdx.x & 31, g = head / a.G;
+  const T* q = static_cast<const T*>(a.q) + (long long)q_row * a.q_stride + head * HD;
+  const T* k = static_cast<const T*>(a.k) + (long long)k0 * a.k_stride + g * HD;
+  const T* v = static_cast<const T*>(a.v) + (long long)k0 * a.v_stride + g * HD;
+  auto score = [&](int t) {
+    float x = 0.f;
+    for (int d = 0; d < HD; d += 8) {
+      float y[8], z[8];
+      load8(q + d, y);
+      load8(k + (long long)t * a.k_stride + d, z);
+#pragma unroll
+      for (int c = 0; c < 8; c++) x = fmaf(y[c], z[c], x);
+    }
+    return x * a.scale_log2;
+  };
+  float m = -INFINITY, l = 0.f;
+  for (int t = lo + lane; t <= hi; t += 32) {
+    const float x = score(t), mn = fmaxf(m, x);
+    if (x == -INFINITY) continue;  // no weight
+    l = fmaf(l, exp2f(m - mn), exp2f(x - mn));
+    m = mn;
+  }
+  const float top = warp_max(m);
+  l = warp_sum(m == -INFINITY ? l : l * exp2f(m - top));
+  const float inv = 1.f / l;
+  float acc[4] = {};
+  for (int t0 = lo; t0 <= hi; t0 += 32) {
+    const float p = t0 + lane <= hi ? exp2f(score(t0 + lane) - top) * inv : 0.f;
+    const int n = min(32, hi - t0 + 1);
+    for (int j = 0; j < n; j++) {
+      const float w = __shfl_sync(0xffffffffu, p, j);
+      float y[4];
+      load4(v + (long long)(t0 + j) * a.v_stride + 4 * lane, y);
+#pragma unroll
+      for (int c = 0; c < 4; c++) acc[c] = fmaf(w, y[c], acc[c]);
+    }
+  }
+  store4(static_cast<T*>(a.out) + ((long long)q_row * a.H + head) * HD + 4 * lane, acc);
+}
+
+// Of a half's 128 rows of an item, computes those again whose stored result the values that they see do not explain.  An
+// infinity is explained by a visible value that is not finite, a NaN by a visible NaN, or by a visible infinity where no
+// hidden value of the item's tiles is not finite.  By the half's four warps; `tid` 0 .. 127 is also the row.
+template <bool BF16>
+__device__ __noinline__ void mend_rows(const VarlenArgs& a, const Item it, int hd, int tid, Mend& s) {
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  const int lane = tid & 31, warp = tid >> 5, off = it.lk - it.lq;
+  const int first = it.r0 + hd * BM, r = first + tid, qi = r / a.G, head = it.g * a.G + r % a.G;
+  const int q_last = min(it.lq - 1, (first + BM - 1) / a.G);
+  auto first_key = [&](int pos) { return a.window > 0 ? max(0, pos - a.window + 1) : 0; };
+  uint32_t bad[8] = {};  // this thread's row: dimensions, as in Mend::need
+  if (qi < it.lq && off + qi >= 0) {
+    const uint4* row = reinterpret_cast<const uint4*>(static_cast<const T*>(a.out) + ((long long)(it.q0 + qi) * a.H + head) * HD);
+    if (row->x != kNoSum)
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        const uint4 w = row[i];
+        const uint32_t f = not_finite4<BF16>(make_uint2(w.x, w.y)), h = not_finite4<BF16>(make_uint2(w.z, w.w));
+        const uint32_t inf = (f & 15u) | (h & 15u) << 4, nan = f >> 4 | h & 0xf0u;
+        bad[i / 4] |= (inf & ~nan) << (8 * (i & 3));
+        bad[4 + i / 4] |= nan << (8 * (i & 3));
+      }
+  }
+  uint32_t any = 0;
+#pragma unroll
+  for (int i = 0; i < 8; i++) any |= bad[i];
+  if (tid < 8) s.need[tid] = s.seen[tid] = 0u;
+  half_sync(hd);
+  if (any)
+#pragma unroll
+    for (int i = 0; i < 8; i++) atomicOr(&s.need[i], bad[i]);
+  const bool some = __any_sync(0xffffffffu, any != 0);
+  if (lane == 0) s.rows[warp] = some;
+  half_sync(hd);
+  if (!(s.rows[0] | s.rows[1] | s.rows[2] | s.rows[3])) return;
+  // A lane has dimensions 4 lane .. + 3: bits 0 .. 3 and 4 .. 7 of these masks are words 0 .. 3 and 4 .. 7 of Mend's.
+  const int word = lane >> 3, bit = 4 * (lane & 7);
+  auto part = [&](const uint32_t* w) { return (w[word] >> bit & 15u) | (w[4 + word] >> bit & 15u) << 4; };
+  const T* v = static_cast<const T*>(a.v) + (long long)it.k0 * a.v_stride + it.g * HD + 4 * lane;
+  auto value = [&](int t) { return not_finite4<BF16>(*reinterpret_cast<const uint2*>(v + (long long)t * a.v_stride)); };
+  // Keys that every row of the half sees: a warp looks at eight of every 32.
+  const int all_lo = first_key(off + q_last), all_hi = off + first / a.G;
+  const uint32_t mine = part(s.need), dims = (mine | mine >> 4) & 15u;
+  for (int t0 = all_lo + 8 * warp; t0 <= all_hi; t0 += 32) {
+    uint32_t f = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+      if (t0 + j <= all_hi) f |= value(t0 + j);
+    if (f &= dims * 17u) {
+      atomicOr(&s.seen[word], (f & 15u) << bit);
+      atomicOr(&s.seen[4 + word], (f >> 4) << bit);
+    }
+    const volatile uint32_t* now = s.seen;
+    if (__all_sync(0xffffffffu, (mine & ~((now[word] >> bit & 15u) | (now[4 + word] >> bit & 15u) << 4)) == 0)) break;
+  }
+  half_sync(hd);
+  const uint32_t seen = part(s.seen);
+  uint32_t left = 0;
+#pragma unroll
+  for (int i = 0; i < 8; i++) left |= bad[i] & ~s.seen[i];
+  for (uint32_t rows = __ballot_sync(0xffffffffu, left != 0); rows; rows &= rows - 1) {
+    const int src = __ffs(rows) - 1;
+    const int pos = __shfl_sync(0xffffffffu, off + qi, src), h = __shfl_sync(0xffffffffu, head, src), lo = first_key(pos);
+    uint32_t open = 0;  // of this lane's four dimensions
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const uint32_t w = __shfl_sync(0xffffffffu, bad[i], src);
+      if ((i & 3) == word) open |= (w >> bit & 15u) << (i & 4);
+    }
+    // the keys that this row sees and some other of the half does not
+    uint32_t visible = seen;
+    for (int t = lo; t < min(all_lo, pos + 1); t++) visible |= value(t);
+    for (int t = max(max(lo, all_lo), all_hi + 1); t <= pos; t++) visible |= value(t);
+    open &= ~visible;
+    if (const uint32_t either = open >> 4 & visible & 15u; __any_sync(0xffffffffu, either != 0)) {
+      uint32_t hidden = 0;
+      for (int t = it.n_first; t < lo; t++) hidden |= value(t);
+      for (int t = pos + 1; t < min(it.lk, it.n_first + it.ntiles * BN); t++) hidden |= value(t);
+      open &= ~((either & ~hidden) << 4);
+    }
+    if (__any_sync(0xffffffffu, open != 0)) row_alone<BF16>(a, it.q0 + pos - off, h, it.k0, lo, pos);
+  }
+  half_sync(hd);  // the masks are free again
+}
+
 // TMEM (512 columns): O of the two halves, P of the two, and ONE buffer for S.
 // A softmax thread takes its whole row of S into registers at once, so the
 // buffer is free again some 100 cycles after the product is done, and the
@@ -382,7 +516,7 @@ constexpr uint32_t kColP = 256, kColS = 384;
 template <bool BF16>
 __global__ void __launch_bounds__(384, 1)
     prefill_varlen_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                          const __grid_constant__ CUtensorMap tmV, const VarlenArgs a) {
+                          const __grid_constant__ CUtensorMap tmV, const __grid_constant__ VarlenArgs a) {
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -392,8 +526,10 @@ __global__ void __launch_bounds__(384, 1)
   __shared__ uint32_t tmem_slot;
   __shared__ RawItem s_item;
   __shared__ int s_scan[24];
+  __shared__ Mend s_mend[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
+  if (tid < 2) s_mend[tid].any = s_mend[tid].late = 0;
   if (tid == 0) {
     for (int i = 0; i < kBars; i++)
       mbar_init(&bars[i], i >= kPHalf ? 4 : (i >= kKEmpty && i < kVFull) || (i >= kVEmpty && i < kSFull) ? 2 : 1);
@@ -615,14 +751,15 @@ __global__ void __launch_bounds__(384, 1)
     const uint32_t sc = tmem + lane_off + kColS, pc = tmem + lane_off + kColP + hd * 64, oc = tmem + lane_off + hd * HD;
     // A finished item's result: out of TMEM and into the output.  It runs after the NEXT item's first P is in TMEM, which
     // waited for the finished item's last product.
-    int f_row = -1, f_head = 0, f_k0 = 0, f_lo = 0, f_hi = -1;  // this thread's finished row: query row (-1: none), head, visible keys
+    int f_row = -1, f_head = 0;  // this thread's finished row: query row (-1: none), head
+    bool f_empty = false;        // it sees no key
     float f_l = 0.f;
     bool fin = false;
     auto epilogue = [&]() {
-      const bool empty = f_lo > f_hi;
+      const bool sum = f_l > 0.f && f_l < INFINITY;  // else the row is NaN, whatever its values are
       const float inv = 1.f / f_l;
       const uint64_t inv2 = f2(inv, inv);
-      uint64_t sum = f2(0.f, 0.f);
+      uint32_t top = 0u;  // largest magnitude of the stored elements, by their bits
       T* dst = static_cast<T*>(a.out) + ((long long)f_row * a.H + f_head) * HD;
 #pragma unroll 1
       for (int c = 0; c < 4; c++) {
@@ -632,31 +769,22 @@ __global__ void __launch_bounds__(384, 1)
         float w[16];
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-          const uint64_t y = f2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]));
-          sum = f2_fma(y, f2(0.f, 0.f), sum);  // NaN once anything is not finite
           float y0, y1;
-          f2_get(f2_mul(y, inv2), y0, y1);
-          w[i] = __uint_as_float(pack16<BF16>(y0, y1));
+          f2_get(f2_mul(f2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])), inv2), y0, y1);
+          const uint32_t y = pack16<BF16>(y0, y1);
+          top = __vmaxu2(top, y & 0x7fff7fffu);
+          w[i] = __uint_as_float(f_empty ? 0u : sum ? y : kNoSum);
         }
-        if (f_row >= 0 && !empty) {
+        if (f_row >= 0) {
           st_global_v8(reinterpret_cast<float*>(dst + 32 * c), w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]);
           st_global_v8(reinterpret_cast<float*>(dst + 32 * c + 16), w[8], w[9], w[10], w[11], w[12], w[13], w[14], w[15]);
         }
       }
       tc_fence_before();
-      __syncwarp();  // (also: a row's stores come before row_alone's)
+      __syncwarp();
       if (lane == 0) bar_arrive(bar(kOFree + hd));
-      float s0, s1;
-      f2_get(sum, s0, s1);
-      const bool bad = f_row >= 0 && !empty && !(s0 + s1 == 0.f && f_l > 0.f && f_l < INFINITY);
-      if (f_row >= 0 && empty)
-#pragma unroll 1
-        for (int i = 0; i < HD; i += 16) st_global_v8(reinterpret_cast<float*>(dst + i), 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f);
-      for (uint32_t rows = __ballot_sync(0xffffffffu, bad); rows; rows &= rows - 1) {
-        const int src = __ffs(rows) - 1;
-        row_alone<T>(a, __shfl_sync(0xffffffffu, f_row, src), __shfl_sync(0xffffffffu, f_head, src),
-                     __shfl_sync(0xffffffffu, f_k0, src), __shfl_sync(0xffffffffu, f_lo, src), __shfl_sync(0xffffffffu, f_hi, src));
-      }
+      const bool bad = f_row >= 0 && !f_empty && sum && not_finite<BF16>(top);
+      if (__any_sync(0xffffffffu, bad) && lane == 0) s_mend[hd].any = 1;
       fin = false;
     };
     int nt = 0;  // key tiles of this half so far
@@ -760,14 +888,23 @@ __global__ void __launch_bounds__(384, 1)
       fin = true;
       f_row = exists ? it.q0 + qi : -1;
       f_head = it.g * a.G + r - qi * a.G;
-      f_k0 = it.k0;
-      f_lo = row_lo, f_hi = row_hi;
+      f_empty = row_lo > row_hi;
       f_l = l;
       nt += it.ntiles;
     }
     if (ok && fin && wait(kPVDone + hd, (nt - 1) & 1)) {
       tc_fence_after();
       epilogue();
+    }
+    if (!ok && lane == 0) s_mend[hd].late = 1;
+    half_sync(hd);  // the half's results are stored
+    if (s_mend[hd].any && !s_mend[hd].late) {
+      RawItem next = load_item(0);
+      for (int k = 0; next.g >= 0; k++) {
+        const Item it = unpack(next);
+        next = load_item(k + 1);
+        mend_rows<BF16>(a, it, hd, row, s_mend[hd]);
+      }
     }
   }
   tc_fence_before();
