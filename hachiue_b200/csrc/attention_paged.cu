@@ -1034,10 +1034,23 @@ int launch(hcu_context* h, PagedAttnArgs a) {
   const long long chunks = (span + CHUNK - 1) / CHUNK + (a.window > 0 ? 1 : 0);
   a.cluster = 1;
   while (a.cluster < kMaxCluster && a.cluster * NW < chunks && 2 * a.cluster * units <= grid) a.cluster *= 2;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[1];
+  cfg.blockDim = dim3(32 * NW);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = h->stream;
+  cfg.attrs = attr;
   if (chunks <= std::min(kMaxCluster, kClusterChunks * a.cluster) * NW && units <= grid && h->opt_attn_chunk == 0) {
     a.split = kCluster;
-    grid = units * a.cluster;
-  } else if (room >= (size_t)grid * (2 * record + sizeof(int4)) && most < 0x7fffffffLL) {
+    cfg.gridDim = dim3((unsigned)(units * a.cluster));
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = a.cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kern, a) == cudaSuccess) return HCU_OK;
+    (void)cudaGetLastError();  // no room for a cluster on this device: by the other ways
+  }
+  if (room >= (size_t)grid * (2 * record + sizeof(int4)) && most < 0x7fffffffLL) {
     a.split = kLine;
     grid = std::min(grid, (most + a.min_chunks - 1) / a.min_chunks);
   } else {
@@ -1046,17 +1059,8 @@ int launch(hcu_context* h, PagedAttnArgs a) {
   }
   a.open = reinterpret_cast<int4*>(static_cast<uint8_t*>(h->workspace) + kTicketBytes);
   a.part = reinterpret_cast<float*>(a.open + grid);
-  cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute attr[1];
   cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(32 * NW);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = h->stream;
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = a.split == kCluster ? a.cluster : 1;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = a.split == kCluster ? 1 : 0;
+  cfg.numAttrs = 0;
   HCU_TRY(check_cuda(cudaLaunchKernelEx(&cfg, kern, a), "hcu_attention_paged: launch"));
   if (a.split != kLine || grid == 1) return HCU_OK;
   cfg.gridDim = dim3((unsigned)(grid - 1), RB);  // no unit goes on behind the last CTA
@@ -1064,7 +1068,6 @@ int launch(hcu_context* h, PagedAttnArgs a) {
   cfg.dynamicSmemBytes = 0;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
   cfg.numAttrs = 1;
   return check_cuda(cudaLaunchKernelEx(&cfg, attn_paged_join_kernel<DH, RB>, a), "hcu_attention_paged: join");
 }
