@@ -1061,7 +1061,8 @@ int launch(hcu_context* h, PagedAttnArgs a) {
   a.part = reinterpret_cast<float*>(a.open + grid);
   cfg.gridDim = dim3((unsigned)grid);
   cfg.numAttrs = 0;
-  HCU_TRY(check_cuda(cudaLaunchKernelEx(&cfg, kern, a), "hcu_attention_paged: launch"));
+  (void)cudaLaunchKernelEx(&cfg, kern, a);
+  HCU_TRY(after_launch("hcu_attention_paged: launch"));  // takes the error, if there is one, so that no later call finds it
   if (a.split != kLine || grid == 1) return HCU_OK;
   cfg.gridDim = dim3((unsigned)(grid - 1), RB);  // no unit goes on behind the last CTA
   cfg.blockDim = dim3(128);
@@ -1069,7 +1070,8 @@ int launch(hcu_context* h, PagedAttnArgs a) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.numAttrs = 1;
-  return check_cuda(cudaLaunchKernelEx(&cfg, attn_paged_join_kernel<DH, RB>, a), "hcu_attention_paged: join");
+  (void)cudaLaunchKernelEx(&cfg, attn_paged_join_kernel<DH, RB>, a);
+  return after_launch("hcu_attention_paged: join");
 }
 
 template <int DH>

@@ -1,5 +1,5 @@
-"""How hcu_attention_paged launches its kernels, on the CPU: the host code of attention_paged.cu linked with a stand-in for the
-CUDA runtime that records launches and refuses those that it is told to."""
+"""How hcu_attention_paged and hcu_prefill_varlen launch their kernels, on the CPU: their host code linked with a stand-in for
+the CUDA runtime that records launches and refuses those that it is told to."""
 import ctypes
 import os
 import shutil
@@ -35,18 +35,26 @@ cudaError_t cudaLaunchKernelExC(const cudaLaunchConfig_t* c, const void*, void**
   launches.push_back(l);
   return cudaSuccess;
 }
-cudaError_t cudaLaunchKernel(const void*, dim3, dim3, void**, size_t, cudaStream_t) { return cudaErrorUnknown; }
+cudaError_t cudaLaunchKernel(const void*, dim3 g, dim3 b, void**, size_t, cudaStream_t) {
+  if (refuse_all > 1) return last = cudaErrorInvalidConfiguration;
+  launches.push_back({{g.x, g.y, g.z}, b.x, 0, 0});
+  return cudaSuccess;
+}
 void** __cudaRegisterFatBinary(void*) { static void* p; return &p; }
 void __cudaRegisterFatBinaryEnd(void**) {}
 void __cudaUnregisterFatBinary(void**) {}
 void __cudaRegisterFunction(void**, const char*, char*, const char*, int, uint3*, uint3*, dim3*, dim3*, int*) {}
 unsigned __cudaPushCallConfiguration(dim3, dim3, size_t, void*) { return 0; }
-cudaError_t __cudaPopCallConfiguration(dim3*, dim3*, size_t*, void*) { return cudaSuccess; }
+cudaError_t __cudaPopCallConfiguration(dim3* g, dim3* b, size_t* s, void*) { return *g = *b = dim3(1), *s = 0, cudaSuccess; }
 }
 namespace hcu {
 int fail(int code, const char*, ...) { return code; }
 int check_cuda(cudaError_t e, const char*) { return e == cudaSuccess ? HCU_OK : HCU_ECUDA; }
 int begin_op(hcu_context*, const char*) { return HCU_OK; }
+int after_launch(const char* what) { return check_cuda(cudaGetLastError(), what); }
+int make_tensor_map(CUtensorMap*, CUtensorMapDataType, int, void*, const uint64_t*, const uint64_t*, const uint32_t*, CUtensorMapSwizzle) {
+  return HCU_OK;
+}
 }
 extern "C" int run(const hcu_attention_paged_params* p, const hcu_paged_kv* kv, size_t workspace, int clusters_refused, int all_refused,
                    unsigned (*out)[6], int* n, int* left) {
@@ -61,6 +69,17 @@ extern "C" int run(const hcu_attention_paged_params* p, const hcu_paged_kv* kv, 
   *left = last;
   return rc;
 }
+extern "C" int run_prefill(const hcu_prefill_varlen_params* p, int all_refused, int* n, int* left) {
+  hcu_context h;
+  h.workspace = (void*)(1 << 20);
+  h.workspace_bytes = 64 << 20;
+  launches.clear();
+  refuse_all = all_refused, last = cudaSuccess;
+  const int rc = hcu_prefill_varlen(&h, p, (void*)4096, (void*)4096, (void*)4096, (void*)4096);
+  *n = (int)launches.size();
+  *left = last;
+  return rc;
+}
 """
 
 
@@ -69,16 +88,18 @@ def host(tmp_path_factory):
     if not shutil.which("g++"):
         pytest.skip("no g++")
     build.build()
-    obj = os.path.join(build.BUILD, "attention_paged.o")
-    src = os.path.join(build.CSRC, "attention_paged.cu")
-    if not os.path.exists(obj) or os.path.getmtime(obj) < os.path.getmtime(src):
-        os.makedirs(build.BUILD, exist_ok=True)
-        build._compile(src, False, [])
+    objs = []
+    for name in ("attention_paged", "prefill_varlen"):
+        obj, src = os.path.join(build.BUILD, name + ".o"), os.path.join(build.CSRC, name + ".cu")
+        if not os.path.exists(obj) or os.path.getmtime(obj) < os.path.getmtime(src):
+            os.makedirs(build.BUILD, exist_ok=True)
+            build._compile(src, False, [])
+        objs.append(obj)
     d = tmp_path_factory.mktemp("host")
     fake, lib = d / "fake.cpp", d / "host.so"
     fake.write_text(FAKE)
     cuda = os.path.join(os.path.dirname(os.path.dirname(build.nvcc())), "include")
-    subprocess.run(["g++", "-std=c++17", "-shared", "-fPIC", "-I", cuda, "-I", build.INCLUDE, "-I", build.CSRC, str(fake), obj, "-o", str(lib)],
+    subprocess.run(["g++", "-std=c++17", "-shared", "-fPIC", "-I", cuda, "-I", build.INCLUDE, "-I", build.CSRC, str(fake), *objs, "-o", str(lib)],
                    check=True, capture_output=True)
     return ctypes.CDLL(str(lib))
 
@@ -116,8 +137,15 @@ def test_a_refused_cluster_falls_back(host, case):
     assert rc == 0 and left == 0 and len(got) == 1 and not got[0]["cluster"] and got[0]["x"] <= 296
 
 
-def test_a_launch_that_fails_is_reported(host):
-    rc, got, _ = launches(host, all_refused=1)
-    assert rc == _lib.HCU_ECUDA and not got
-    rc, got, _ = launches(host, all_refused=1, max_context=100000)
-    assert rc == _lib.HCU_ECUDA and not got
+def test_a_launch_that_fails_is_reported_once(host):
+    """By the call that makes it: the error does not stay for a later one to find."""
+    for case in (dict(), dict(max_context=100000)):
+        rc, got, left = launches(host, all_refused=1, **case)
+        assert rc == _lib.HCU_ECUDA and not got and left == 0
+    n, left = ctypes.c_int(), ctypes.c_int()
+    for total, before in ((64, 0), (100000, 1)):  # in one launch; behind the list of items
+        p = _lib.hcu_prefill_varlen_params(2, 16, 8, 128, 0, _lib.DT_BF16, total, total, 4096, None, 0, 0, 0)
+        assert host.run_prefill(ctypes.byref(p), 0, ctypes.byref(n), ctypes.byref(left)) == 0 and n.value == before + 1
+        for refused in (1, 2):
+            assert host.run_prefill(ctypes.byref(p), refused, ctypes.byref(n), ctypes.byref(left)) == _lib.HCU_ECUDA
+            assert left.value == 0 and n.value == (before if refused == 1 else 0)
