@@ -592,10 +592,14 @@ class CudaBackend:
         if B == 0 or S == 0:
             return
         pages = table[1]
+        if not (0 <= window_size <= 0x7fffffff and 0 <= max_context <= 0x7fffffff):  # a 32-bit field would wrap
+            raise HachiueError(_lib.HCU_EINVAL, f"hachiue: attention_paged: window_size ({window_size}) and max_context "
+                                                f"({max_context}) must lie within 0 .. 2^31 - 1")
         self._bind_stream()
         p = self._paged_params  # every field is set
         p.batch, p.S, p.H, p.windowSize, p.dtype = B, S, H, window_size, _DT[dtype]
-        p.max_context, p.table_stride = max_context or pages * kv.page_size, pages
+        # a wide table may hold more than the library's largest context
+        p.max_context, p.table_stride = max_context or min(pages * kv.page_size, 0x7fffff00), pages
         p.block_table, p.context = block_table.data_ptr(), context.data_ptr()
         check(self.lib.hcu_attention_paged(self._h, ctypes.byref(p), q.data_ptr(), ctypes.byref(kv), out.data_ptr()))
 
@@ -624,6 +628,8 @@ class CudaBackend:
                 raise HachiueError(_lib.HCU_EINVAL, "hachiue: prefill_varlen takes contiguous int32 offsets [B + 1]")
         if cu_q.dtype != torch.int32 or cu_q.dim() != 1 or cu_q.shape[0] < 1 or not cu_q.is_contiguous():
             raise HachiueError(_lib.HCU_EINVAL, "hachiue: prefill_varlen takes contiguous int32 offsets [B + 1]")
+        if not 0 <= window <= 0x7fffffff:
+            raise HachiueError(_lib.HCU_EINVAL, f"hachiue: {op}: window ({window}) must lie within 0 .. 2^31 - 1")
         if nq == 0 or cu_q.shape[0] == 1:
             return
         self._bind_stream()
