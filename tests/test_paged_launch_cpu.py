@@ -99,7 +99,7 @@ def host(tmp_path_factory):
     fake, lib = d / "fake.cpp", d / "host.so"
     fake.write_text(FAKE)
     cuda = os.path.join(os.path.dirname(os.path.dirname(build.nvcc())), "include")
-    subprocess.run(["g++", "-std=c++17", "-shared", "-fPIC", "-I", cuda, "-I", build.INCLUDE, "-I", build.CSRC, str(fake), *objs, "-o", str(lib)],
+    subprocess.run(["g++", "-std=c++17", "-shared", "-fPIC", "-Wl,-Bsymbolic", "-I", cuda, "-I", build.INCLUDE, "-I", build.CSRC, str(fake), *objs, "-o", str(lib)],
                    check=True, capture_output=True)
     return ctypes.CDLL(str(lib))
 
