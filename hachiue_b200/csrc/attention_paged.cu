@@ -38,10 +38,10 @@
 // warp fetches its chunks into a ring of its own, two ahead, and never waits for
 // another warp until they join their sums.
 //
-// Measured, bf16, 32 query and 8 KV heads of 128: 64 sequences of 271k tokens
-// in all 84 us, 312 MB at 3.7 TB/s; one of 131072 47 us.  Issue-bound: 700 instructions per
-// chunk at 56 % of the slots, of which the masks and shifts of the codes are a quarter;
-// 128 registers allow 16 warps per SM.
+// Measured, bf16, 32 query and 8 KV heads of 128, calls in a row: 64 sequences of 271k
+// tokens in all 85 us, 312 MB at 3.7 TB/s; one of 131072 47 us.  Issue-bound: 700
+// instructions per chunk at 55 % of the slots, of which the masks and shifts of the codes
+// are a quarter; 128 registers allow 16 warps per SM.
 #include <algorithm>
 #include <cfloat>
 
@@ -73,8 +73,9 @@ constexpr int NW = 8;          // warps of a CTA
 // chunks, or each to a cluster of CTAs, which joins its parts through shared
 // memory without a second kernel.  The host takes clusters for short contexts
 // and few units: up to four chunks per warp, in up to eight CTAs (replayed graphs, f32, 16 / 8
-// heads of 128, cluster / line: one sequence of 256 tokens 9.0 / 11.4 us, of 1024
-// 10.1 / 11.4, 16 of 1024 14.3 / 16.6, 16 of 2048 19.7 / 21.8; one of 4096 13.5 / 12.1).
+// heads of 128, cluster / line: one sequence of 256 tokens 8.9 / 11.7 us, of 1024
+// 10.2 / 11.7, 16 of 1024 14.7 / 17.1, 16 of 2048 20.3 / 22.6; one of 2048 11.9 / 11.9, of
+// 4096 13.8 / 12.3).
 constexpr int kWarpUnits = 0, kLine = 1, kCluster = 2;
 constexpr int CHUNK = 32;      // tokens a warp takes at a time
 constexpr int kUnitCost = 3;    // chunks that a unit's queries and sums cost a warp besides its chunks
@@ -208,7 +209,7 @@ constexpr int paged_row_floats(int dh) { return dh + 4; }  // of the warps' sums
 constexpr size_t paged_smem(int dh, int rb) {
   return (size_t)NW * STAGES * paged_stage_bytes(dh) + (size_t)NW * rb * paged_row_floats(dh) * 4;
 }
-// Per SM.  One row per thread fits 128 registers; two (bf16, eight rows) do not: two CTAs 67 us, one 59 (32 sequences, 64 / 8 heads).
+// Per SM.  One row per thread fits 128 registers; two (bf16, eight rows) do not: two CTAs 67 us, one 60 (32 sequences, 64 / 8 heads).
 constexpr int paged_ctas(int dh, int ct) { return dh == 128 && ct == 2 ? 2 : 1; }
 
 // The work of a call is a line of chunks: sequence after sequence, in each
@@ -256,8 +257,9 @@ __global__ void __launch_bounds__(32 * NW, paged_ctas(DH, CT)) attn_paged_kernel
   static_assert(CT * MT == 1 || (CT * MT == 2 && (MT == 1 || EXACT)), "one f16 number or two");
   constexpr bool WIDE = CT * MT == 2;          // two f16 numbers: queries may be f32
   constexpr int KB = CHUNK * DH / 2, CB = CHUNK * NB * 2;  // bytes of a stage's codes, of its scales
-  // Steps of 16 tokens in the loop's body: with two of these the code outgrows the instruction cache (bf16, four tokens
-  // of 32 / 8 heads over 16 x 4000 tokens: 58 us unrolled, 54 rolled; one token of 32 / 8 over 64 sequences: 85 and 89).
+  // Steps of 16 tokens in the loop's body: with two of these the code outgrows the instruction cache (replayed graphs, bf16,
+  // four tokens of 32 / 8 heads over 16 x 4000 tokens: 53.6 us unrolled, 50.2 rolled; f32, four tokens of 16 / 2 heads of 256
+  // over 16 x 4096: 83 and 76; bf16, one token of 32 / 8 over 64 x 1612: 39.6 and 40.2).
   constexpr int kSteps = DH == 256 || NC == 2 ? 1 : 2;
   constexpr int RS = paged_row_floats(DH);
   constexpr size_t REC = (size_t)RB * (DH + 2);  // floats of a global record

@@ -10,7 +10,7 @@
 //    the tokens, each with the next one's rows on their way into L2 (a block per
 //    token spent its life waiting for its slot, then its angles, then its rows: 76
 //    against 65 us below).  8192 tokens of 32 query, 8 key and 8 value heads of 128,
-//    bf16: 65 us, 181 MB at 2.8 TB/s, of which the values' and keys' codes
+//    bf16: 65 us (L2 flushed), 181 MB at 2.8 TB/s, of which the values' and keys' codes
 //    take 40: 370 instructions per warp and two rows, at 70 % of the issue rate.
 //  * Read: eight bytes of codes per lane, so that a warp has four rows of 128 of
 //    both tensors in flight, and writes whole 32-byte sectors.  16384 rows of 8 heads

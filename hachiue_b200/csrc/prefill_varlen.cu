@@ -14,8 +14,9 @@
 //    number of key tiles, so that the persistent CTAs' shares are near equal
 //    whatever the lengths are.  (A call with no more items than SMs needs no list.)
 //  * Warp roles: K / V by TMA (warp 0), tcgen05.mma of each tile (warps 1, 2: one
-//    warp for both spent more time on its barriers than the products take), Q rows
-//    by cp.async (warp 3), and a softmax warpgroup per tile, one thread per row.  S
+//    warp for both spent more time on its barriers than the products take), Q tiles
+//    by TMA, or row by row with cp.async where G does not divide 128 (warp 3), and a
+//    softmax warpgroup per tile, one thread per row.  S
 //    is in TMEM, P goes back over its columns, O stays in TMEM across the keys.
 //    While one tile's softmax runs the tensor cores work on the other tile.
 //  * O is rescaled only when a row's maximum grows by more than 2^8: P stays
@@ -28,10 +29,11 @@
 //    is open, and computes again, over their visible keys alone, the rows whose result
 //    no visible value explains (mend_rows: slow and exact).
 //
-// Measured, bf16, D = 128: 8192 tokens in eight prompts of 1 to 3001, 32 / 8 heads,
-// 146 us, 955 TFLOP/s (0.57 of the library's dense rate); 32772 tokens, 16 / 4 heads,
-// window 1024, 247 us, 975.  A pair of tiles takes 3300 cycles, 2900 of them the
-// chain S -> softmax -> P -> P V of one row; tensor pipe 58 %, SFU 58 %.
+// Measured, bf16, D = 128, calls in a row (which run at the power cap): 8192 tokens in
+// eight prompts of 1 to 3001, 32 / 8 heads, 162 us, 863 TFLOP/s (0.51 of the library's
+// dense burst rate); 32772 tokens, 16 / 4 heads, window 1024, 289 us, 832.  Single calls
+// with L2 flushed take 153 and 261.  A pair of tiles takes 3300 cycles, 2900 of them the
+// chain S -> softmax -> P -> P V of one row; tensor pipe 59 %, SFU 59 %.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -299,7 +301,7 @@ __device__ __forceinline__ int item_index(int k) {
 
 // The item of this CTA where there are no more items than CTAs: each thread takes a sequence (at most kDirectBatch), checks it
 // as varlen_items_kernel does, and the one whose blocks hold the CTA's writes the item.  A launch less: 77 tokens of
-// 16 / 8 heads take 9.5 us in a replayed graph, through the list 10.1.
+// 16 / 8 heads take 8.3 us in a replayed graph, through the list 10.0.
 constexpr int kDirectBatch = 384;
 __device__ __noinline__ void own_item(const VarlenArgs& a, RawItem* item, int* scan) {
   const int b = threadIdx.x, lane = b & 31, warp = b >> 5;

@@ -642,8 +642,11 @@ int hcu_attention_paged(hcu_handle h, const hcu_attention_paged_params *p, const
  * D = 128.  Tensor cores, f32 accumulation; the probabilities are rounded to
  * `dtype` for their product with the values.
  *
- * Rows of out that no sequence covers are left as they were, and rows of k and
- * v outside a sequence have no influence on it, whatever they hold.  The
+ * Rows of out that no sequence covers are left as they were.  out must not
+ * overlap q, k or v.  Rows of k and v outside a sequence have no influence on
+ * it, and a row that a query does not see none on that query, whatever they
+ * hold (NaN or infinite values cost time: rows that they spoil are computed
+ * again after the others, key by key).  The
  * offsets must not decrease and must lie within the totals: a sequence whose
  * offsets do not, or whose queries begin below an earlier offset of cu_q, is
  * skipped and sets bit 2 of the device status.  The work list
