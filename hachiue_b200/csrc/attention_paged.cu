@@ -29,10 +29,10 @@
 //    for each row.  The weighted probabilities of a row and block of 32 dimensions
 //    are held times a power of two E of their own, so that the largest lies between
 //    2^8 and 2^15 whatever the scales of other blocks and of tokens without weight
-//    are: one below 2^-22 of the largest loses bits (f16's smallest number is 2^-24).
-//    (With one exponent for all blocks, that of the largest scale, values 2^-18 of
-//    another block's were off by 1e-4.)  M and the E move only when a number would
-//    pass 2^15.
+//    are, and none is off by more than 2^-32 of it beside its rounding (f16's smallest
+//    number is 2^-24).  (With one exponent for all blocks, that of the largest scale,
+//    values 2^-18 of another block's were off by 1e-4.)  M and the E move only when a
+//    number would pass 2^15.
 //
 // The work is cut by chunks of 32 tokens, not by sequences: see PagedPlan.  A
 // warp fetches its chunks into a ring of its own, two ahead, and never waits for

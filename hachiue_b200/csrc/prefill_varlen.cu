@@ -380,6 +380,7 @@ __device__ __noinline__ void row_alone(const VarlenArgs& a, int q_row, int head,
   const T* v = static_cast<const T*>(a.v) + (long long)k0 * a.v_stride + g * HD;
   auto score = [&](int t) {
     float x = 0.f;
+#pragma unroll 8
     for (int d = 0; d < HD; d += 8) {
       float y[8], z[8];
       load8(q + d, y);
@@ -402,13 +403,17 @@ __device__ __noinline__ void row_alone(const VarlenArgs& a, int q_row, int head,
   float acc[4] = {};
   for (int t0 = lo; t0 <= hi; t0 += 32) {
     const float p = t0 + lane <= hi ? exp2f(score(t0 + lane) - top) * inv : 0.f;
-    const int n = min(32, hi - t0 + 1);
-    for (int j = 0; j < n; j++) {
-      const float w = __shfl_sync(0xffffffffu, p, j);
-      float y[4];
-      load4(v + (long long)(t0 + j) * a.v_stride + 4 * lane, y);
+    for (int j0 = 0; j0 < min(32, hi - t0 + 1); j0 += 8) {
+      float y[8][4];
 #pragma unroll
-      for (int c = 0; c < 4; c++) acc[c] = fmaf(w, y[c], acc[c]);
+      for (int j = 0; j < 8; j++) load4(v + (long long)min(t0 + j0 + j, hi) * a.v_stride + 4 * lane, y[j]);
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const float w = __shfl_sync(0xffffffffu, p, j0 + j);
+        if (t0 + j0 + j <= hi)
+#pragma unroll
+          for (int c = 0; c < 4; c++) acc[c] = fmaf(w, y[j][c], acc[c]);
+      }
     }
   }
   store4(static_cast<T*>(a.out) + ((long long)q_row * a.H + head) * HD + 4 * lane, acc);
